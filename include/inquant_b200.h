@@ -435,6 +435,39 @@ int inq_decode_launch_shape(int32_t n_pairs, int64_t total_units, int32_t block_
 int inq_decode_launch_shape_uniform(int32_t n_pairs, int64_t pair_units, int32_t block_tokens, int32_t n_pad, int32_t value_kind,
                                     int32_t value_groups, int32_t ctas_per_sm, inq_decode_shape_t* shape);
 
+/* ---------------------------------------------------------------- prompts of several requests
+ * Causal attention of packed sequences and the attention weight their keys received.  Sequence b owns
+ * query rows cu_q[b] .. cu_q[b + 1] and key / value rows cu_k[b] .. cu_k[b + 1] (device int32 [n_seq + 1],
+ * not falling); its last query sits at its last key.  Offsets outside the tensors are cut to them and set
+ * INQ_STATUS_BAD_INDEX.  Rows of no sequence are not written, a query without a key gives zeros and -infinity.
+ * Strides are in elements, rows start on 16 bytes, head_dim is 64 or 128, dtype INQ_F16 or INQ_BF16. */
+typedef struct {
+  const void *q, *k, *v;      /* [rows, heads, head_dim] */
+  void* out;                  /* [q_rows, q_heads, head_dim] */
+  float* lse;                 /* [q_heads, q_rows], natural logarithm: written by inq_prompt_attention (or NULL),
+                               * read by inq_prompt_weights */
+  float* weights;             /* [kv_heads, k_rows]: written by inq_prompt_weights */
+  int64_t q_stride_t, q_stride_h, k_stride_t, k_stride_h, v_stride_t, v_stride_h, o_stride_t, o_stride_h;
+  int64_t lse_stride, weights_stride;       /* between heads */
+  const int32_t *cu_q, *cu_k;
+  int64_t q_rows, k_rows;
+  int32_t n_seq, q_heads, kv_heads, head_dim, dtype;
+  int32_t window;             /* inq_prompt_weights: the last `window` queries of a sequence count, 0 = all */
+  float scale;
+  int32_t reserved;
+  int32_t* status;
+  void* workspace;            /* scratch of one launch at a time, or NULL (items are then not cut) */
+  int64_t workspace_bytes;
+} inq_prompt_args_t;
+int inq_prompt_attention(const inq_prompt_args_t* args /* host */, inq_stream_t stream);
+/* weights[h][j] = sum over the query heads of KV head h and the counted queries i that see key j of
+ * exp(scale * q_i k_j - lse_i) */
+int inq_prompt_weights(const inq_prompt_args_t* args /* host */, inq_stream_t stream);
+/* Scratch with which inq_prompt_attention (weights = 0) or inq_prompt_weights (weights = 1) cuts its items as it would
+ * on the current device; 0 where it does not cut. */
+int64_t inq_prompt_workspace_bytes(int32_t q_heads, int32_t kv_heads, int32_t head_dim, int64_t q_rows, int64_t k_rows, int32_t n_seq,
+                                   int32_t weights, int32_t window);
+
 /* ---------------------------------------------------------------- incremental append
  * Writes the key and value rows of ONE new token (all KV heads) at `tail_position` of the
  * exact recent tail and, while the attention sink is still filling (sink_position >= 0),

@@ -19,6 +19,7 @@ SOURCES = {
     "decode.cu": [],
     "append.cu": [],
     "prefill.cu": [],
+    "prompt.cu": [],
     "decode_generic.cu": [],
     "exchange.cu": [],
     "pages.cu": [],

@@ -33,13 +33,10 @@
 // Shared-memory operand tiles hold 128 rows of 128 2-byte elements as two slabs of 64 columns;
 // inside a slab a row is 128 bytes and its 16-byte chunks are XOR-swizzled with the row index
 // modulo 8 (the 128-byte swizzle of the tensor-core descriptors).
-#include <cuda.h>
-
 #include <algorithm>
 #include <atomic>
-#include <type_traits>
 
-#include "tcgen05.cuh"
+#include "attention.cuh"
 
 namespace inq {
 
@@ -68,53 +65,6 @@ struct PrefillParams {
   float scale_log2e;
   int* status;
 };
-
-__device__ __forceinline__ void pf_arrive(unsigned mbar) {
-  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(mbar) : "memory");
-}
-__device__ __forceinline__ float pf_exp2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-// two fp32 values in one 64-bit register, for the packed units
-__device__ __forceinline__ unsigned long long pf_pair(float lo, float hi) {
-  unsigned long long d;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "f"(lo), "f"(hi));
-  return d;
-}
-__device__ __forceinline__ void pf_unpair(unsigned long long d, float& lo, float& hi) {
-  asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(d));
-}
-__device__ __forceinline__ unsigned long long pf_fma2(unsigned long long a, unsigned long long b, unsigned long long c) {
-  unsigned long long d;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
-  return d;
-}
-__device__ __forceinline__ unsigned long long pf_add2(unsigned long long a, unsigned long long b) {
-  unsigned long long d;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
-  return d;
-}
-template <typename QT>
-__device__ __forceinline__ unsigned pf_pack2(float lo, float hi) {
-  if (std::is_same<QT, __half>::value) {
-    __half2 h = __floats2half2_rn(lo, hi);
-    return *reinterpret_cast<unsigned*>(&h);
-  }
-  __nv_bfloat162 b = __floats2bfloat162_rn(lo, hi);
-  return *reinterpret_cast<unsigned*>(&b);
-}
-
-// One TMA box: 64 columns (128 bytes) x `rows` rows of head `z`, starting at column x and row y, into
-// a swizzled slab; rows beyond the tensor are zero-filled by the hardware.
-__device__ __forceinline__ void pf_tma(unsigned dst, const CUtensorMap* map, int x, int y, int z, unsigned mbar) {
-  asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
-               ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(z), "r"(mbar) : "memory");
-}
-__device__ __forceinline__ void pf_expect(unsigned mbar, unsigned bytes) {
-  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(mbar), "r"(bytes) : "memory");
-}
 
 template <typename QT>
 __global__ void __launch_bounds__(kPfThreads, 1) prefill_kernel(const PrefillParams P, const __grid_constant__ CUtensorMap map_q,
@@ -508,34 +458,6 @@ __global__ void __launch_bounds__(kPfMergeRows * 32) prefill_merge_kernel(const 
 using namespace inq;
 
 namespace {
-typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
-                                  const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
-                                  CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-EncodeTiledFn encode_tiled() {
-  static EncodeTiledFn fn = nullptr;
-  if (!fn) {
-    void* p = nullptr;
-    cudaDriverEntryPointQueryResult result;
-    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &result) == cudaSuccess &&
-        result == cudaDriverEntryPointSuccess)
-      fn = (EncodeTiledFn)p;
-  }
-  return fn;
-}
-// [heads][tokens][128] tensor of 2-byte elements, boxes of 64 columns x `box_rows` rows, 128-byte swizzle
-bool make_map(CUtensorMap* map, const void* base, int dtype, long long tokens, long long heads, long long stride_t,
-              long long stride_h, int box_rows) {
-  EncodeTiledFn fn = encode_tiled();
-  if (!fn) return false;
-  if (heads == 1) stride_h = tokens * stride_t;   // unused, but must be a valid stride
-  const cuuint64_t dims[3] = {128, (cuuint64_t)tokens, (cuuint64_t)heads};
-  const cuuint64_t strides[2] = {(cuuint64_t)stride_t * 2, (cuuint64_t)stride_h * 2};
-  const cuuint32_t box[3] = {64, (cuuint32_t)box_rows, 1};
-  const cuuint32_t elem[3] = {1, 1, 1};
-  return fn(map, dtype == INQ_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, (void*)base, dims,
-            strides, box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
-}
 // The shares that setmaxnreg hands out must not exceed what the kernel is launched with.  The library holds one
 // binary of the kernel for one architecture, so a yes is kept for the process; a query that fails is
 // reported like every other runtime error and asked again by the next call.
@@ -618,9 +540,9 @@ extern "C" int inq_prefill_attention(const inq_prefill_args_t* a, inq_stream_t s
       a->v_stride_t < 128)
     return INQ_ERR_ARGUMENT;
   CUtensorMap map_q, map_k, map_v;
-  if (!make_map(&map_q, a->q, a->dtype, a->q_tokens, a->q_heads, a->q_stride_t, a->q_stride_h, kPfTile) ||
-      !make_map(&map_k, a->k, a->dtype, a->kv_tokens, a->kv_heads, a->k_stride_t, a->k_stride_h, kPfTile) ||
-      !make_map(&map_v, a->v, a->dtype, a->kv_tokens, a->kv_heads, a->v_stride_t, a->v_stride_h, kPfTile))
+  if (!make_map(&map_q, a->q, a->dtype, 128, a->q_tokens, a->q_heads, a->q_stride_t, a->q_stride_h, kPfTile) ||
+      !make_map(&map_k, a->k, a->dtype, 128, a->kv_tokens, a->kv_heads, a->k_stride_t, a->k_stride_h, kPfTile) ||
+      !make_map(&map_v, a->v, a->dtype, 128, a->kv_tokens, a->kv_heads, a->v_stride_t, a->v_stride_h, kPfTile))
     return INQ_ERR_ARGUMENT;
   const int fit = a->dtype == INQ_F16 ? registers_fit<__half>() : registers_fit<__nv_bfloat16>();
   if (fit != INQ_OK) return fit;

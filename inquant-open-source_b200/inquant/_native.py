@@ -148,6 +148,16 @@ class PrefillArgs(ctypes.Structure):
                 ("workspace", c_void_p), ("workspace_bytes", c_int64)]
 
 
+class PromptArgs(ctypes.Structure):
+    _fields_ = [("q", c_void_p), ("k", c_void_p), ("v", c_void_p), ("out", c_void_p), ("lse", c_void_p), ("weights", c_void_p),
+                ("q_stride_t", c_int64), ("q_stride_h", c_int64), ("k_stride_t", c_int64), ("k_stride_h", c_int64),
+                ("v_stride_t", c_int64), ("v_stride_h", c_int64), ("o_stride_t", c_int64), ("o_stride_h", c_int64),
+                ("lse_stride", c_int64), ("weights_stride", c_int64), ("cu_q", c_void_p), ("cu_k", c_void_p),
+                ("q_rows", c_int64), ("k_rows", c_int64), ("n_seq", c_int32), ("q_heads", c_int32), ("kv_heads", c_int32),
+                ("head_dim", c_int32), ("dtype", c_int32), ("window", c_int32), ("scale", ctypes.c_float), ("reserved", c_int32),
+                ("status", c_void_p), ("workspace", c_void_p), ("workspace_bytes", c_int64)]
+
+
 class ExchangeRank(ctypes.Structure):
     _fields_ = [("local", c_void_p), ("inboxes", ctypes.POINTER(c_void_p)), ("out", c_void_p),
                 ("epoch", c_void_p), ("status", c_void_p), ("rank", c_int32)]
@@ -179,6 +189,8 @@ def library() -> ctypes.CDLL:
         lib.inq_decode_generic_workspace_floats.argtypes = [c_int32, c_int32, c_int32, c_int32, c_int32]
         lib.inq_prefill_workspace_bytes.restype = c_int64
         lib.inq_prefill_workspace_bytes.argtypes = [c_int32, c_int32]
+        lib.inq_prompt_workspace_bytes.restype = c_int64
+        lib.inq_prompt_workspace_bytes.argtypes = [c_int32, c_int32, c_int32, c_int64, c_int64, c_int32, c_int32, c_int32]
         lib.inq_exchange_inbox_bytes.restype = c_int64
         lib.inq_exchange_inbox_bytes.argtypes = [c_int32, c_int64]
         lib.inq_decode_exchange_inbox_bytes.restype = c_int64
@@ -238,7 +250,7 @@ EXPORTS = (
     "inq_build_roles", "inq_write_codec_pages",
     "inq_decode_attention", "inq_decode_attention_noalloc", "inq_decode_units", "inq_merge_partials", "inq_decode_workspace_floats", "inq_decode_launch_shape", "inq_decode_launch_shape_uniform", "inq_append_token", "inq_append_token_batch", "inq_seal_blocks", "inq_restore_history",
     "inq_prefill_attention", "inq_decode_generic", "inq_decode_generic_workspace_floats",
-    "inq_prefill_workspace_bytes",
+    "inq_prefill_workspace_bytes", "inq_prompt_attention", "inq_prompt_weights", "inq_prompt_workspace_bytes",
     "inq_exchange_merge", "inq_exchange_inbox_bytes", "inq_decode_exchange_inbox_bytes", "inq_restore_blocks_table", "inq_peer_buffer_create", "inq_peer_buffer_open",
     "inq_peer_buffer_close", "inq_peer_buffer_destroy",
 )
@@ -264,6 +276,8 @@ SIGNATURES = {
     "inq_merge_partials": [_P, _I, _L, _P, _I, _P],
     "inq_prefill_attention": [_P, _P],
     "inq_decode_generic": [_P, _P],
+    "inq_prompt_attention": [_P, _P],
+    "inq_prompt_weights": [_P, _P],
     "inq_exchange_merge": [_P, _P],
     "inq_peer_buffer_create": [_L, _P, _P],
     "inq_peer_buffer_open": [_P, _P],
