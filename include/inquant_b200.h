@@ -468,6 +468,70 @@ int inq_prompt_weights(const inq_prompt_args_t* args /* host */, inq_stream_t st
 int64_t inq_prompt_workspace_bytes(int32_t q_heads, int32_t kv_heads, int32_t head_dim, int64_t q_rows, int64_t k_rows, int32_t n_seq,
                                    int32_t weights, int32_t window);
 
+/* ---------------------------------------------------------------- uncompressed pages: decode
+ * Attention of one new token per request over a paged cache of 16-bit keys and values.  Token t of request b
+ * lies in page table[b][t / page_tokens], at offset t % page_tokens; the pages' strides are free (rows of unit
+ * channel stride that start on 16 bytes).  lengths[b] tokens are cached; with new_k / new_v the request's new row is stored
+ * behind them (lengths is not changed: the layers of a model share it) and attended to.  A negative length marks an
+ * unused row: zeros, nothing stored; zeros also where nothing is cached.  A page id outside the pool is never used as an
+ * address: its tokens are left out and INQ_STATUS_BAD_INDEX is set, as it is for a length that the table cannot hold.
+ * With out_weights, fp32 [requests, kv_heads, >= table_columns * page_tokens]:
+ *   out_weights[b][h][t] = weights[b][h][t] (0 for the new token and where weights is NULL)
+ *                          + sum of the attention weights of token t over the query heads of h
+ * for every token attended to; out_weights may be weights.  Strides are in elements. */
+typedef struct {
+  const void* q;                  /* [requests, q_heads, head_dim] */
+  void *k, *v;                    /* [pages, kv_heads, page_tokens, head_dim] */
+  const void *new_k, *new_v;      /* [requests, kv_heads, head_dim], or NULL */
+  void* out;                      /* [requests, q_heads, head_dim] */
+  const float* weights;
+  float* out_weights;
+  int64_t q_stride_b, q_stride_h, o_stride_b, o_stride_h;
+  int64_t k_stride_p, k_stride_h, k_stride_t, v_stride_p, v_stride_h, v_stride_t;
+  int64_t new_k_stride_b, new_k_stride_h, new_v_stride_b, new_v_stride_h;
+  int64_t w_stride_b, w_stride_h, ow_stride_b, ow_stride_h;
+  const int32_t* table;           /* [requests, table_columns] */
+  const int32_t* lengths;         /* [requests] */
+  int64_t table_stride, pages;
+  int32_t requests, q_heads, kv_heads, head_dim, page_tokens, table_columns, dtype;
+  float scale;
+  int32_t* status;
+  void* workspace;                /* scratch of one call at a time */
+  int64_t workspace_bytes;
+} inq_paged_attention_args_t;
+int inq_paged_attention(const inq_paged_attention_args_t* args /* host */, inq_stream_t stream);
+/* Scratch of such a call on the current device (reads the counts, head_dim and out_weights alone). */
+int64_t inq_paged_attention_workspace_bytes(const inq_paged_attention_args_t* args /* host */);
+
+/* ---------------------------------------------------------------- uncompressed pages: eviction
+ * Keeps, per request with more than `budget` cached tokens and per KV head, the `budget` tokens of most worth: first
+ * those with positions[b][h][t] < sink or >= seen[b] - recent, then by falling weights[b][h][t] (NaN last, ties: the lowest
+ * t).  A kept token t >= budget moves into a place that falls free in front of the budget, the i-th such token into
+ * the i-th free place: its rows of k and v, its weight and its position.  out_weights and out_positions [.., budget] get
+ * the state of the places (0 and -1 where no token is), out_lengths min(lengths, budget); each may be its input.
+ * The pages of a request that evicts belong to it alone.  sink + recent <= budget.  A page id outside the pool is not
+ * used and sets INQ_STATUS_BAD_INDEX, as does a length beyond the table or `columns`, which counts as that. */
+typedef struct {
+  void *k, *v;                    /* [pages, kv_heads, page_tokens, head_dim], 16-bit elements */
+  int64_t k_stride_p, k_stride_h, k_stride_t, v_stride_p, v_stride_h, v_stride_t;
+  const int32_t* table;           /* [requests, table_columns] */
+  const int32_t* lengths;         /* [requests] */
+  const int32_t* seen;            /* [requests]: tokens that the request has had, the evicted ones among them */
+  const float* weights;           /* [requests, kv_heads, columns] */
+  const int32_t* positions;
+  float* out_weights;
+  int32_t *out_positions, *out_lengths;
+  int64_t table_stride, w_stride_b, w_stride_h, p_stride_b, p_stride_h, ow_stride_b, ow_stride_h, op_stride_b, op_stride_h;
+  int64_t pages, columns;
+  int32_t requests, kv_heads, head_dim, page_tokens, table_columns, budget, sink, recent;
+  int32_t* status;
+  void* workspace;                /* scratch of one call at a time */
+  int64_t workspace_bytes;
+} inq_evict_args_t;
+int inq_evict_tokens(const inq_evict_args_t* args /* host */, inq_stream_t stream);
+/* capacity: table_columns * page_tokens */
+int64_t inq_evict_workspace_bytes(int32_t requests, int32_t kv_heads, int32_t budget, int64_t capacity);
+
 /* ---------------------------------------------------------------- incremental append
  * Writes the key and value rows of ONE new token (all KV heads) at `tail_position` of the
  * exact recent tail and, while the attention sink is still filling (sink_position >= 0),

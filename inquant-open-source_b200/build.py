@@ -20,6 +20,8 @@ SOURCES = {
     "append.cu": [],
     "prefill.cu": [],
     "prompt.cu": [],
+    "dense_paged.cu": [],
+    "evict.cu": [],
     "decode_generic.cu": [],
     "exchange.cu": [],
     "pages.cu": [],

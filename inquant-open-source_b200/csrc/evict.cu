@@ -1,0 +1,317 @@
+// Eviction from an uncompressed paged cache by accumulated attention weight.
+//
+// Per request and KV head the `budget` tokens of most worth stay: those whose position is below `sink` or among the
+// last `recent` that were seen, whatever their weight, then by falling weight (ties: the lowest place).  The kept tokens
+// behind the budget move into the places that fall free in front of it, both in rising order; the others stay where
+// they are.  So a step that evicts a few tokens of many moves few rows, no row is both read and written, and attention,
+// for which the order of tokens in the cache means nothing, goes on as before.
+//
+// evict_select_kernel finds the worth of the last token that stays by a radix select over 32-bit keys (digits of 11, 11
+// and 10 bits, histograms in shared memory): one cluster per row (request, KV head), each CTA with a slice of it, the
+// histograms added over distributed shared memory.  It writes the lists of free places and of tokens that move.
+// evict_move_kernel moves the rows of K and V: 4 D elements read and written per token, which is what bounds it.
+#include <cooperative_groups.h>
+
+#include <algorithm>
+
+#include "common.cuh"
+
+namespace cg = cooperative_groups;
+
+namespace inq {
+
+constexpr int kEvThreads = 512, kEvBins = 2048, kEvMaxCluster = 8, kEvPerThread = 8;
+
+struct EvictParams {
+  void *k, *v;
+  long long k_sp, k_sh, k_st, v_sp, v_sh, v_st;
+  const int *table, *lengths, *seen, *positions;
+  const float* weights;
+  int *out_positions, *out_lengths;
+  float* out_weights;
+  long long table_stride, w_sb, w_sh, p_sb, p_sh, ow_sb, ow_sh, op_sb, op_sh;
+  long long pages, capacity;
+  int requests, kv_heads, page_tokens, page_shift, budget, sink, recent, row_bytes;
+  long long list_columns;
+  int* lists;          // per row: count, then up to list_columns free places, then as many tokens that move
+  int* status;
+};
+
+// Rises with the worth of a token; a NaN is worth less than anything.
+__device__ __forceinline__ unsigned worth(float w) {
+  if (w != w) return 0u;
+  const unsigned u = __float_as_uint(w + 0.f);          // -0 counts as 0
+  return (u & 0x80000000u) ? ~u : u | 0x80000000u;
+}
+
+// Sum over the threads in front of this one, and over all of them.
+__device__ __forceinline__ int block_prefix(int mine, int& all, int* scratch /* 17 ints */) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  int sum = mine;
+#pragma unroll
+  for (int d = 1; d < 32; d <<= 1) {
+    const int other = __shfl_up_sync(0xffffffffu, sum, d);
+    if (lane >= d) sum += other;
+  }
+  __syncthreads();
+  if (lane == 31) scratch[warp] = sum;
+  __syncthreads();
+  int before = 0;
+  all = 0;
+#pragma unroll
+  for (int w = 0; w < kEvThreads / 32; ++w) {
+    const int n = scratch[w];
+    if (w < warp) before += n;
+    all += n;
+  }
+  return before + sum - mine;
+}
+
+__global__ void __launch_bounds__(kEvThreads) evict_select_kernel(const EvictParams P) {
+  cg::cluster_group cluster = cg::this_cluster();
+  const int ctas = (int)cluster.num_blocks(), me = (int)cluster.block_rank();
+  const int row = blockIdx.x / ctas, b = row / P.kv_heads, h = row % P.kv_heads, tid = threadIdx.x;
+  __shared__ int histogram[kEvBins];
+  __shared__ int shared_counts[3];                    // this CTA's ties, free places and moving tokens
+  __shared__ int scratch[kEvThreads / 32 + 1], chosen[2];
+  follow_stream();
+  const long long asked = P.lengths[b];
+  const int length = (int)min(max(asked, 0LL), P.capacity), budget = P.budget;
+  if (asked > P.capacity && row % P.kv_heads == 0 && me == 0 && tid == 0) atomicOr(P.status, INQ_STATUS_BAD_INDEX);
+  const int left = min(length, budget);
+  const float* const w = P.weights + b * P.w_sb + h * P.w_sh;
+  const int* const pos = P.positions + b * P.p_sb + h * P.p_sh;
+  float* const out_w = P.out_weights + b * P.ow_sb + h * P.ow_sh;
+  int* const out_p = P.out_positions + b * P.op_sb + h * P.op_sh;
+  int* const list = P.lists + row * (2 * P.list_columns + 1);
+  // places that no token fills
+  for (int j = left + me * kEvThreads + tid; j < budget; j += ctas * kEvThreads) {
+    out_w[j] = 0.f;
+    out_p[j] = -1;
+  }
+  if (length <= budget) {       // the same in every CTA of the cluster
+    for (int j = me * kEvThreads + tid; j < left; j += ctas * kEvThreads) {
+      out_w[j] = w[j];
+      out_p[j] = pos[j];
+    }
+    if (me == 0 && tid == 0) list[0] = 0;
+    return;
+  }
+  const long long safe_from = (long long)P.seen[b] - P.recent;
+  const int slice = (length + ctas - 1) / ctas, lo = min(me * slice, length), hi = min(lo + slice, length);
+  auto key = [&](int j) {
+    const int p = pos[j];
+    return p < P.sink || p >= safe_from ? 0xffffffffu : worth(w[j]);
+  };
+
+  // ---- the key of the last token that stays: `want` tokens of those that begin with `prefix` are still to be found
+  unsigned prefix = 0;
+  int want = budget;
+#pragma unroll 1
+  for (int pass = 0; pass < 3; ++pass) {
+    const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, bins = pass == 2 ? 1024 : 2048;
+    for (int i = tid; i < kEvBins; i += kEvThreads) histogram[i] = 0;
+    __syncthreads();
+    for (int j = lo + tid; j < hi; j += kEvThreads) {
+      const unsigned k = key(j);
+      if (pass == 0 || (k >> (pass == 1 ? 21 : 10)) == prefix) atomicAdd(histogram + ((k >> shift) & (bins - 1)), 1);
+    }
+    cluster.sync();
+    // every CTA finds the digit for itself: a thread adds four neighbouring bins over the cluster, highest bins first
+    int mine[4], sum = 0, all;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int bin = kEvBins - 1 - (4 * tid + i);
+      mine[i] = 0;
+      for (int c = 0; c < ctas; ++c) mine[i] += cluster.map_shared_rank(histogram, c)[bin];
+      sum += mine[i];
+    }
+    int before = block_prefix(sum, all, scratch);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if (before < want && before + mine[i] >= want) {
+        chosen[0] = kEvBins - 1 - (4 * tid + i);
+        chosen[1] = want - before;
+      }
+      before += mine[i];
+    }
+    __syncthreads();
+    prefix = (prefix << (pass == 2 ? 10 : 11)) | (unsigned)chosen[0];
+    want = chosen[1];
+    if (pass == 2 && tid == 0) shared_counts[0] = histogram[chosen[0]];
+    cluster.sync();       // nobody reads this CTA's histogram any more
+  }
+  // tokens above the threshold stay, and the first `want` of those at it
+  int ties_before = 0;
+  for (int c = 0; c < me; ++c) ties_before += cluster.map_shared_rank(shared_counts, c)[0];
+
+  // ---- twice over the slice: the free places and moving tokens of this CTA, then their lists
+  int holes = 0, moves = 0;          // in front of the group of tokens in work
+#pragma unroll 1
+  for (int round = 0; round < 2; ++round) {
+    int ties = ties_before;
+    if (round == 1) {
+      cluster.sync();
+      holes = moves = 0;
+      for (int c = 0; c < me; ++c) {
+        holes += cluster.map_shared_rank(shared_counts, c)[1];
+        moves += cluster.map_shared_rank(shared_counts, c)[2];
+      }
+    }
+#pragma unroll 1
+    for (int j0 = lo; j0 < hi; j0 += kEvThreads * kEvPerThread) {
+      unsigned keys[kEvPerThread];
+      int equal = 0, all_equal;
+#pragma unroll
+      for (int i = 0; i < kEvPerThread; ++i) {
+        const int j = j0 + tid * kEvPerThread + i;
+        keys[i] = j < hi ? key(j) : 0u;
+        equal += j < hi && keys[i] == prefix;
+      }
+      int rank = ties + block_prefix(equal, all_equal, scratch);
+      ties += all_equal;
+      unsigned kept = 0;
+      int mine_holes = 0, mine_moves = 0;
+#pragma unroll
+      for (int i = 0; i < kEvPerThread; ++i) {
+        const int j = j0 + tid * kEvPerThread + i;
+        if (j >= hi) continue;
+        const bool tie = keys[i] == prefix;
+        const bool stays = keys[i] > prefix || (tie && rank < want);
+        rank += tie;
+        kept |= (unsigned)stays << i;
+        mine_holes += !stays && j < left;
+        mine_moves += stays && j >= left;
+      }
+      int all_packed;
+      int packed = block_prefix(mine_holes | (mine_moves << 16), all_packed, scratch);
+      if (round == 1) {
+        int hole = holes + (packed & 0xffff), move = moves + (packed >> 16);
+#pragma unroll
+        for (int i = 0; i < kEvPerThread; ++i) {
+          const int j = j0 + tid * kEvPerThread + i;
+          if (j >= hi) continue;
+          const bool stays = (kept >> i) & 1u;
+          if (j < left) {
+            if (stays) {
+              out_w[j] = w[j];
+              out_p[j] = pos[j];
+            } else {
+              list[1 + hole++] = j;
+            }
+          } else if (stays) {
+            list[1 + P.list_columns + move++] = j;
+          }
+        }
+      }
+      holes += all_packed & 0xffff;
+      moves += all_packed >> 16;
+    }
+    if (round == 0) {
+      __syncthreads();
+      if (tid == 0) {
+        shared_counts[1] = holes;
+        shared_counts[2] = moves;
+      }
+    }
+  }
+  if (me == ctas - 1 && tid == 0) list[0] = moves;
+  cluster.sync();       // the counts of a CTA are read until here
+}
+
+// A warp moves one token: half of its lanes the key row, the others the value row, 16 bytes each.
+constexpr int kEvMoveThreads = 256, kEvMoveTokens = 64;      // tokens of a block
+__global__ void __launch_bounds__(kEvMoveThreads) evict_move_kernel(const EvictParams P) {
+  follow_stream();
+  const int row = blockIdx.x, b = row / P.kv_heads, h = row % P.kv_heads, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int* const list = P.lists + row * (2 * P.list_columns + 1);
+  if (blockIdx.y == 0 && h == 0 && threadIdx.x == 0) P.out_lengths[b] = min(P.lengths[b], P.budget);
+  const int count = list[0];
+  auto address = [&](int j, bool& fine) {
+    const int column = P.page_shift >= 0 ? j >> P.page_shift : j / P.page_tokens;
+    const int page = __ldg(P.table + b * P.table_stride + column), o = j - column * P.page_tokens;
+    fine = page >= 0 && page < P.pages;
+    return lane < 16 ? (char*)P.k + 2 * (page * P.k_sp + h * P.k_sh + o * P.k_st) : (char*)P.v + 2 * (page * P.v_sp + h * P.v_sh + o * P.v_st);
+  };
+  for (int i = blockIdx.y * kEvMoveTokens + warp; i < min(count, (int)(blockIdx.y + 1) * kEvMoveTokens); i += kEvMoveThreads / 32) {
+    const int to = list[1 + i], from = list[1 + P.list_columns + i];
+    bool to_fine, from_fine;
+    char* const dst = address(to, to_fine);
+    const char* const src = address(from, from_fine);
+    if (to_fine && from_fine) {
+      const int at = (lane & 15) * 16;
+      if (at < P.row_bytes) *(uint4*)(dst + at) = *(const uint4*)(src + at);
+    } else if (lane == 0) {
+      atomicOr(P.status, INQ_STATUS_BAD_INDEX);
+    }
+    if (lane == 0) {
+      P.out_weights[b * P.ow_sb + h * P.ow_sh + to] = P.weights[b * P.w_sb + h * P.w_sh + from];
+      P.out_positions[b * P.op_sb + h * P.op_sh + to] = P.positions[b * P.p_sb + h * P.p_sh + from];
+    }
+  }
+}
+
+}  // namespace inq
+
+using namespace inq;
+
+extern "C" int64_t inq_evict_workspace_bytes(int32_t requests, int32_t kv_heads, int32_t budget, int64_t capacity) {
+  return requests < 1 || kv_heads < 1 || budget < 1 || capacity < 1
+             ? 0 : (int64_t)requests * kv_heads * (2 * std::min<int64_t>(budget, capacity) + 1) * (int64_t)sizeof(int);
+}
+
+extern "C" int inq_evict_tokens(const inq_evict_args_t* a, inq_stream_t stream_) {
+  if (!a || !a->k || !a->v || !a->table || !a->lengths || !a->seen || !a->positions || !a->weights || !a->out_positions ||
+      !a->out_lengths || !a->out_weights || !a->status)
+    return INQ_ERR_ARGUMENT;
+  if (a->requests < 1 || a->kv_heads < 1 || a->pages < 1 || a->page_tokens < 1 || a->table_columns < 1) return INQ_ERR_ARGUMENT;
+  if (a->budget < 1 || a->sink < 0 || a->recent < 0 || (long long)a->sink + a->recent > a->budget) return INQ_ERR_ARGUMENT;
+  if (a->head_dim < 8 || a->head_dim > 128 || a->head_dim % 8) return INQ_ERR_UNSUPPORTED;
+  if ((a->k_stride_p | a->k_stride_h | a->k_stride_t | a->v_stride_p | a->v_stride_h | a->v_stride_t) & 7) return INQ_ERR_ARGUMENT;
+  if (((uintptr_t)a->k | (uintptr_t)a->v) & 15) return INQ_ERR_ARGUMENT;
+  const long long capacity = (long long)a->table_columns * a->page_tokens, rows = (long long)a->requests * a->kv_heads;
+  if (capacity > 0x3fffffffLL || a->budget > 0x3fffffff || rows * kEvMaxCluster > 0x7fffffffLL) return INQ_ERR_CAPACITY;
+  if (!a->workspace || a->workspace_bytes < inq_evict_workspace_bytes(a->requests, a->kv_heads, a->budget, capacity)) return INQ_ERR_CAPACITY;
+  int device = 0, n_sm = 0;
+  INQ_CUDA_CHECK(cudaGetDevice(&device));
+  INQ_CUDA_CHECK(cudaDeviceGetAttribute(&n_sm, cudaDevAttrMultiProcessorCount, device));
+  EvictParams P = {};
+  P.k = a->k; P.v = a->v;
+  P.k_sp = a->k_stride_p; P.k_sh = a->k_stride_h; P.k_st = a->k_stride_t;
+  P.v_sp = a->v_stride_p; P.v_sh = a->v_stride_h; P.v_st = a->v_stride_t;
+  P.table = a->table; P.lengths = a->lengths; P.seen = a->seen; P.positions = a->positions; P.weights = a->weights;
+  P.out_positions = a->out_positions; P.out_lengths = a->out_lengths; P.out_weights = a->out_weights;
+  P.table_stride = a->table_stride; P.w_sb = a->w_stride_b; P.w_sh = a->w_stride_h; P.p_sb = a->p_stride_b; P.p_sh = a->p_stride_h;
+  P.ow_sb = a->ow_stride_b; P.ow_sh = a->ow_stride_h; P.op_sb = a->op_stride_b; P.op_sh = a->op_stride_h;
+  P.pages = a->pages; P.capacity = std::min<long long>(capacity, a->columns);
+  P.requests = a->requests; P.kv_heads = a->kv_heads; P.page_tokens = a->page_tokens;
+  P.page_shift = -1;
+  for (int i = 0; i < 30; ++i)
+    if (a->page_tokens == 1 << i) P.page_shift = i;
+  P.list_columns = std::min<long long>(a->budget, capacity);
+  P.budget = a->budget; P.sink = a->sink; P.recent = a->recent; P.row_bytes = 2 * a->head_dim;
+  P.lists = (int*)a->workspace; P.status = a->status;
+  // slices of a row: while they fill the SMs and hold 2048 tokens at least
+  int ctas = 1;
+  while (ctas < kEvMaxCluster && rows * ctas * 2 <= 2 * n_sm && P.capacity / (2 * ctas) >= 2048) ctas *= 2;
+  cudaStream_t stream = (cudaStream_t)stream_;
+  {
+    cudaLaunchAttribute attrs[2];
+    attrs[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attrs[0].val.programmaticStreamSerializationAllowed = 1;
+    attrs[1].id = cudaLaunchAttributeClusterDimension;
+    attrs[1].val.clusterDim.x = ctas;
+    attrs[1].val.clusterDim.y = attrs[1].val.clusterDim.z = 1;
+    cudaLaunchConfig_t config = {};
+    config.gridDim = dim3((unsigned)(rows * ctas));
+    config.blockDim = dim3(kEvThreads);
+    config.stream = stream;
+    config.attrs = attrs;
+    config.numAttrs = 2;
+    INQ_CUDA_CHECK(cudaLaunchKernelEx(&config, evict_select_kernel, P));
+  }
+  const unsigned blocks = (unsigned)((std::min<long long>(P.budget, P.capacity) + kEvMoveTokens - 1) / kEvMoveTokens);
+  if (blocks > 65535) return INQ_ERR_CAPACITY;
+  INQ_CUDA_CHECK(launch_following(evict_move_kernel, dim3((unsigned)rows, blocks), kEvMoveThreads, 0, stream, P));
+  return INQ_OK;
+}

@@ -158,6 +158,32 @@ class PromptArgs(ctypes.Structure):
                 ("status", c_void_p), ("workspace", c_void_p), ("workspace_bytes", c_int64)]
 
 
+class PagedAttentionArgs(ctypes.Structure):
+    _fields_ = [("q", c_void_p), ("k", c_void_p), ("v", c_void_p), ("new_k", c_void_p), ("new_v", c_void_p), ("out", c_void_p),
+                ("weights", c_void_p), ("out_weights", c_void_p),
+                ("q_stride_b", c_int64), ("q_stride_h", c_int64), ("o_stride_b", c_int64), ("o_stride_h", c_int64),
+                ("k_stride_p", c_int64), ("k_stride_h", c_int64), ("k_stride_t", c_int64),
+                ("v_stride_p", c_int64), ("v_stride_h", c_int64), ("v_stride_t", c_int64),
+                ("new_k_stride_b", c_int64), ("new_k_stride_h", c_int64), ("new_v_stride_b", c_int64), ("new_v_stride_h", c_int64),
+                ("w_stride_b", c_int64), ("w_stride_h", c_int64), ("ow_stride_b", c_int64), ("ow_stride_h", c_int64),
+                ("table", c_void_p), ("lengths", c_void_p), ("table_stride", c_int64), ("pages", c_int64),
+                ("requests", c_int32), ("q_heads", c_int32), ("kv_heads", c_int32), ("head_dim", c_int32), ("page_tokens", c_int32),
+                ("table_columns", c_int32), ("dtype", c_int32), ("scale", ctypes.c_float), ("status", c_void_p),
+                ("workspace", c_void_p), ("workspace_bytes", c_int64)]
+
+
+class EvictArgs(ctypes.Structure):
+    _fields_ = [("k", c_void_p), ("v", c_void_p), ("k_stride_p", c_int64), ("k_stride_h", c_int64), ("k_stride_t", c_int64),
+                ("v_stride_p", c_int64), ("v_stride_h", c_int64), ("v_stride_t", c_int64),
+                ("table", c_void_p), ("lengths", c_void_p), ("seen", c_void_p), ("weights", c_void_p), ("positions", c_void_p),
+                ("out_weights", c_void_p), ("out_positions", c_void_p), ("out_lengths", c_void_p), ("table_stride", c_int64),
+                ("w_stride_b", c_int64), ("w_stride_h", c_int64), ("p_stride_b", c_int64), ("p_stride_h", c_int64),
+                ("ow_stride_b", c_int64), ("ow_stride_h", c_int64), ("op_stride_b", c_int64), ("op_stride_h", c_int64),
+                ("pages", c_int64), ("columns", c_int64), ("requests", c_int32), ("kv_heads", c_int32), ("head_dim", c_int32),
+                ("page_tokens", c_int32), ("table_columns", c_int32), ("budget", c_int32), ("sink", c_int32), ("recent", c_int32),
+                ("status", c_void_p), ("workspace", c_void_p), ("workspace_bytes", c_int64)]
+
+
 class ExchangeRank(ctypes.Structure):
     _fields_ = [("local", c_void_p), ("inboxes", ctypes.POINTER(c_void_p)), ("out", c_void_p),
                 ("epoch", c_void_p), ("status", c_void_p), ("rank", c_int32)]
@@ -191,6 +217,10 @@ def library() -> ctypes.CDLL:
         lib.inq_prefill_workspace_bytes.argtypes = [c_int32, c_int32]
         lib.inq_prompt_workspace_bytes.restype = c_int64
         lib.inq_prompt_workspace_bytes.argtypes = [c_int32, c_int32, c_int32, c_int64, c_int64, c_int32, c_int32, c_int32]
+        lib.inq_paged_attention_workspace_bytes.restype = c_int64
+        lib.inq_paged_attention_workspace_bytes.argtypes = [c_void_p]
+        lib.inq_evict_workspace_bytes.restype = c_int64
+        lib.inq_evict_workspace_bytes.argtypes = [c_int32, c_int32, c_int32, c_int64]
         lib.inq_exchange_inbox_bytes.restype = c_int64
         lib.inq_exchange_inbox_bytes.argtypes = [c_int32, c_int64]
         lib.inq_decode_exchange_inbox_bytes.restype = c_int64
@@ -251,6 +281,7 @@ EXPORTS = (
     "inq_decode_attention", "inq_decode_attention_noalloc", "inq_decode_units", "inq_merge_partials", "inq_decode_workspace_floats", "inq_decode_launch_shape", "inq_decode_launch_shape_uniform", "inq_append_token", "inq_append_token_batch", "inq_seal_blocks", "inq_restore_history",
     "inq_prefill_attention", "inq_decode_generic", "inq_decode_generic_workspace_floats",
     "inq_prefill_workspace_bytes", "inq_prompt_attention", "inq_prompt_weights", "inq_prompt_workspace_bytes",
+    "inq_paged_attention", "inq_paged_attention_workspace_bytes", "inq_evict_tokens", "inq_evict_workspace_bytes",
     "inq_exchange_merge", "inq_exchange_inbox_bytes", "inq_decode_exchange_inbox_bytes", "inq_restore_blocks_table", "inq_peer_buffer_create", "inq_peer_buffer_open",
     "inq_peer_buffer_close", "inq_peer_buffer_destroy",
 )
@@ -276,6 +307,8 @@ SIGNATURES = {
     "inq_merge_partials": [_P, _I, _L, _P, _I, _P],
     "inq_prefill_attention": [_P, _P],
     "inq_decode_generic": [_P, _P],
+    "inq_paged_attention": [_P, _P],
+    "inq_evict_tokens": [_P, _P],
     "inq_prompt_attention": [_P, _P],
     "inq_prompt_weights": [_P, _P],
     "inq_exchange_merge": [_P, _P],

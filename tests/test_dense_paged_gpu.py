@@ -1,0 +1,372 @@
+"""Decode over uncompressed pages and eviction (``inquant.dense_paged``) against their formulas in 64 bits.
+
+Bounds.  u is half a step of the dtype.  A logit's fp32 error is at most delta = D 2^-24 scale sum |q_c k_c|, the relative
+error of its exponential; 2^-20 covers the exponential unit, the factors of the joins and fp32 sums in chains of a few
+hundred.  A probability is rounded to the dtype once (u) before the product with the values, its normaliser is
+not (2 delta for both), the result is rounded once: |out - exact| <= sum p |v| (u + 2 delta) + u |exact| (1 + u).  A
+weight is a sum of unrounded probabilities: 2 delta of it, and a step of the accumulated sum."""
+import math
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+
+
+def ints(values):
+    return torch.tensor(values, dtype=torch.int32, device=DEV)
+
+
+class Pool:
+    """A paged cache with the given lengths, its pages in random order and what no token fills not a number."""
+
+    def __init__(self, lengths, heads, dim, page, dtype, seed=0, spare=0, columns=None):
+        g = torch.Generator(device=DEV).manual_seed(seed)
+        self.lengths, self.page = lengths, page
+        need = [max(1, -(-(max(n, 0) + 1) // page)) for n in lengths]
+        self.columns = columns or max(need) + spare
+        ids = torch.randperm(sum(need) + 2, generator=g, device=DEV).to(torch.int32)
+        self.table = torch.full((len(lengths), self.columns), -5, dtype=torch.int32, device=DEV)     # unused entries are nobody's
+        self.keys = torch.full((sum(need) + 2, heads, page, dim), float("nan"), dtype=dtype, device=DEV)
+        self.values = self.keys.clone()
+        at = 0
+        for b, n in enumerate(need):
+            self.table[b, :n] = ids[at:at + n]
+            at += n
+            if lengths[b] > 0:
+                k, v = (torch.randn((lengths[b], heads, dim), generator=g, device=DEV).to(dtype) for _ in range(2))
+                self.put(b, torch.arange(lengths[b], device=DEV), k, v)
+        self.n = ints(lengths)
+
+    def places(self, b, tokens):
+        return self.table[b].long()[tokens // self.page], tokens % self.page
+
+    def put(self, b, tokens, k, v):
+        p, o = self.places(b, tokens)
+        self.keys[p, :, o], self.values[p, :, o] = k, v
+
+    def get(self, b, count):
+        p, o = self.places(b, torch.arange(count, device=DEV))
+        return self.keys[p, :, o], self.values[p, :, o]
+
+
+def check_token(pool, q, got, weights=None, old=None, fresh=None, scale=None, tokens=None):
+    """Compares output (and accumulated weights) with the formula over what the pool holds now."""
+    u, dim = torch.finfo(q.dtype).eps / 2, q.shape[2]
+    scale = dim ** -0.5 if scale is None else scale
+    heads, group = pool.keys.shape[1], q.shape[1] // pool.keys.shape[1]
+    for b, n in enumerate(tokens if tokens is not None else [max(n, 0) + (fresh is not None and n >= 0) for n in pool.lengths]):
+        if n == 0:
+            assert (got[b] == 0).all()
+            continue
+        k, v = (t.double().transpose(0, 1) for t in pool.get(b, n))
+        x = q[b].double().reshape(heads, group, dim)
+        logits = x @ k.transpose(1, 2) * scale
+        delta = dim * 2.0 ** -24 * scale * (x.abs() @ k.abs().transpose(1, 2)).amax(2, keepdim=True) + 2.0 ** -20
+        p = torch.softmax(logits, 2)
+        want, share = (p @ v).reshape(-1, dim), (p @ v.abs()).reshape(-1, dim)
+        allowed = share * (u + 2 * delta.reshape(-1, 1)) + u * want.abs() * (1 + u) + torch.finfo(q.dtype).smallest_normal
+        off = (got[b].double() - want).abs()
+        assert (off <= allowed).all(), (b, n, (off / allowed).max())
+        if weights is not None:
+            step = p.sum(1)
+            before = torch.zeros_like(step) if old is None else old[b, :, :n].double().clone()
+            if fresh is not None and old is not None:
+                before[:, n - 1] = 0
+            allowed = (p * 2 * delta).sum(1) + (group + 1) * 2.0 ** -24 * (step + before)
+            assert ((weights[b, :, :n].double() - step - before).abs() <= allowed).all()
+
+
+def query(requests, q_heads, dim, dtype, seed=7):
+    return torch.randn((requests, q_heads, dim), generator=torch.Generator(device=DEV).manual_seed(seed), device=DEV).to(dtype)
+
+
+SHAPES = [(28, 4, 128, torch.bfloat16), (12, 1, 128, torch.float16), (8, 8, 64, torch.float16), (40, 2, 64, torch.bfloat16),
+          (20, 1, 128, torch.bfloat16)]
+
+
+@pytest.mark.parametrize("q_heads,heads,dim,dtype", SHAPES)
+@pytest.mark.parametrize("page", [1, 16, 24, 256])
+@pytest.mark.parametrize("lengths", [[1], [15, 16, 17], [127, 128, 129, 0, 1], [700, -1, 2500, 3]])
+def test_tokens_over_pages(q_heads, heads, dim, dtype, page, lengths):
+    from inquant.dense_paged import paged_attention
+    pool = Pool(lengths, heads, dim, page, dtype)
+    q = query(len(lengths), q_heads, dim, dtype)
+    kept = pool.keys.clone(), pool.values.clone()
+    out = paged_attention(q, pool.keys, pool.values, pool.table, pool.n)
+    check_token(pool, q, out)
+    assert torch.equal(pool.keys.view(torch.int16), kept[0].view(torch.int16)) and torch.equal(pool.values.view(torch.int16), kept[1].view(torch.int16))
+
+
+@pytest.mark.parametrize("q_heads,heads,dim,dtype", SHAPES)
+@pytest.mark.parametrize("page", [16, 24, 64])
+@pytest.mark.parametrize("lengths", [[0], [0, 1, 127, 128], [-1, 300, 0, 1111]])
+def test_new_tokens_are_stored_and_weights_kept_up(q_heads, heads, dim, dtype, page, lengths):
+    from inquant.dense_paged import paged_attention
+    pool = Pool(lengths, heads, dim, page, dtype, seed=1, spare=1)
+    q = query(len(lengths), q_heads, dim, dtype)
+    new_k, new_v = query(len(lengths), heads, dim, dtype, 8), query(len(lengths), heads, dim, dtype, 9)
+    width = pool.columns * page
+    old = torch.rand((len(lengths), heads, width + 3), device=DEV)
+    before = pool.keys.clone()
+    into = torch.full((len(lengths), heads, width), 5.0, device=DEV)
+    out, w = paged_attention(q, pool.keys, pool.values, pool.table, pool.n, new_key=new_k, new_value=new_v, weights=old, out_weights=into)
+    assert w is into
+    for b, n in enumerate(lengths):
+        if n >= 0:
+            k, v = pool.get(b, n + 1)
+            assert torch.equal(k[n], new_k[b]) and torch.equal(v[n], new_v[b])
+            p, o = pool.places(b, torch.tensor([n], device=DEV))
+            before[p, :, o] = new_k[b]
+        assert (into[b, :, max(n + 1, 0):] == 5.0).all()
+    assert torch.equal(before.view(torch.int16), pool.keys.view(torch.int16))      # nothing else was written
+    check_token(pool, q, out, w, old, fresh=True)
+    # in place, and this step's weights alone
+    again = old.clone()
+    out2, w2 = paged_attention(q, pool.keys, pool.values, pool.table, pool.n, new_key=new_k, new_value=new_v, weights=again)
+    assert w2 is again and torch.equal(out2, out)
+    for b, n in enumerate(lengths):
+        assert torch.equal(again[b, :, :max(n + 1, 0)], into[b, :, :max(n + 1, 0)])
+    _, alone = paged_attention(q, pool.keys, pool.values, pool.table, pool.n, new_key=new_k, new_value=new_v, out_weights=into)
+    check_token(pool, q, out, alone, None, fresh=True)
+
+
+@pytest.mark.parametrize("lengths", [[40000], [1] * 300 + [5000], [0] * 40 + [130] * 40])
+def test_many_parts_and_many_requests(lengths):
+    from inquant.dense_paged import paged_attention
+    pool = Pool(lengths, 2, 128, 16, torch.bfloat16, seed=2)
+    q = query(len(lengths), 14, 128, torch.bfloat16)
+    weights = torch.zeros((len(lengths), 2, pool.columns * 16), device=DEV)
+    out, w = paged_attention(q, pool.keys, pool.values, pool.table, pool.n, out_weights=weights)
+    check_token(pool, q, out, w)
+    assert torch.equal(out, paged_attention(q, pool.keys, pool.values, pool.table, pool.n))
+
+
+def test_large_logits_and_rising_maxima():
+    from inquant.dense_paged import paged_attention
+    pool = Pool([3000], 2, 128, 16, torch.bfloat16, seed=3)
+    p, o = pool.places(0, torch.arange(3000, device=DEV))
+    pool.keys[p, :, o] *= torch.linspace(0.1, 8, 3000, device=DEV)[:, None, None].to(torch.bfloat16)
+    q = query(1, 8, 128, torch.bfloat16) * 2
+    check_token(pool, q, paged_attention(q, pool.keys, pool.values, pool.table, pool.n))
+
+
+def test_strides_of_pages_and_rows():
+    from inquant.dense_paged import paged_attention
+    lengths = [300, 77]
+    pool = Pool(lengths, 2, 128, 16, torch.bfloat16, seed=4)
+    q = query(2, 8, 128, torch.bfloat16)
+    new_k, new_v = query(2, 2, 128, torch.bfloat16, 8), query(2, 2, 128, torch.bfloat16, 9)
+    want = paged_attention(q, pool.keys.clone(), pool.values.clone(), pool.table, pool.n, new_key=new_k, new_value=new_v)
+    both = torch.empty((pool.keys.shape[0], 2, 16, 2, 128), dtype=q.dtype, device=DEV)       # token-major, K beside V
+    keys, values = both[:, 0].transpose(1, 2), both[:, 1].transpose(1, 2)
+    keys.copy_(pool.keys), values.copy_(pool.values)
+    table = torch.full((2, pool.columns + 5), -9, dtype=torch.int32, device=DEV)
+    table[:, :pool.columns] = pool.table
+    for shift in (0, 3):      # query and new rows that do not start on 16 bytes are copied
+        x, nk, nv = (torch.empty(t.numel() + shift, dtype=t.dtype, device=DEV)[shift:].view(t.shape).copy_(t) for t in (q, new_k, new_v))
+        room = torch.empty((2, 8, 256), dtype=q.dtype, device=DEV)[:, :, 128:]
+        got = paged_attention(x, keys, values, table[:, :pool.columns], pool.n.repeat_interleave(2)[::2], new_key=nk, new_value=nv, out=room)
+        assert got is room and torch.equal(got, want)
+
+
+def test_pages_and_lengths_out_of_range():
+    from inquant import _native as N
+    from inquant.dense_paged import paged_attention
+    lengths = [200, 40]
+    pool = Pool(lengths, 2, 128, 16, torch.bfloat16, seed=5)
+    q = query(2, 4, 128, torch.bfloat16)
+    new = query(2, 2, 128, torch.bfloat16, 8)
+    assert N.take_status(q.device) == 0
+    want = paged_attention(q, pool.keys, pool.values, pool.table, pool.n)
+    for bad in (-1, pool.keys.shape[0], 2 ** 31 - 1):
+        table = pool.table.clone()
+        table[0, 3:6] = bad       # tokens 48 .. 95 are left out
+        weights = torch.full((2, 2, pool.columns * 16), 7.0, device=DEV)
+        out, w = paged_attention(q, pool.keys, pool.values, table, pool.n, out_weights=weights)
+        assert N.take_status(q.device) == N.STATUS_BAD_INDEX
+        assert torch.equal(out[1], want[1]) and (w[0, :, 48:96] == 0).all() and torch.isfinite(out).all()
+        k, v = pool.get(0, 200)
+        rest = torch.cat([torch.arange(48), torch.arange(96, 200)]).to(DEV)
+        p = torch.softmax(q[0].double().view(2, 2, 128) @ k[rest].double().permute(1, 2, 0) * 128 ** -0.5, 2)
+        assert ((p @ v[rest].double().transpose(0, 1)).view(4, 128) - out[0].double()).abs().max() < 2.0 ** -7
+    # a table that has no room for the new token, a length beyond it: nothing is stored, the table's tokens are attended to
+    short = pool.table[:, :2].contiguous()
+    keys = pool.keys.clone()
+    full = paged_attention(q, pool.keys, pool.values, short, ints([32, 32]))
+    for n in (32, 100, 2 ** 31 - 1):
+        out = paged_attention(q, pool.keys, pool.values, short, ints([n, 32]), new_key=new, new_value=new)
+        assert N.take_status(q.device) == N.STATUS_BAD_INDEX and torch.equal(out, full)
+    assert torch.equal(keys.view(torch.int16), pool.keys.view(torch.int16))
+    # a place for the new token in a page that is not there
+    table = pool.table.clone()
+    table[0, 12] = -1             # tokens 192 .. 207
+    out = paged_attention(q, pool.keys, pool.values, table, pool.n, new_key=new, new_value=new)
+    assert N.take_status(q.device) == N.STATUS_BAD_INDEX and torch.isfinite(out).all()
+    assert torch.equal(keys.view(torch.int16)[pool.table[0, 12].long()], pool.keys.view(torch.int16)[pool.table[0, 12].long()])
+
+
+def test_captured_steps_follow_lengths_and_share_no_scratch():
+    from inquant.dense_paged import paged_attention
+    lengths = [100, 900]
+    pool = Pool(lengths, 4, 128, 16, torch.bfloat16, seed=6, spare=4)
+    q = query(2, 28, 128, torch.bfloat16)
+    n = ints(lengths)
+    weights = torch.zeros((2, 4, pool.columns * 16), device=DEV)
+    graphs = []
+    for _ in range(2):
+        stream = torch.cuda.Stream()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream):
+            got = paged_attention(q, pool.keys, pool.values, pool.table, n, out_weights=torch.zeros_like(weights))
+        graphs.append((graph, got, stream))
+    for mix in ([100, 900], [1, 33], [0, -1], [64, 800]):
+        n.copy_(ints(mix))
+        want = paged_attention(q, pool.keys, pool.values, pool.table, ints(mix), out_weights=torch.zeros_like(weights))
+        torch.cuda.synchronize()
+        for graph, _, stream in graphs:
+            with torch.cuda.stream(stream):
+                graph.replay()
+        torch.cuda.synchronize()
+        for _, got, _ in graphs:
+            assert torch.equal(got[0], want[0])
+            for b in range(2):
+                assert torch.equal(got[1][b, :, :max(mix[b], 0)], want[1][b, :, :max(mix[b], 0)])
+
+
+def test_a_long_cache_whose_offsets_pass_32_bits():
+    """Pages behind 2^31 elements of a pool that shares its storage with other data."""
+    from inquant.dense_paged import paged_attention
+    lengths = [500]
+    pool = Pool(lengths, 2, 128, 16, torch.bfloat16, seed=7)
+    wide = torch.empty(2 ** 31 + 40 * 4096, dtype=torch.bfloat16, device=DEV)
+    count = pool.keys.shape[0]
+    keys = wide.as_strided((count, 2, 16, 128), (2 ** 31 // count // 8 * 8, 2048, 128, 1))
+    keys.copy_(pool.keys)
+    q = query(1, 14, 128, torch.bfloat16)
+    assert torch.equal(paged_attention(q, keys, pool.values, pool.table, pool.n), paged_attention(q, pool.keys, pool.values, pool.table, pool.n))
+
+
+# ------------------------------------------------------------------------------------------------ eviction
+def evicted(weights, positions, length, seen, budget, sink, recent):
+    """Places (origin of what lies at each of the first min(length, budget) places) of one row, from the definition."""
+    w = [(-math.inf if math.isnan(x) else x) for x in weights[:length].tolist()]
+    nan = [math.isnan(x) for x in weights[:length].tolist()]
+    p = positions[:length].tolist()
+    if length <= budget:
+        return list(range(length))
+    safe = [p[j] < sink or p[j] >= seen - recent for j in range(length)]
+    order = sorted(range(length), key=lambda j: (not safe[j], not safe[j] and nan[j], 0.0 if safe[j] else -w[j], j))
+    kept = set(order[:budget])
+    free = [j for j in range(budget) if j not in kept]
+    moving = [j for j in range(budget, length) if j in kept]
+    origin = list(range(budget))
+    for to, source in zip(free, moving):
+        origin[to] = source
+    return origin
+
+
+def check_evict(pool, heads, lengths, seen, weights, positions, budget, sink, recent, in_place=False):
+    from inquant.dense_paged import evict_tokens
+    keys, values = pool.keys.clone(), pool.values.clone()
+    want = [[evicted(weights[b, h].cpu(), positions[b, h].cpu(), max(n, 0), seen[b], budget, sink, recent) for h in range(heads)]
+            for b, n in enumerate(lengths)]
+    w0, p0, n0 = weights.clone(), positions.clone(), ints(lengths)
+    into = dict(out_weights=weights, out_positions=positions, out_lengths=n0) if in_place else {}
+    n, w, p = evict_tokens(pool.keys, pool.values, pool.table, n0, weights, positions, ints(seen), budget, sink=sink, recent=recent, **into)
+    assert n.tolist() == [min(x, budget) for x in lengths]
+    for b in range(len(lengths)):
+        for h in range(heads):
+            o = torch.tensor(want[b][h], dtype=torch.long, device=DEV)
+            assert torch.equal(p[b, h, :len(o)], p0[b, h, o])
+            assert torch.equal(w[b, h, :len(o)].nan_to_num(-7), w0[b, h, o].nan_to_num(-7))
+            assert (w[b, h, len(o):budget] == 0).all() and (p[b, h, len(o):budget] == -1).all()
+            if len(o):
+                page, offset = pool.places(b, o)
+                to_page, to_offset = pool.places(b, torch.arange(len(o), device=DEV))
+                for new, old in ((pool.keys, keys), (pool.values, values)):
+                    assert torch.equal(new[to_page, h, to_offset], old[page, h, offset])
+                    old[to_page, h, to_offset] = new[to_page, h, to_offset]
+    # nothing else was written
+    assert torch.equal(keys.view(torch.int16), pool.keys.view(torch.int16)) and torch.equal(values.view(torch.int16), pool.values.view(torch.int16))
+
+
+def eviction_state(lengths, heads, columns, seed, ties=0.3):
+    g = torch.Generator(device=DEV).manual_seed(seed)
+    weights = torch.exp(2 * torch.randn((len(lengths), heads, columns), generator=g, device=DEV))
+    weights[torch.rand(weights.shape, generator=g, device=DEV) < ties] = 0.0
+    seen = [2 * max(n, 0) + 3 for n in lengths]
+    positions = torch.zeros((len(lengths), heads, columns), dtype=torch.int32, device=DEV)
+    for b, n in enumerate(lengths):
+        for h in range(heads):
+            if n > 0:
+                positions[b, h, :n] = torch.randperm(seen[b], generator=g, device=DEV)[:n]
+    return weights, positions, seen
+
+
+@pytest.mark.parametrize("lengths,budget,sink,recent", [
+    ([300], 256, 4, 32), ([5000, 17, 0, -1, 257, 256], 256, 4, 100), ([3], 2, 0, 0), ([2], 1, 1, 0), ([1000, 900], 700, 0, 700),
+    ([9000], 8192, 4, 512), ([20000, 4], 37, 3, 30), ([33], 32, 16, 16)])
+@pytest.mark.parametrize("page,in_place", [(16, False), (24, True)])
+def test_tokens_of_least_weight_leave(lengths, budget, sink, recent, page, in_place):
+    pool = Pool(lengths, 2, 128, page, torch.bfloat16, seed=11)
+    width = max(pool.columns * page, budget)
+    weights, positions, seen = eviction_state(lengths, 2, width, 12)
+    check_evict(pool, 2, lengths, seen, weights, positions, budget, sink, recent, in_place)
+
+
+@pytest.mark.parametrize("heads,dim,dtype", [(1, 64, torch.float16), (8, 128, torch.float16)])
+def test_eviction_of_other_shapes(heads, dim, dtype):
+    lengths = [700, 64, 4100]
+    pool = Pool(lengths, heads, dim, 32, dtype, seed=13)
+    weights, positions, seen = eviction_state(lengths, heads, pool.columns * 32, 14)
+    check_evict(pool, heads, lengths, seen, weights, positions, 512, 4, 64)
+
+
+@pytest.mark.parametrize("value", [0.0, 1.5, -2.0, float("nan"), float("inf"), 1e-42])
+def test_weights_that_all_tie(value):
+    lengths = [1500]
+    pool = Pool(lengths, 2, 128, 16, torch.bfloat16, seed=15)
+    weights, positions, seen = eviction_state(lengths, 2, pool.columns * 16, 16)
+    weights[:] = value
+    check_evict(pool, 2, lengths, seen, weights, positions, 1000, 4, 50)
+
+
+def test_order_of_special_weights():
+    lengths = [700]
+    pool = Pool(lengths, 1, 128, 16, torch.bfloat16, seed=17)
+    weights, positions, seen = eviction_state(lengths, 1, pool.columns * 16, 18)
+    specials = torch.tensor([float("nan"), float("-inf"), -3.0, -0.0, 0.0, 1e-42, -1e-42, 1.0, float("inf")], device=DEV)
+    weights[0, 0, :700] = specials[torch.arange(700, device=DEV) % 9]
+    for budget in (60, 200, 350, 500, 640, 699):
+        check_evict(pool, 1, lengths, seen, weights, positions, budget, 0, 0)
+
+
+def test_more_protected_tokens_than_the_budget_holds():
+    """Positions are distinct in earnest; equal ones must not lead anywhere else than to the first places."""
+    lengths = [600]
+    pool = Pool(lengths, 2, 128, 16, torch.bfloat16, seed=19)
+    weights, positions, seen = eviction_state(lengths, 2, pool.columns * 16, 20)
+    positions[:] = 0
+    check_evict(pool, 2, lengths, seen, weights, positions, 512, 4, 64)
+
+
+def test_eviction_out_of_range():
+    from inquant import _native as N
+    from inquant.dense_paged import evict_tokens
+    lengths = [600, 300]
+    pool = Pool(lengths, 2, 128, 16, torch.bfloat16, seed=21)
+    weights, positions, seen = eviction_state(lengths, 2, pool.columns * 16, 22)
+    table = pool.table.clone()
+    table[0, 30:] = 10 ** 9
+    assert N.take_status(pool.keys.device) == 0
+    kept = pool.keys.clone()
+    n, w, p = evict_tokens(pool.keys, pool.values, table, pool.n, weights, positions, ints(seen), 256, sink=4, recent=64)
+    assert N.take_status(pool.keys.device) == N.STATUS_BAD_INDEX and n.tolist() == [256, 256]
+    other = torch.ones(pool.keys.shape[0], dtype=torch.bool, device=DEV)
+    other[pool.table[0].long()] = False
+    other[pool.table[1].long().clamp_min(0)] = False
+    assert torch.equal(kept[other].view(torch.int16), pool.keys[other].view(torch.int16))
+    n, _, _ = evict_tokens(pool.keys, pool.values, pool.table, ints([2 ** 31 - 1, 300]), weights, positions, ints(seen), 256)
+    assert N.take_status(pool.keys.device) == N.STATUS_BAD_INDEX and n.tolist() == [256, 256]
