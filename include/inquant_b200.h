@@ -510,7 +510,8 @@ int64_t inq_paged_attention_workspace_bytes(const inq_paged_attention_args_t* ar
  * the i-th free place: its rows of k and v, its weight and its position.  out_weights and out_positions [.., budget] get
  * the state of the places (0 and -1 where no token is), out_lengths min(lengths, budget); each may be its input.
  * The pages of a request that evicts belong to it alone.  sink + recent <= budget.  A page id outside the pool is not
- * used and sets INQ_STATUS_BAD_INDEX, as does a length beyond the table or `columns`, which counts as that. */
+ * used and sets INQ_STATUS_BAD_INDEX, as does a length beyond the table or `columns`, which counts as that.  A table
+ * holds fewer than 2^22 tokens per request. */
 typedef struct {
   void *k, *v;                    /* [pages, kv_heads, page_tokens, head_dim], 16-bit elements */
   int64_t k_stride_p, k_stride_h, k_stride_t, v_stride_p, v_stride_h, v_stride_t;

@@ -20,7 +20,7 @@ namespace cg = cooperative_groups;
 
 namespace inq {
 
-constexpr int kEvThreads = 512, kEvBins = 2048, kEvMaxCluster = 8, kEvPerThread = 8;
+constexpr int kEvThreads = 512, kEvBins = 2048, kEvMaxCluster = 8;
 
 struct EvictParams {
   void *k, *v;
@@ -67,14 +67,17 @@ __device__ __forceinline__ int block_prefix(int mine, int& all, int* scratch /* 
   return before + sum - mine;
 }
 
+// KEYS: tokens per thread whose keys stay in registers over all passes; a slice of more is read anew for each.
+template <int KEYS>
 __global__ void __launch_bounds__(kEvThreads) evict_select_kernel(const EvictParams P) {
   cg::cluster_group cluster = cg::this_cluster();
   const int ctas = (int)cluster.num_blocks(), me = (int)cluster.block_rank();
   const int row = blockIdx.x / ctas, b = row / P.kv_heads, h = row % P.kv_heads, tid = threadIdx.x;
-  __shared__ int histogram[kEvBins];
+  __shared__ __align__(16) int histogram[kEvBins];
   __shared__ int shared_counts[3];                    // this CTA's ties, free places and moving tokens
   __shared__ int scratch[kEvThreads / 32 + 1], chosen[2];
   follow_stream();
+  allow_next();
   const long long asked = P.lengths[b];
   const int length = (int)min(max(asked, 0LL), P.capacity), budget = P.budget;
   if (asked > P.capacity && row % P.kv_heads == 0 && me == 0 && tid == 0) atomicOr(P.status, INQ_STATUS_BAD_INDEX);
@@ -99,41 +102,57 @@ __global__ void __launch_bounds__(kEvThreads) evict_select_kernel(const EvictPar
   }
   const long long safe_from = (long long)P.seen[b] - P.recent;
   const int slice = (length + ctas - 1) / ctas, lo = min(me * slice, length), hi = min(lo + slice, length);
-  auto key = [&](int j) {
-    const int p = pos[j];
-    return p < P.sink || p >= safe_from ? 0xffffffffu : worth(w[j]);
+  constexpr int kGroup = kEvThreads * KEYS;
+  const int groups = (hi - lo + kGroup - 1) / kGroup;
+  unsigned keys[KEYS];          // of neighbouring tokens; 0 behind the slice, where no token is looked for
+  auto load = [&](int g) {
+#pragma unroll
+    for (int i = 0; i < KEYS; ++i) {
+      const int j = lo + g * kGroup + tid * KEYS + i;
+      keys[i] = 0u;
+      if (j < hi) {
+        const int p = __ldg(pos + j);
+        keys[i] = p < P.sink || p >= safe_from ? 0xffffffffu : worth(__ldg(w + j));
+      }
+    }
   };
+  if (groups <= 1) load(0);
 
   // ---- the key of the last token that stays: `want` tokens of those that begin with `prefix` are still to be found
   unsigned prefix = 0;
   int want = budget;
 #pragma unroll 1
   for (int pass = 0; pass < 3; ++pass) {
-    const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, bins = pass == 2 ? 1024 : 2048;
-    for (int i = tid; i < kEvBins; i += kEvThreads) histogram[i] = 0;
+    const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, above = pass == 0 ? 32 : pass == 1 ? 21 : 10;
+    const unsigned bins = pass == 2 ? 1024u : 2048u;
+    static_assert(kEvBins == 4 * kEvThreads, "a thread clears and adds four bins");
+    ((int4*)histogram)[tid] = make_int4(0, 0, 0, 0);
     __syncthreads();
-    for (int j = lo + tid; j < hi; j += kEvThreads) {
-      const unsigned k = key(j);
-      if (pass == 0 || (k >> (pass == 1 ? 21 : 10)) == prefix) atomicAdd(histogram + ((k >> shift) & (bins - 1)), 1);
+#pragma unroll 1
+    for (int g = 0; g < groups; ++g) {
+      if (groups > 1) load(g);
+      const int count = hi - (lo + g * kGroup + tid * KEYS);
+#pragma unroll
+      for (int i = 0; i < KEYS; ++i)
+        if (i < count && (pass == 0 || keys[i] >> above == prefix)) atomicAdd(histogram + ((keys[i] >> shift) & (bins - 1)), 1);
     }
     cluster.sync();
     // every CTA finds the digit for itself: a thread adds four neighbouring bins over the cluster, highest bins first
-    int mine[4], sum = 0, all;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int bin = kEvBins - 1 - (4 * tid + i);
-      mine[i] = 0;
-      for (int c = 0; c < ctas; ++c) mine[i] += cluster.map_shared_rank(histogram, c)[bin];
-      sum += mine[i];
+    int4 mine = make_int4(0, 0, 0, 0);
+    for (int c = 0; c < ctas; ++c) {
+      const int4 n = ((const int4*)cluster.map_shared_rank(histogram, c))[kEvThreads - 1 - tid];
+      mine = make_int4(mine.x + n.x, mine.y + n.y, mine.z + n.z, mine.w + n.w);
     }
-    int before = block_prefix(sum, all, scratch);
+    int all;
+    int before = block_prefix(mine.x + mine.y + mine.z + mine.w, all, scratch);
+    const int each[4] = {mine.w, mine.z, mine.y, mine.x};
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      if (before < want && before + mine[i] >= want) {
+      if (before < want && before + each[i] >= want) {
         chosen[0] = kEvBins - 1 - (4 * tid + i);
         chosen[1] = want - before;
       }
-      before += mine[i];
+      before += each[i];
     }
     __syncthreads();
     prefix = (prefix << (pass == 2 ? 10 : 11)) | (unsigned)chosen[0];
@@ -145,12 +164,12 @@ __global__ void __launch_bounds__(kEvThreads) evict_select_kernel(const EvictPar
   int ties_before = 0;
   for (int c = 0; c < me; ++c) ties_before += cluster.map_shared_rank(shared_counts, c)[0];
 
-  // ---- twice over the slice: the free places and moving tokens of this CTA, then their lists
+  // ---- twice over the slice: the free places and moving tokens of this CTA, then their lists (a CTA alone starts at zero)
   int holes = 0, moves = 0;          // in front of the group of tokens in work
 #pragma unroll 1
-  for (int round = 0; round < 2; ++round) {
+  for (int round = ctas == 1; round < 2; ++round) {
     int ties = ties_before;
-    if (round == 1) {
+    if (round == 1 && ctas > 1) {
       cluster.sync();
       holes = moves = 0;
       for (int c = 0; c < me; ++c) {
@@ -159,38 +178,32 @@ __global__ void __launch_bounds__(kEvThreads) evict_select_kernel(const EvictPar
       }
     }
 #pragma unroll 1
-    for (int j0 = lo; j0 < hi; j0 += kEvThreads * kEvPerThread) {
-      unsigned keys[kEvPerThread];
+    for (int g = 0; g < groups; ++g) {
+      if (groups > 1) load(g);
+      const int j0 = lo + g * kGroup + tid * KEYS, count = hi - j0;
       int equal = 0, all_equal;
 #pragma unroll
-      for (int i = 0; i < kEvPerThread; ++i) {
-        const int j = j0 + tid * kEvPerThread + i;
-        keys[i] = j < hi ? key(j) : 0u;
-        equal += j < hi && keys[i] == prefix;
-      }
+      for (int i = 0; i < KEYS; ++i) equal += i < count && keys[i] == prefix;
       int rank = ties + block_prefix(equal, all_equal, scratch);
       ties += all_equal;
       unsigned kept = 0;
       int mine_holes = 0, mine_moves = 0;
 #pragma unroll
-      for (int i = 0; i < kEvPerThread; ++i) {
-        const int j = j0 + tid * kEvPerThread + i;
-        if (j >= hi) continue;
-        const bool tie = keys[i] == prefix;
-        const bool stays = keys[i] > prefix || (tie && rank < want);
-        rank += tie;
+      for (int i = 0; i < KEYS; ++i) {
+        const bool tie = keys[i] == prefix, stays = i < count && (keys[i] > prefix || (tie && rank < want));
+        rank += i < count && tie;
         kept |= (unsigned)stays << i;
-        mine_holes += !stays && j < left;
-        mine_moves += stays && j >= left;
+        mine_holes += i < count && !stays && j0 + i < left;
+        mine_moves += stays && j0 + i >= left;
       }
       int all_packed;
-      int packed = block_prefix(mine_holes | (mine_moves << 16), all_packed, scratch);
+      const int packed = block_prefix(mine_holes | (mine_moves << 16), all_packed, scratch);
       if (round == 1) {
         int hole = holes + (packed & 0xffff), move = moves + (packed >> 16);
 #pragma unroll
-        for (int i = 0; i < kEvPerThread; ++i) {
-          const int j = j0 + tid * kEvPerThread + i;
-          if (j >= hi) continue;
+        for (int i = 0; i < KEYS; ++i) {
+          const int j = j0 + i;
+          if (i >= count) continue;
           const bool stays = (kept >> i) & 1u;
           if (j < left) {
             if (stays) {
@@ -219,35 +232,45 @@ __global__ void __launch_bounds__(kEvThreads) evict_select_kernel(const EvictPar
   cluster.sync();       // the counts of a CTA are read until here
 }
 
-// A warp moves one token: half of its lanes the key row, the others the value row, 16 bytes each.
-constexpr int kEvMoveThreads = 256, kEvMoveTokens = 64;      // tokens of a block
+// A warp moves eight tokens at once, and asks for all of them before it writes the first: half of its lanes the key rows, the
+// others the value rows, 16 bytes each.
+constexpr int kEvMoveThreads = 256, kEvMoveEach = 8, kEvMoveTokens = kEvMoveThreads / 32 * kEvMoveEach;      // tokens of a block
 __global__ void __launch_bounds__(kEvMoveThreads) evict_move_kernel(const EvictParams P) {
   follow_stream();
   const int row = blockIdx.x, b = row / P.kv_heads, h = row % P.kv_heads, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int* const list = P.lists + row * (2 * P.list_columns + 1);
   if (blockIdx.y == 0 && h == 0 && threadIdx.x == 0) P.out_lengths[b] = min(P.lengths[b], P.budget);
-  const int count = list[0];
-  auto address = [&](int j, bool& fine) {
-    const int column = P.page_shift >= 0 ? j >> P.page_shift : j / P.page_tokens;
-    const int page = __ldg(P.table + b * P.table_stride + column), o = j - column * P.page_tokens;
-    fine = page >= 0 && page < P.pages;
-    return lane < 16 ? (char*)P.k + 2 * (page * P.k_sp + h * P.k_sh + o * P.k_st) : (char*)P.v + 2 * (page * P.v_sp + h * P.v_sh + o * P.v_st);
-  };
-  for (int i = blockIdx.y * kEvMoveTokens + warp; i < min(count, (int)(blockIdx.y + 1) * kEvMoveTokens); i += kEvMoveThreads / 32) {
-    const int to = list[1 + i], from = list[1 + P.list_columns + i];
-    bool to_fine, from_fine;
-    char* const dst = address(to, to_fine);
-    const char* const src = address(from, from_fine);
-    if (to_fine && from_fine) {
-      const int at = (lane & 15) * 16;
-      if (at < P.row_bytes) *(uint4*)(dst + at) = *(const uint4*)(src + at);
-    } else if (lane == 0) {
-      atomicOr(P.status, INQ_STATUS_BAD_INDEX);
-    }
-    if (lane == 0) {
-      P.out_weights[b * P.ow_sb + h * P.ow_sh + to] = P.weights[b * P.w_sb + h * P.w_sh + from];
-      P.out_positions[b * P.op_sb + h * P.op_sh + to] = P.positions[b * P.p_sb + h * P.p_sh + from];
-    }
+  const int count = __ldcg(list), i0 = blockIdx.y * kEvMoveTokens + warp * kEvMoveEach;
+  if (i0 >= count) return;
+  // lane 2 i (+ 1) finds the page and offset of where token i goes (comes from), and moves its weight and position
+  const int i = i0 + (lane >> 1);
+  const bool some = lane < 2 * kEvMoveEach && i < count;
+  const int j = some ? __ldcg(list + 1 + (lane & 1 ? P.list_columns : 0) + i) : 0;
+  const int column = P.page_shift >= 0 ? j >> P.page_shift : j / P.page_tokens, o = j - column * P.page_tokens;
+  int page = some ? __ldg(P.table + b * P.table_stride + column) : -1;
+  if (some && (page < 0 || page >= P.pages)) {
+    atomicOr(P.status, INQ_STATUS_BAD_INDEX);
+    page = -1;
+  }
+  const int place = __shfl_xor_sync(0xffffffffu, j, 1);
+  if (some && (lane & 1)) {
+    P.out_weights[b * P.ow_sb + h * P.ow_sh + place] = P.weights[b * P.w_sb + h * P.w_sh + j];
+    P.out_positions[b * P.op_sb + h * P.op_sh + place] = P.positions[b * P.p_sb + h * P.p_sh + j];
+  }
+  const bool key = lane < 16;
+  const long long sp = key ? P.k_sp : P.v_sp, st = key ? P.k_st : P.v_st;
+  char* const base = (char*)(key ? P.k : P.v) + 2 * h * (key ? P.k_sh : P.v_sh) + (lane & 15) * 16;
+  const bool mine = (lane & 15) * 16 < P.row_bytes;
+  uint4 rows[kEvMoveEach];
+#pragma unroll
+  for (int n = 0; n < kEvMoveEach; ++n) {
+    const int to = __shfl_sync(0xffffffffu, page, 2 * n), from = __shfl_sync(0xffffffffu, page, 2 * n + 1), from_o = __shfl_sync(0xffffffffu, o, 2 * n + 1);
+    if (to >= 0 && from >= 0 && mine) rows[n] = __ldcs((const uint4*)(base + 2 * (from * sp + from_o * st)));
+  }
+#pragma unroll
+  for (int n = 0; n < kEvMoveEach; ++n) {
+    const int to = __shfl_sync(0xffffffffu, page, 2 * n), from = __shfl_sync(0xffffffffu, page, 2 * n + 1), to_o = __shfl_sync(0xffffffffu, o, 2 * n);
+    if (to >= 0 && from >= 0 && mine) *(uint4*)(base + 2 * (to * sp + to_o * st)) = rows[n];
   }
 }
 
@@ -270,7 +293,7 @@ extern "C" int inq_evict_tokens(const inq_evict_args_t* a, inq_stream_t stream_)
   if ((a->k_stride_p | a->k_stride_h | a->k_stride_t | a->v_stride_p | a->v_stride_h | a->v_stride_t) & 7) return INQ_ERR_ARGUMENT;
   if (((uintptr_t)a->k | (uintptr_t)a->v) & 15) return INQ_ERR_ARGUMENT;
   const long long capacity = (long long)a->table_columns * a->page_tokens, rows = (long long)a->requests * a->kv_heads;
-  if (capacity > 0x3fffffffLL || a->budget > 0x3fffffff || rows * kEvMaxCluster > 0x7fffffffLL) return INQ_ERR_CAPACITY;
+  if (capacity > 0x3fffffLL || a->budget > 0x3fffffff || rows * kEvMaxCluster > 0x7fffffffLL) return INQ_ERR_CAPACITY;
   if (!a->workspace || a->workspace_bytes < inq_evict_workspace_bytes(a->requests, a->kv_heads, a->budget, capacity)) return INQ_ERR_CAPACITY;
   int device = 0, n_sm = 0;
   INQ_CUDA_CHECK(cudaGetDevice(&device));
@@ -308,10 +331,15 @@ extern "C" int inq_evict_tokens(const inq_evict_args_t* a, inq_stream_t stream_)
     config.stream = stream;
     config.attrs = attrs;
     config.numAttrs = 2;
-    INQ_CUDA_CHECK(cudaLaunchKernelEx(&config, evict_select_kernel, P));
+    // keys of a slice in registers where 16 per thread do; fewer registers where 4 do
+    const long long slice = (P.capacity + ctas - 1) / ctas;
+    INQ_CUDA_CHECK(slice <= 4 * kEvThreads ? cudaLaunchKernelEx(&config, evict_select_kernel<4>, P)
+                                           : slice <= 8 * kEvThreads ? cudaLaunchKernelEx(&config, evict_select_kernel<8>, P)
+                                                                     : cudaLaunchKernelEx(&config, evict_select_kernel<16>, P));
   }
-  const unsigned blocks = (unsigned)((std::min<long long>(P.budget, P.capacity) + kEvMoveTokens - 1) / kEvMoveTokens);
-  if (blocks > 65535) return INQ_ERR_CAPACITY;
+  // as many tokens move as places fall free, at most, and as there are behind the budget
+  const long long most = std::min<long long>(P.budget, std::max<long long>(P.capacity - P.budget, 1));
+  const unsigned blocks = (unsigned)((most + kEvMoveTokens - 1) / kEvMoveTokens);
   INQ_CUDA_CHECK(launch_following(evict_move_kernel, dim3((unsigned)rows, blocks), kEvMoveThreads, 0, stream, P));
   return INQ_OK;
 }

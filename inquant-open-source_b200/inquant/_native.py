@@ -259,6 +259,9 @@ def host():
             module, found = None, f"nothing that loads here ({exc})"
         if found == host_built_for():
             module.bind(*(ctypes.cast(f, c_void_p).value for f in (lib.inq_decode_attention, lib.inq_append_token)), torch.Tensor)
+            module.bind_dense(*(ctypes.cast(f, c_void_p).value for f in (
+                lib.inq_prompt_attention, lib.inq_prompt_weights, lib.inq_prompt_workspace_bytes, lib.inq_paged_attention,
+                lib.inq_paged_attention_workspace_bytes, lib.inq_evict_tokens, lib.inq_evict_workspace_bytes)))
             _host = module
         else:
             warnings.warn(f"inquant/_host.so is built for {found}, not for {host_built_for()}: decode and append take their slower "
@@ -341,6 +344,11 @@ def require_cuda(tensor: torch.Tensor, what: str) -> None:
 
 
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
+def native_call(tensor):
+    """The native host side for a call on an ordinary CUDA tensor, else None."""
+    return host() if type(tensor) is torch.Tensor and tensor.is_cuda else None
 
 
 def stream_handle(device: torch.device) -> int:

@@ -50,7 +50,6 @@ def _check_state(name: str, t: torch.Tensor, dtype: torch.dtype, requests: int, 
         raise ValueError(f"{name} must be a {dtype} tensor [{requests}, {heads}, >= {columns}] with unit token stride on the pages' device")
 
 
-@torch.no_grad()
 def paged_attention(query: torch.Tensor, key_pages: torch.Tensor, value_pages: torch.Tensor, block_table: torch.Tensor,
                     lengths: torch.Tensor, *, scale: float | None = None, new_key: torch.Tensor | None = None,
                     new_value: torch.Tensor | None = None, weights: torch.Tensor | None = None, out_weights: torch.Tensor | None = None,
@@ -67,6 +66,19 @@ def paged_attention(query: torch.Tensor, key_pages: torch.Tensor, value_pages: t
     outside the pool is never used as an address: its tokens are left out, and ``STATUS_BAD_INDEX`` is set in the
     device's status word, as it is for a length beyond the table.  Two requests may share pages as long as neither
     stores into them.  Returns the output [B, Hq, D], and with weights ``(output, out_weights)``."""
+    host = N.native_call(query)      # the ordinary call in native code, the rest takes the checks and copies below
+    if host is not None:
+        result = host.paged_attention(query, key_pages, value_pages, block_table, lengths, scale, new_key, new_value, weights, out_weights, out,
+                                      N.status_word(query.device).data_ptr())
+        if type(result) is int:
+            N.check(result, "inq_paged_attention")
+        if result is not None:
+            return result
+    return _paged_attention(query, key_pages, value_pages, block_table, lengths, scale, new_key, new_value, weights, out_weights, out)
+
+
+@torch.no_grad()
+def _paged_attention(query, key_pages, value_pages, block_table, lengths, scale, new_key, new_value, weights, out_weights, out):
     _check_pages("paged_attention", key_pages, value_pages, block_table, lengths)
     pages, heads, page_tokens, dim = key_pages.shape
     requests, device = block_table.shape[0], key_pages.device
@@ -123,7 +135,6 @@ def paged_attention(query: torch.Tensor, key_pages: torch.Tensor, value_pages: t
     return out if out_weights is None else (out, out_weights)
 
 
-@torch.no_grad()
 def evict_tokens(key_pages: torch.Tensor, value_pages: torch.Tensor, block_table: torch.Tensor, lengths: torch.Tensor,
                  weights: torch.Tensor, positions: torch.Tensor, seen: torch.Tensor, budget: int, *, sink: int = 4, recent: int = 128,
                  out_weights: torch.Tensor | None = None, out_positions: torch.Tensor | None = None,
@@ -141,6 +152,21 @@ def evict_tokens(key_pages: torch.Tensor, value_pages: torch.Tensor, block_table
     and ``seen`` are int32 [B]; pages of a request that evicts belong to it alone.  A page id outside the pool is not
     used, and sets ``STATUS_BAD_INDEX``, as does a length beyond the table or the columns of ``weights`` (it
     counts as that)."""
+    host = N.native_call(key_pages)
+    if host is not None and type(budget) is int and type(sink) is int and type(recent) is int and 0 < budget < 2 ** 31 and abs(sink) + abs(recent) < 2 ** 31:
+        result = host.evict_tokens(key_pages, value_pages, block_table, lengths, weights, positions, seen, budget, sink, recent, out_weights,
+                                   out_positions, out_lengths, N.status_word(key_pages.device).data_ptr())
+        if type(result) is int:
+            N.check(result, "inq_evict_tokens")
+        if result is not None:
+            return result
+    return _evict_tokens(key_pages, value_pages, block_table, lengths, weights, positions, seen, budget, sink, recent, out_weights, out_positions,
+                         out_lengths)
+
+
+@torch.no_grad()
+def _evict_tokens(key_pages, value_pages, block_table, lengths, weights, positions, seen, budget, sink, recent, out_weights, out_positions,
+                  out_lengths):
     _check_pages("evict_tokens", key_pages, value_pages, block_table, lengths)
     pages, heads, page_tokens, dim = key_pages.shape
     requests, device = block_table.shape[0], key_pages.device

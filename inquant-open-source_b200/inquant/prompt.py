@@ -73,7 +73,6 @@ def _arguments(query, key, cu_seqlens, cu_seqlens_k, scale, window, weights) -> 
     return args
 
 
-@torch.no_grad()
 def prompt_attention(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor, cu_seqlens: torch.Tensor,
                      cu_seqlens_k: torch.Tensor | None = None, *, scale: float | None = None, out: torch.Tensor | None = None,
                      lse: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
@@ -87,6 +86,18 @@ def prompt_attention(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor
     value behind a sequence or at a position that a query does not see never reaches that query, infinities and
     NaN included.  Offsets outside the tensors, or falling ones, are cut to what the tensors hold, and set
     ``STATUS_BAD_INDEX`` in the device's status word."""
+    host = N.native_call(query)      # the ordinary call in native code, the rest takes the checks and copies below
+    if host is not None:
+        result = host.prompt_attention(query, key, value, cu_seqlens, cu_seqlens_k, scale, out, lse, N.status_word(query.device).data_ptr())
+        if type(result) is int:
+            N.check(result, "inq_prompt_attention")
+        if result is not None:
+            return result
+    return _prompt_attention(query, key, value, cu_seqlens, cu_seqlens_k, scale, out, lse)
+
+
+@torch.no_grad()
+def _prompt_attention(query, key, value, cu_seqlens, cu_seqlens_k, scale, out, lse):
     _check_states("prompt_attention", query, key)
     if value.shape != key.shape:
         raise ValueError("Expected query [tokens, Hq, D] and key/value [tokens, H, D]")
@@ -123,7 +134,6 @@ def prompt_attention(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor
     return out, lse
 
 
-@torch.no_grad()
 def prompt_weights(query: torch.Tensor, key: torch.Tensor, lse: torch.Tensor, cu_seqlens: torch.Tensor,
                    cu_seqlens_k: torch.Tensor | None = None, *, scale: float | None = None, window: int | None = None,
                    out: torch.Tensor | None = None) -> torch.Tensor:
@@ -132,6 +142,18 @@ def prompt_weights(query: torch.Tensor, key: torch.Tensor, lse: torch.Tensor, cu
     arguments.  With ``window`` only the last ``window`` queries of every sequence count (a prompt's end is the
     better judge of what its continuation reads, and costs less).  Sums are fp32 in a fixed order.  Keys that no counted
     query sees get zero; rows of no sequence are left as they were in ``out``."""
+    host = N.native_call(query)
+    if host is not None and (window is None or type(window) is int and 0 < window <= 0x7fffffff):
+        result = host.prompt_weights(query, key, lse, cu_seqlens, cu_seqlens_k, scale, window or 0, out, N.status_word(query.device).data_ptr())
+        if type(result) is int:
+            N.check(result, "inq_prompt_weights")
+        if result is not None:
+            return result
+    return _prompt_weights(query, key, lse, cu_seqlens, cu_seqlens_k, scale, window, out)
+
+
+@torch.no_grad()
+def _prompt_weights(query, key, lse, cu_seqlens, cu_seqlens_k, scale, window, out):
     _check_states("prompt_weights", query, key)
     scale = _scale(scale, query.shape[2])
     if window is not None and window < 1:
