@@ -424,13 +424,36 @@ __global__ void __launch_bounds__(kDpThreads, 1) paged_kernel(const DensePagedPa
   }
 }
 
-// Joins the parts of pairs that ranges cut.  The first requests x query heads blocks take a row each (a thread a
-// channel); with weights, further blocks take 1024 tokens of a KV head each.
-constexpr int kDpJoinThreads = 128, kDpJoinTokens = 1024;
+// Joins the parts of pairs that ranges cut.  The first requests x query heads blocks take a row each; with weights,
+// further blocks take 512 tokens of a KV head each.  A part's maximum and sum are read by a thread each, 32 at a time, and
+// its output by D / 4 threads, 512 / D parts at once.
+constexpr int kDpJoinThreads = 128, kDpJoinEach = 4, kDpJoinTokens = kDpJoinThreads * kDpJoinEach;
+// Reference maximum and sum of a row over its parts c0 .. c0 + n - 1, the same in every lane; the whole warp takes part.
+__device__ __forceinline__ float2 join_sums(const float* first, long long stride, int n) {
+  const int lane = threadIdx.x & 31;
+  float top = kDpNegBig, sum = 0.f;
+  for (int c = lane; c < n; c += 32) {
+    const float2 ml = __ldcg((const float2*)(first + c * stride));
+    const float next = fmaxf(top, ml.x);
+    sum = sum * pf_exp2(top - next) + ml.y * pf_exp2(ml.x - next);
+    top = next;
+  }
+#pragma unroll
+  for (int d = 16; d; d >>= 1) {
+    const float other_top = __shfl_xor_sync(0xffffffffu, top, d), other = __shfl_xor_sync(0xffffffffu, sum, d);
+    const float next = fmaxf(top, other_top);
+    sum = sum * pf_exp2(top - next) + other * pf_exp2(other_top - next);
+    top = next;
+  }
+  return make_float2(top, sum);
+}
 template <typename QT, int D>
 __global__ void __launch_bounds__(kDpJoinThreads) paged_join_kernel(const DensePagedParams P, int most_ctas, int weight_blocks) {
+  constexpr int kAtOnce = 4 * kDpJoinThreads / D, kStride = 16 * (D + 2);
+  __shared__ float4 partial[kAtOnce][D / 4];
+  __shared__ float lse_s[64];
   follow_stream();
-  const int tid = threadIdx.x, rows_in_all = P.requests * P.q_heads;
+  const int tid = threadIdx.x, warp = tid >> 5, rows_in_all = P.requests * P.q_heads;
   const bool row_block = (int)blockIdx.x < rows_in_all;
   const int job = row_block ? blockIdx.x : blockIdx.x - rows_in_all;
   const int b = row_block ? job / P.q_heads : job / (P.kv_heads * weight_blocks);
@@ -442,67 +465,81 @@ __global__ void __launch_bounds__(kDpJoinThreads) paged_join_kernel(const DenseP
     if (row_block && tid < D) ((QT*)P.out)[b * P.o_sb + (long long)head * P.o_sh + tid] = from_float<QT>(0.f);
     return;
   }
+  const int t0 = row_block ? 0 : job % weight_blocks * kDpJoinTokens;
+  if (t0 >= r.tokens) return;
   long long before;
   const long long total = count_units(P, b, before);
   const int ctas = range_count(total, most_ctas);
   // parts of a pair: record of part c is c + pair
-  auto parts = [&](int pair, int& c0, int& c1) {
+  auto parts = [&](int pair, int& c0, int& n) {
     const long long u0 = before + (long long)pair * r.units;
     c0 = range_of(total, u0, ctas);
-    c1 = range_of(total, u0 + r.units - 1, ctas);
+    n = range_of(total, u0 + r.units - 1, ctas) - c0 + 1;
   };
+  auto record = [&](int c0, int pair, int g) { return P.records + ((c0 + (long long)b * per + pair) * 16 + g % 16) * (D + 2); };
   if (row_block) {
     const int head = job % P.q_heads, g = head % P.group, pair = head / P.group * P.chunks + g / 16;
-    int c0, c1;
-    parts(pair, c0, c1);
-    if (c0 == c1) return;       // written by the CTA that had the whole pair
-    const float* const rec = P.records + ((c0 + (long long)b * per + pair) * 16 + g % 16) * (D + 2);
-    const long long stride = 16 * (D + 2);
-    float top = kDpNegBig;
-    for (int c = 0; c <= c1 - c0; ++c) top = fmaxf(top, __ldcg(rec + c * stride + D));
-    float sum = 0.f, weight = 0.f;
-    if (tid < D) {
+    int c0, n;
+    parts(pair, c0, n);
+    if (n == 1) return;       // written by the CTA that had the whole pair
+    const float* const rec = record(c0, pair, g);
+    const float2 whole = join_sums(rec + D, kStride, n);
+    const int first = tid / (D / 4), c = tid % (D / 4);
+    float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 4
-      for (int c = 0; c <= c1 - c0; ++c) {
-        const float2 ml = __ldcg((const float2*)(rec + c * stride + D));
-        const float f = pf_exp2(ml.x - top);
-        weight = fmaf(ml.y, f, weight);
-        sum = fmaf(__ldcg(rec + c * stride + tid), f, sum);
+    for (int i = first; i < n; i += kAtOnce) {
+      const float f = pf_exp2(__ldcg(rec + (long long)i * kStride + D) - whole.x);
+      const float2 lo = __ldcg((const float2*)(rec + (long long)i * kStride + 4 * c)), hi = __ldcg((const float2*)(rec + (long long)i * kStride + 4 * c + 2));
+      sum.x = fmaf(lo.x, f, sum.x);
+      sum.y = fmaf(lo.y, f, sum.y);
+      sum.z = fmaf(hi.x, f, sum.z);
+      sum.w = fmaf(hi.y, f, sum.w);
+    }
+    partial[first][c] = sum;
+    __syncthreads();
+    if (tid < D / 4) {
+#pragma unroll
+      for (int i = 1; i < kAtOnce; ++i) {
+        const float4 x = partial[i][tid];
+        sum = make_float4(sum.x + x.x, sum.y + x.y, sum.z + x.z, sum.w + x.w);
       }
-      ((QT*)P.out)[b * P.o_sb + (long long)head * P.o_sh + tid] = from_float<QT>(weight == 0.f ? 0.f : sum / weight);
+      const float inv = whole.y == 0.f ? 0.f : 1.f / whole.y;
+      *(uint2*)((QT*)P.out + b * P.o_sb + (long long)head * P.o_sh + 4 * tid) =
+          make_uint2(pf_pack2<QT>(sum.x * inv, sum.y * inv), pf_pack2<QT>(sum.z * inv, sum.w * inv));
     }
     return;
   }
-  // ---- weights of 1024 tokens of one KV head
-  const int kvh = job / weight_blocks % P.kv_heads, t0 = job % weight_blocks * kDpJoinTokens;
-  if (t0 >= r.tokens) return;
-  float sums[kDpJoinTokens / kDpJoinThreads];
+  // ---- weights of 512 tokens of one KV head
+  const int kvh = job / weight_blocks % P.kv_heads;
+  float sums[kDpJoinEach];
 #pragma unroll
-  for (int i = 0; i < kDpJoinTokens / kDpJoinThreads; ++i) {
+  for (int i = 0; i < kDpJoinEach; ++i) {
     const int t = t0 + tid + i * kDpJoinThreads;
     sums[i] = P.weights && t < r.tokens && t != r.fresh ? P.weights[b * P.w_sb + kvh * P.w_sh + t] : 0.f;
   }
-  for (int g = 0; g < P.group; ++g) {
-    const int pair = kvh * P.chunks + g / 16;
-    int c0, c1;
-    parts(pair, c0, c1);
-    const float* const rec = P.records + ((c0 + (long long)b * per + pair) * 16 + g % 16) * (D + 2) + D;
-    float top = kDpNegBig, weight = 0.f;
-    for (int c = 0; c <= c1 - c0; ++c) top = fmaxf(top, __ldcg(rec + c * 16LL * (D + 2)));
-    for (int c = 0; c <= c1 - c0; ++c) {
-      const float2 ml = __ldcg((const float2*)(rec + c * 16LL * (D + 2)));
-      weight = fmaf(ml.y, pf_exp2(ml.x - top), weight);
+  const float* const logits = P.logits + ((long long)b * P.q_heads + kvh * P.group) * P.capacity;
+  for (int g0 = 0; g0 < P.group; g0 += 64) {
+    __syncthreads();
+    for (int g = g0 + warp; g < min(g0 + 64, P.group); g += kDpJoinThreads / 32) {
+      const int pair = kvh * P.chunks + g / 16;
+      int c0, n;
+      parts(pair, c0, n);
+      const float2 whole = join_sums(record(c0, pair, g) + D, kStride, n);
+      if ((tid & 31) == 0) lse_s[g - g0] = whole.y == 0.f ? __int_as_float(0x7f800000) : whole.x + log2f(whole.y);
     }
-    const float lse = weight == 0.f ? __int_as_float(0x7f800000) : top + log2f(weight);
-    const float* const logits = P.logits + ((long long)b * P.q_heads + kvh * P.group + g) * P.capacity;
+    __syncthreads();
+#pragma unroll 4
+    for (int g = g0; g < min(g0 + 64, P.group); ++g) {
+      const float lse = lse_s[g - g0];
 #pragma unroll
-    for (int i = 0; i < kDpJoinTokens / kDpJoinThreads; ++i) {
-      const int t = t0 + tid + i * kDpJoinThreads;
-      if (t < r.tokens) sums[i] += pf_exp2(__ldcg(logits + t) - lse);
+      for (int i = 0; i < kDpJoinEach; ++i) {
+        const int t = t0 + tid + i * kDpJoinThreads;
+        if (t < r.tokens) sums[i] += pf_exp2(__ldcg(logits + g * P.capacity + t) - lse);
+      }
     }
   }
 #pragma unroll
-  for (int i = 0; i < kDpJoinTokens / kDpJoinThreads; ++i) {
+  for (int i = 0; i < kDpJoinEach; ++i) {
     const int t = t0 + tid + i * kDpJoinThreads;
     if (t < r.tokens) P.out_weights[b * P.ow_sb + kvh * P.ow_sh + t] = sums[i];
   }

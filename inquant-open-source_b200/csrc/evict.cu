@@ -6,8 +6,8 @@
 // they are.  So a step that evicts a few tokens of many moves few rows, no row is both read and written, and attention,
 // for which the order of tokens in the cache means nothing, goes on as before.
 //
-// evict_select_kernel finds the worth of the last token that stays by a radix select over 32-bit keys (digits of 11, 11
-// and 10 bits, histograms in shared memory): one cluster per row (request, KV head), each CTA with a slice of it, the
+// evict_select_kernel finds the worth of the last token that stays by a radix select over 32-bit keys (four digits of 8
+// bits, histograms in shared memory): one cluster per row (request, KV head), each CTA with a slice of it, the
 // histograms added over distributed shared memory.  It writes the lists of free places and of tokens that move.
 // evict_move_kernel moves the rows of K and V: 4 D elements read and written per token, which is what bounds it.
 #include <cooperative_groups.h>
@@ -20,7 +20,7 @@ namespace cg = cooperative_groups;
 
 namespace inq {
 
-constexpr int kEvThreads = 512, kEvBins = 2048, kEvMaxCluster = 8;
+constexpr int kEvThreads = 512, kEvBins = 256, kEvPasses = 4, kEvMaxCluster = 8;
 
 struct EvictParams {
   void *k, *v;
@@ -44,17 +44,11 @@ __device__ __forceinline__ unsigned worth(float w) {
   return (u & 0x80000000u) ? ~u : u | 0x80000000u;
 }
 
-// Sum over the threads in front of this one, and over all of them.
-__device__ __forceinline__ int block_prefix(int mine, int& all, int* scratch /* 17 ints */) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  int sum = mine;
-#pragma unroll
-  for (int d = 1; d < 32; d <<= 1) {
-    const int other = __shfl_up_sync(0xffffffffu, sum, d);
-    if (lane >= d) sum += other;
-  }
+// Sum over the warps in front of this one, and over all of them, of a number that a warp's lanes agree on.
+__device__ __forceinline__ int warps_before(int mine, int& all, int* scratch /* one per warp */) {
+  const int warp = threadIdx.x >> 5;
   __syncthreads();
-  if (lane == 31) scratch[warp] = sum;
+  if ((threadIdx.x & 31) == 0) scratch[warp] = mine;
   __syncthreads();
   int before = 0;
   all = 0;
@@ -64,18 +58,19 @@ __device__ __forceinline__ int block_prefix(int mine, int& all, int* scratch /* 
     if (w < warp) before += n;
     all += n;
   }
-  return before + sum - mine;
+  return before;
 }
 
 // KEYS: tokens per thread whose keys stay in registers over all passes; a slice of more is read anew for each.
 template <int KEYS>
-__global__ void __launch_bounds__(kEvThreads) evict_select_kernel(const EvictParams P) {
+__global__ void __launch_bounds__(kEvThreads, KEYS <= 5 ? 2 : 1) evict_select_kernel(const EvictParams P) {
   cg::cluster_group cluster = cg::this_cluster();
   const int ctas = (int)cluster.num_blocks(), me = (int)cluster.block_rank();
   const int row = blockIdx.x / ctas, b = row / P.kv_heads, h = row % P.kv_heads, tid = threadIdx.x;
-  __shared__ __align__(16) int histogram[kEvBins];
-  __shared__ int shared_counts[3];                    // this CTA's ties, free places and moving tokens
-  __shared__ int scratch[kEvThreads / 32 + 1], chosen[2];
+  __shared__ int histograms[kEvPasses][kEvBins];      // one per pass: none is cleared while others read it
+  __shared__ int shared_counts[2];                    // this CTA's free places and moving tokens
+  __shared__ int scratch[kEvThreads / 32], chosen[kEvPasses][2];
+  const int warp = tid >> 5, lane = tid & 31;
   follow_stream();
   allow_next();
   const long long asked = P.lengths[b];
@@ -104,129 +99,146 @@ __global__ void __launch_bounds__(kEvThreads) evict_select_kernel(const EvictPar
   const int slice = (length + ctas - 1) / ctas, lo = min(me * slice, length), hi = min(lo + slice, length);
   constexpr int kGroup = kEvThreads * KEYS;
   const int groups = (hi - lo + kGroup - 1) / kGroup;
-  unsigned keys[KEYS];          // of neighbouring tokens; 0 behind the slice, where no token is looked for
+  // A warp owns 32 KEYS neighbouring tokens of a group, lane l every 32nd of them from the l-th: loads and stores of a
+  // warp are whole lines, and the order of tokens is that of (i, lane), which ballots count.
+  unsigned keys[KEYS];          // 0 behind the slice, where no token is looked for
+  int p[KEYS];
+  float x[KEYS];
+  auto first_token = [&](int g) { return lo + g * kGroup + warp * (32 * KEYS) + lane; };
   auto load = [&](int g) {
+    const int j0 = first_token(g);
 #pragma unroll
     for (int i = 0; i < KEYS; ++i) {
-      const int j = lo + g * kGroup + tid * KEYS + i;
-      keys[i] = 0u;
-      if (j < hi) {
-        const int p = __ldg(pos + j);
-        keys[i] = p < P.sink || p >= safe_from ? 0xffffffffu : worth(__ldg(w + j));
-      }
+      p[i] = j0 + 32 * i < hi ? __ldg(pos + j0 + 32 * i) : 0;
+      x[i] = j0 + 32 * i < hi ? __ldg(w + j0 + 32 * i) : 0.f;
     }
+#pragma unroll
+    for (int i = 0; i < KEYS; ++i) keys[i] = j0 + 32 * i >= hi ? 0u : p[i] < P.sink || p[i] >= safe_from ? 0xffffffffu : worth(x[i]);
   };
   if (groups <= 1) load(0);
+  for (int i = tid; i < kEvPasses * kEvBins; i += kEvThreads) histograms[0][i] = 0;
+  __syncthreads();
 
   // ---- the key of the last token that stays: `want` tokens of those that begin with `prefix` are still to be found
   unsigned prefix = 0;
   int want = budget;
 #pragma unroll 1
-  for (int pass = 0; pass < 3; ++pass) {
-    const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, above = pass == 0 ? 32 : pass == 1 ? 21 : 10;
-    const unsigned bins = pass == 2 ? 1024u : 2048u;
-    static_assert(kEvBins == 4 * kEvThreads, "a thread clears and adds four bins");
-    ((int4*)histogram)[tid] = make_int4(0, 0, 0, 0);
-    __syncthreads();
+  for (int pass = 0; pass < kEvPasses; ++pass) {
+    const int shift = 24 - 8 * pass;
+    int* const histogram = histograms[pass];
 #pragma unroll 1
     for (int g = 0; g < groups; ++g) {
       if (groups > 1) load(g);
-      const int count = hi - (lo + g * kGroup + tid * KEYS);
+      const int j0 = first_token(g);
 #pragma unroll
       for (int i = 0; i < KEYS; ++i)
-        if (i < count && (pass == 0 || keys[i] >> above == prefix)) atomicAdd(histogram + ((keys[i] >> shift) & (bins - 1)), 1);
+        if (j0 + 32 * i < hi && (pass == 0 || keys[i] >> (shift + 8) == prefix)) atomicAdd(histogram + ((keys[i] >> shift) & 255u), 1);
     }
     cluster.sync();
-    // every CTA finds the digit for itself: a thread adds four neighbouring bins over the cluster, highest bins first
-    int4 mine = make_int4(0, 0, 0, 0);
-    for (int c = 0; c < ctas; ++c) {
-      const int4 n = ((const int4*)cluster.map_shared_rank(histogram, c))[kEvThreads - 1 - tid];
-      mine = make_int4(mine.x + n.x, mine.y + n.y, mine.z + n.z, mine.w + n.w);
-    }
-    int all;
-    int before = block_prefix(mine.x + mine.y + mine.z + mine.w, all, scratch);
-    const int each[4] = {mine.w, mine.z, mine.y, mine.x};
+    // every CTA finds the digit for itself: a thread adds a bin over the cluster, the highest first
+    int mine = 0, all;
+    if (tid < kEvBins) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      if (before < want && before + each[i] >= want) {
-        chosen[0] = kEvBins - 1 - (4 * tid + i);
-        chosen[1] = want - before;
-      }
-      before += each[i];
+      for (int c = 0; c < kEvMaxCluster; ++c)
+        if (c < ctas) mine += cluster.map_shared_rank(histogram, c)[kEvBins - 1 - tid];
+    }
+    int sum = mine;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const int other = __shfl_up_sync(0xffffffffu, sum, d);
+      if (lane >= d) sum += other;
+    }
+    const int before = sum - mine + warps_before(__shfl_sync(0xffffffffu, sum, 31), all, scratch);
+    if (before < want && before + mine >= want) {
+      chosen[pass][0] = kEvBins - 1 - tid;
+      chosen[pass][1] = want - before;
     }
     __syncthreads();
-    prefix = (prefix << (pass == 2 ? 10 : 11)) | (unsigned)chosen[0];
-    want = chosen[1];
-    if (pass == 2 && tid == 0) shared_counts[0] = histogram[chosen[0]];
-    cluster.sync();       // nobody reads this CTA's histogram any more
+    prefix = prefix << 8 | (unsigned)chosen[pass][0];
+    want = chosen[pass][1];
   }
   // tokens above the threshold stay, and the first `want` of those at it
   int ties_before = 0;
-  for (int c = 0; c < me; ++c) ties_before += cluster.map_shared_rank(shared_counts, c)[0];
+  for (int c = 0; c < me; ++c) ties_before += cluster.map_shared_rank(histograms[kEvPasses - 1], c)[prefix & 255u];
 
-  // ---- twice over the slice: the free places and moving tokens of this CTA, then their lists (a CTA alone starts at zero)
-  int holes = 0, moves = 0;          // in front of the group of tokens in work
-#pragma unroll 1
-  for (int round = ctas == 1; round < 2; ++round) {
-    int ties = ties_before;
-    if (round == 1 && ctas > 1) {
-      cluster.sync();
-      holes = moves = 0;
-      for (int c = 0; c < me; ++c) {
-        holes += cluster.map_shared_rank(shared_counts, c)[1];
-        moves += cluster.map_shared_rank(shared_counts, c)[2];
-      }
+  // ---- which tokens stay; the free places and moving tokens, counted over the slice and then listed
+  const unsigned behind = (1u << lane) - 1u;        // lanes in front of this one
+  unsigned kept = 0;
+  int ties = ties_before, holes = 0, moves = 0, mine_before = 0;        // of the groups in front of the one in work, and inside it
+  int group_holes = 0, group_moves = 0;
+  auto decide = [&](int g) {
+    const int j0 = first_token(g);
+    int equal = 0, all_equal, all_packed;
+#pragma unroll
+    for (int i = 0; i < KEYS; ++i) equal += __popc(__ballot_sync(0xffffffffu, j0 + 32 * i < hi && keys[i] == prefix));
+    int rank = ties + warps_before(equal, all_equal, scratch), mine_holes = 0, mine_moves = 0;
+    ties += all_equal;
+    kept = 0;
+#pragma unroll
+    for (int i = 0; i < KEYS; ++i) {
+      const int j = j0 + 32 * i;
+      const bool tie = j < hi && keys[i] == prefix;
+      const unsigned tied = __ballot_sync(0xffffffffu, tie);
+      const bool stays = j < hi && (keys[i] > prefix || (tie && rank + __popc(tied & behind) < want));
+      rank += __popc(tied);
+      kept |= (unsigned)stays << i;
+      mine_holes += __popc(__ballot_sync(0xffffffffu, j < left && j < hi && !stays));
+      mine_moves += __popc(__ballot_sync(0xffffffffu, j >= left && stays));
     }
-#pragma unroll 1
+    mine_before = warps_before(mine_holes | (mine_moves << 16), all_packed, scratch);
+    group_holes = all_packed & 0xffff;
+    group_moves = all_packed >> 16;
+  };
+  if (groups == 1) {
+    decide(0);
+  } else {
     for (int g = 0; g < groups; ++g) {
-      if (groups > 1) load(g);
-      const int j0 = lo + g * kGroup + tid * KEYS, count = hi - j0;
-      int equal = 0, all_equal;
-#pragma unroll
-      for (int i = 0; i < KEYS; ++i) equal += i < count && keys[i] == prefix;
-      int rank = ties + block_prefix(equal, all_equal, scratch);
-      ties += all_equal;
-      unsigned kept = 0;
-      int mine_holes = 0, mine_moves = 0;
-#pragma unroll
-      for (int i = 0; i < KEYS; ++i) {
-        const bool tie = keys[i] == prefix, stays = i < count && (keys[i] > prefix || (tie && rank < want));
-        rank += i < count && tie;
-        kept |= (unsigned)stays << i;
-        mine_holes += i < count && !stays && j0 + i < left;
-        mine_moves += stays && j0 + i >= left;
-      }
-      int all_packed;
-      const int packed = block_prefix(mine_holes | (mine_moves << 16), all_packed, scratch);
-      if (round == 1) {
-        int hole = holes + (packed & 0xffff), move = moves + (packed >> 16);
-#pragma unroll
-        for (int i = 0; i < KEYS; ++i) {
-          const int j = j0 + i;
-          if (i >= count) continue;
-          const bool stays = (kept >> i) & 1u;
-          if (j < left) {
-            if (stays) {
-              out_w[j] = w[j];
-              out_p[j] = pos[j];
-            } else {
-              list[1 + hole++] = j;
-            }
-          } else if (stays) {
-            list[1 + P.list_columns + move++] = j;
-          }
-        }
-      }
-      holes += all_packed & 0xffff;
-      moves += all_packed >> 16;
+      load(g);
+      decide(g);
+      holes += group_holes;
+      moves += group_moves;
     }
-    if (round == 0) {
-      __syncthreads();
-      if (tid == 0) {
-        shared_counts[1] = holes;
-        shared_counts[2] = moves;
+  }
+  if (ctas > 1) {
+    if (tid == 0) {
+      shared_counts[0] = groups == 1 ? group_holes : holes;
+      shared_counts[1] = groups == 1 ? group_moves : moves;
+    }
+    cluster.sync();
+  }
+  holes = moves = 0;
+#pragma unroll
+  for (int c = 0; c < kEvMaxCluster - 1; ++c) {
+    if (c < me) {
+      holes += cluster.map_shared_rank(shared_counts, c)[0];
+      moves += cluster.map_shared_rank(shared_counts, c)[1];
+    }
+  }
+  ties = ties_before;
+#pragma unroll 1
+  for (int g = 0; g < groups; ++g) {
+    if (groups > 1) {
+      load(g);
+      decide(g);
+    }
+    const int j0 = first_token(g);
+    int hole = holes + (mine_before & 0xffff), move = moves + (mine_before >> 16);
+#pragma unroll
+    for (int i = 0; i < KEYS; ++i) {
+      const int j = j0 + 32 * i;
+      const bool stays = (kept >> i) & 1u, free = j < left && j < hi && !stays, moving = j >= left && stays;
+      const unsigned all_free = __ballot_sync(0xffffffffu, free), all_moving = __ballot_sync(0xffffffffu, moving);
+      if (free) list[1 + hole + __popc(all_free & behind)] = j;
+      if (moving) list[1 + P.list_columns + move + __popc(all_moving & behind)] = j;
+      hole += __popc(all_free);
+      move += __popc(all_moving);
+      if (j < left && stays) {
+        out_w[j] = x[i];
+        out_p[j] = p[i];
       }
     }
+    holes += group_holes;
+    moves += group_moves;
   }
   if (me == ctas - 1 && tid == 0) list[0] = moves;
   cluster.sync();       // the counts of a CTA are read until here
@@ -331,10 +343,10 @@ extern "C" int inq_evict_tokens(const inq_evict_args_t* a, inq_stream_t stream_)
     config.stream = stream;
     config.attrs = attrs;
     config.numAttrs = 2;
-    // keys of a slice in registers where 16 per thread do; fewer registers where 4 do
+    // the keys of a slice in registers where 16 per thread do, in fewer where a power of two and some slack fit
     const long long slice = (P.capacity + ctas - 1) / ctas;
-    INQ_CUDA_CHECK(slice <= 4 * kEvThreads ? cudaLaunchKernelEx(&config, evict_select_kernel<4>, P)
-                                           : slice <= 8 * kEvThreads ? cudaLaunchKernelEx(&config, evict_select_kernel<8>, P)
+    INQ_CUDA_CHECK(slice <= 5 * kEvThreads ? cudaLaunchKernelEx(&config, evict_select_kernel<5>, P)
+                                           : slice <= 9 * kEvThreads ? cudaLaunchKernelEx(&config, evict_select_kernel<9>, P)
                                                                      : cudaLaunchKernelEx(&config, evict_select_kernel<16>, P));
   }
   // as many tokens move as places fall free, at most, and as there are behind the budget
