@@ -7,13 +7,15 @@
 //     one list, cut into equal ranges, one per CTA and one CTA per SM.  The lengths are read on the device, so that a
 //     captured step serves every later length; a pair that no range cuts is finished by its CTA.
 //   * a warp owns 16 tokens of every unit and everything about them: its own ring of asynchronous copies, both
-//     contractions (mma.sync m16n8k16: query heads as rows), its own running maximum, sum and output.  Warps meet
-//     only where their CTA's range of a pair ends; until then no barrier keeps a load waiting.
+//     contractions (mma.sync m16n8k16), its own running maximum, sum and output.  Warps meet only where their CTA's
+//     range of a pair ends; until then no barrier keeps a load waiting.
 // mma.sync suffices: per 512 bytes of a token it computes 8192 operations, a tenth of what the SM could do meanwhile.
+// The parts of a pair that ranges cut are joined, in their order, by the CTA that hands in the last one.
 //
-// A second launch joins the parts of pairs that ranges cut, in their order, and, where weights are asked for, turns the
-// logits that the first one left into them: out_w_j = w_j + sum_g 2^(s_gj - lse_g).
+// Where weights are asked for, a second launch turns the logits that the first one left into them:
+// out_w_j = w_j + sum_g 2^(s_gj - lse_g).
 #include <algorithm>
+#include <atomic>
 
 #include "attention.cuh"
 
@@ -39,6 +41,7 @@ struct DensePagedParams {
   long long w_sb, w_sh, ow_sb, ow_sh;
   float* records;      // [part + pair][rows][D + 2]: unnormalised output, maximum, sum
   float* logits;       // [request][query head][capacity], base 2
+  int* counters;       // [pair]: parts handed in, zero between launches
   long long capacity;
   float scale_log2e;
   int* status;
@@ -159,6 +162,12 @@ __device__ __forceinline__ void dp_mma(float (&c)[4], unsigned a0, unsigned a1, 
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
+__device__ __forceinline__ unsigned dp_transpose(unsigned x) {
+  unsigned y;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
+
 template <int D>
 struct DensePagedShape {
   static constexpr int kRowBytes = 2 * D, kChunks = D / 8;              // 16-byte chunks of a row
@@ -169,11 +178,55 @@ struct DensePagedShape {
   static constexpr int kSmem = kRing + kExchange + kDpWarps * 16 * 2 * 4;
 };
 
-// ROWS: query heads of a pair that the kernel holds, 8 (rows 8 to 15 of the contractions are empty) or 16
-template <typename QT, int D, int ROWS, bool WEIGHTS>
+// Reference maximum and sum of a row over n parts, the same in every lane; the whole warp takes part.
+__device__ __forceinline__ float2 join_sums(const float* first, long long stride, int n) {
+  const int lane = threadIdx.x & 31;
+  float top = kDpNegBig, sum = 0.f;
+  for (int c = lane; c < n; c += 32) {
+    const float2 ml = __ldcg((const float2*)(first + c * stride));
+    const float next = fmaxf(top, ml.x);
+    sum = sum * pf_exp2(top - next) + ml.y * pf_exp2(ml.x - next);
+    top = next;
+  }
+#pragma unroll
+  for (int d = 16; d; d >>= 1) {
+    const float other_top = __shfl_xor_sync(0xffffffffu, top, d), other = __shfl_xor_sync(0xffffffffu, sum, d);
+    const float next = fmaxf(top, other_top);
+    sum = sum * pf_exp2(top - next) + other * pf_exp2(other_top - next);
+    top = next;
+  }
+  return make_float2(top, sum);
+}
+// A row of a cut pair: out = sum_c O_c 2^(m_c - m) / sum_c l_c 2^(m_c - m) over its n parts.  A warp, D / 32 channels a lane.
+template <typename QT, int D>
+__device__ __forceinline__ void join_row(const float* rec, long long stride, int n, QT* out) {
+  constexpr int kEach = D / 32;
+  const int lane = threadIdx.x & 31;
+  const float2 whole = join_sums(rec + D, stride, n);
+  float sum[kEach] = {};
+#pragma unroll 8
+  for (int c = 0; c < n; ++c) {
+    const float f = pf_exp2(__ldcg(rec + c * stride + D) - whole.x);
+#pragma unroll
+    for (int i = 0; i < kEach; i += 2) {
+      const float2 x = __ldcg((const float2*)(rec + c * stride + kEach * lane + i));
+      sum[i] = fmaf(x.x, f, sum[i]);
+      sum[i + 1] = fmaf(x.y, f, sum[i + 1]);
+    }
+  }
+  const float inv = whole.y == 0.f ? 0.f : 1.f / whole.y;
+#pragma unroll
+  for (int i = 0; i < kEach; i += 2) *(unsigned*)(out + kEach * lane + i) = pf_pack2<QT>(sum[i] * inv, sum[i + 1] * inv);
+}
+
+// TILES: query heads of a pair that the kernel holds, in eights.  Both contractions take the cache as their left operand,
+// S^T = K Q^T (16 tokens x 8 heads) and O^T = V^T P^T (16 channels x 8 heads): the query heads of one KV head are few, and as
+// rows of a 16-row operand half of them would be empty.  The probabilities change places between the two by movmatrix.
+template <typename QT, int D, int TILES, bool WEIGHTS>
 __global__ void __launch_bounds__(kDpThreads, 1) paged_kernel(const DensePagedParams P) {
   using S = DensePagedShape<D>;
   constexpr int kStages = S::kStages, kCopies = kDpSlice * S::kChunks / 32;      // 16-byte copies of a lane per K or V slice
+  constexpr int kRowsAtOnce = 32 / S::kChunks;
   extern __shared__ __align__(1024) unsigned char dp_raw[];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const unsigned ring = tc_smem(dp_raw) + warp * kStages * S::kSliceBytes;
@@ -182,6 +235,11 @@ __global__ void __launch_bounds__(kDpThreads, 1) paged_kernel(const DensePagedPa
   follow_stream();
   if (blockIdx.x == 0 && tid < 32)
     for (int b = tid; b < P.requests; b += 32) load_request(P, b, true);
+  // requests with nothing to attend to: zeros
+  for (int b = blockIdx.x; b < P.requests; b += gridDim.x)
+    if (load_request(P, b).units == 0)
+      for (int i = tid; i < P.q_heads * S::kChunks; i += kDpThreads)
+        *(uint4*)((QT*)P.out + b * P.o_sb + (long long)(i / S::kChunks) * P.o_sh + i % S::kChunks * 8) = make_uint4(0u, 0u, 0u, 0u);
   long long unused;
   const long long total = count_units(P, 0, unused);
   const int ctas = range_count(total, gridDim.x);
@@ -190,6 +248,7 @@ __global__ void __launch_bounds__(kDpThreads, 1) paged_kernel(const DensePagedPa
   const long long w0 = range_start(total, blockIdx.x, ctas), w1 = range_start(total, blockIdx.x + 1, ctas);
   Cursor at = seek(P, w0), ahead = at;         // the unit in work and the one to ask for next
   const int count = (int)(w1 - w0);
+  const bool whole = P.page_tokens % kDpSlice == 0;     // a slice lies in one page
 
   // Physical page of the row that lane & 15 stands for, or -1.
   auto look_up = [&](const Cursor& c) {
@@ -201,24 +260,43 @@ __global__ void __launch_bounds__(kDpThreads, 1) paged_kernel(const DensePagedPa
     atomicOr(P.status, INQ_STATUS_BAD_INDEX);
     return -1;
   };
-  // Asks for the slice of unit `c` into a stage; returns the rows that it holds.
+  const int chunk = lane % S::kChunks, row0 = lane / S::kChunks;       // this lane copies chunk `chunk` of rows row0 + kRowsAtOnce i
+  // Asks for the slice of unit `c` into a stage; returns the rows that it holds.  Rows that there are not, and those of a
+  // page outside the pool, are filled with zeros: a masked token's weight is zero, which is no help against what
+  // memory may hold there.
   auto request = [&](const Cursor& c, int page, int stage) {
-    const int t0 = c.unit * kDpUnit + warp * kDpSlice, row = lane & 15, t = t0 + row;
-    const int kvh = c.pair / P.chunks;
-    const bool is_new = t == c.r.fresh;
-    const unsigned valid = __ballot_sync(0xffffffffu, page >= 0 || (is_new && t < c.r.tokens)) & 0xffffu;
-    // rows that there are not, and those of a page outside the pool, are filled with zeros: a masked token's weight is
-    // zero, which is no help against what memory may hold there
-    if (t0 < c.r.tokens) {
+    const int t0 = c.unit * kDpUnit + warp * kDpSlice, kvh = c.pair / P.chunks;
+    const unsigned dst = ring + stage * S::kSliceBytes;
+    unsigned valid = 0;
+    if (whole && t0 + kDpSlice <= c.r.tokens && (c.r.fresh < t0 || c.r.fresh >= t0 + kDpSlice)) {
+      // 16 tokens of one page
+      const long long p = max(page, 0);
+      const int o = (P.page_shift >= 0 ? t0 & (P.page_tokens - 1) : t0 % P.page_tokens) + row0;
+      const char* ks = (const char*)P.k + 2 * (p * P.k_sp + kvh * P.k_sh + o * P.k_st + 8 * chunk);
+      const char* vs = (const char*)P.v + 2 * (p * P.v_sp + kvh * P.v_sh + o * P.v_st + 8 * chunk);
+      const long long kstep = 2 * kRowsAtOnce * P.k_st, vstep = 2 * kRowsAtOnce * P.v_st;
+      const bool have = page >= 0;
+#pragma unroll
+      for (int i = 0; i < kCopies; ++i) {
+        const unsigned to = dst + (row0 + i * kRowsAtOnce) * S::kRowBytes + ((chunk ^ ((row0 + i * kRowsAtOnce) & 7)) << 4);
+        dp_copy16(to, ks, have);
+        dp_copy16(to + kDpSlice * S::kRowBytes, vs, have);
+        ks += kstep;
+        vs += vstep;
+      }
+      valid = have ? 0xffffu : 0u;
+    } else if (t0 < c.r.tokens) {
+      // any row may lie in a page of its own, or be the new token's
+      const int t = t0 + (lane & 15);
+      const bool is_new = t == c.r.fresh;
+      valid = __ballot_sync(0xffffffffu, page >= 0 || (is_new && t < c.r.tokens)) & 0xffffu;
       const long long p = max(page, 0);
       const int o = P.page_shift >= 0 ? t & (P.page_tokens - 1) : t % P.page_tokens;
       const QT* const kr = is_new ? (const QT*)P.new_k + c.b * P.n_sb + kvh * P.n_sh : (const QT*)P.k + p * P.k_sp + kvh * P.k_sh + o * P.k_st;
       const QT* const vr = is_new ? (const QT*)P.new_v + c.b * P.m_sb + kvh * P.m_sh : (const QT*)P.v + p * P.v_sp + kvh * P.v_sh + o * P.v_st;
-      const unsigned dst = ring + stage * S::kSliceBytes;
-      const int chunk = lane % S::kChunks;
-#pragma unroll
+#pragma unroll 1
       for (int i = 0; i < kCopies; ++i) {
-        const int r = i * (32 / S::kChunks) + lane / S::kChunks;
+        const int r = row0 + i * kRowsAtOnce;
         const QT* const ks = (const QT*)__shfl_sync(0xffffffffu, (unsigned long long)kr, r);
         const QT* const vs = (const QT*)__shfl_sync(0xffffffffu, (unsigned long long)vr, r);
         const unsigned to = dst + r * S::kRowBytes + ((chunk ^ (r & 7)) << 4);
@@ -247,10 +325,11 @@ __global__ void __launch_bounds__(kDpThreads, 1) paged_kernel(const DensePagedPa
   unsigned long long rows_ahead = 0;        // 16 bits per requested slice, the oldest lowest
   constexpr int kAhead = kStages - 1;      // slices requested in front of the one in work
   static_assert(kAhead <= 3, "16 bits per slice, and the one in work");
-  int page = look_up(ahead), asked = 0;
+  int page = look_up(ahead), asked = 0, ask_stage = 0, stage = 0;
   auto ask = [&]() {
     if (asked < count) {
-      const unsigned valid = request(ahead, page, asked % kStages);
+      const unsigned valid = request(ahead, page, ask_stage);
+      ask_stage = ask_stage + 1 == kStages ? 0 : ask_stage + 1;
       rows_ahead |= (unsigned long long)valid << (16 * kAhead);
       if (++asked < count) {
         advance(P, ahead);
@@ -265,28 +344,28 @@ __global__ void __launch_bounds__(kDpThreads, 1) paged_kernel(const DensePagedPa
     rows_ahead >>= 16;
   }
 
-  unsigned qf[D / 16][ROWS == 16 ? 4 : 2];
-  float o[D / 8][4], m[2], l[2];
+  unsigned qf[TILES][D / 16][2];                // query heads as right operands
+  float o[TILES][D / 16][4], m[TILES][2], l[TILES][2];      // heads 8 i + 2 (lane & 3) (+ 1)
+  const int c0 = 2 * (lane & 3), g = lane >> 2;
   bool first = true;
   for (int done = 0; done < count; ++done) {
+    const int h0 = at.pair / P.chunks * P.group + at.pair % P.chunks * 16, rows = min(P.group - at.pair % P.chunks * 16, 16);
     if (first) {
-      // a new pair: its query rows as the left operand (rows beyond the group are zero), an empty state
+      // a new pair: its query rows (those beyond the group are zero), an empty state
       first = false;
-      const int h0 = at.pair / P.chunks * P.group + at.pair % P.chunks * 16, rows = min(P.group - at.pair % P.chunks * 16, 16);
 #pragma unroll
-      for (int half = 0; half < ROWS / 8; ++half) {
-        const int r = (lane >> 2) + 8 * half;
-        const QT* const src = (const QT*)P.q + at.b * P.q_sb + (long long)(h0 + min(r, rows - 1)) * P.q_sh + 2 * (lane & 3);
+      for (int i = 0; i < TILES; ++i) {
+        const int r = g + 8 * i;
+        const QT* const src = (const QT*)P.q + at.b * P.q_sb + (long long)(h0 + min(r, rows - 1)) * P.q_sh + c0;
 #pragma unroll
         for (int kk = 0; kk < D / 16; ++kk) {
-          qf[kk][half] = r < rows ? *(const unsigned*)(src + 16 * kk) : 0u;
-          qf[kk][half + ROWS / 8] = r < rows ? *(const unsigned*)(src + 16 * kk + 8) : 0u;
+          qf[i][kk][0] = r < rows ? *(const unsigned*)(src + 16 * kk) : 0u;
+          qf[i][kk][1] = r < rows ? *(const unsigned*)(src + 16 * kk + 8) : 0u;
+          o[i][kk][0] = o[i][kk][1] = o[i][kk][2] = o[i][kk][3] = 0.f;
         }
+        m[i][0] = m[i][1] = kDpNegBig;
+        l[i][0] = l[i][1] = 0.f;
       }
-#pragma unroll
-      for (int i = 0; i < D / 8; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
-      m[0] = m[1] = kDpNegBig;
-      l[0] = l[1] = 0.f;
     }
     ask();
     const unsigned valid = (unsigned)rows_ahead & 0xffffu;
@@ -294,97 +373,104 @@ __global__ void __launch_bounds__(kDpThreads, 1) paged_kernel(const DensePagedPa
     dp_wait<kAhead>();
     __syncwarp();
     if (at.unit * kDpUnit + warp * kDpSlice < at.r.tokens) {
-      const unsigned kbase = ring + (done % kStages) * S::kSliceBytes, vbase = kbase + kDpSlice * S::kRowBytes;
-      float s[2][4] = {};
-      // matrices of a load: tokens 0-7 and 8-15 of 16 channels, as right operands of both token tiles
-      const int krow = (lane & 7) + ((lane >> 4) << 3), kc = (lane >> 3) & 1;
+      const unsigned kbase = ring + stage * S::kSliceBytes, vbase = kbase + kDpSlice * S::kRowBytes;
+      // two chains per tile of heads, so that a contraction does not wait for the one before it
+      float s[TILES][2][4] = {};
+      const int krow = lane & 15, kc = lane >> 4;
 #pragma unroll
       for (int kk = 0; kk < D / 16; ++kk) {
-        unsigned b[4];
-        dp_ldm4(b, kbase + krow * S::kRowBytes + (((2 * kk + kc) ^ (krow & 7)) << 4));
-        const unsigned a0 = qf[kk][0], a1 = ROWS == 16 ? qf[kk][1] : 0u, a2 = qf[kk][ROWS / 8], a3 = ROWS == 16 ? qf[kk][ROWS / 8 + 1] : 0u;
-        dp_mma<QT>(s[0], a0, a1, a2, a3, b[0], b[1]);
-        dp_mma<QT>(s[1], a0, a1, a2, a3, b[2], b[3]);
+        unsigned a[4];
+        dp_ldm4(a, kbase + krow * S::kRowBytes + (((2 * kk + kc) ^ (krow & 7)) << 4));
+#pragma unroll
+        for (int i = 0; i < TILES; ++i) dp_mma<QT>(s[i][kk & 1], a[0], a[1], a[2], a[3], qf[i][kk][0], qf[i][kk][1]);
       }
-      const int c0 = 2 * (lane & 3);
+      unsigned p[TILES][2];
 #pragma unroll
-      for (int n = 0; n < 2; ++n)
+      for (int i = 0; i < TILES; ++i) {
+        float x[4];       // tokens g (0, 1) and g + 8 (2, 3)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          s[n][e] *= P.scale_log2e;
-          if (!((valid >> (8 * n + c0 + (e & 1))) & 1u)) s[n][e] = __int_as_float(0xff800000);
+        for (int e = 0; e < 4; ++e) x[e] = (s[i][0][e] + s[i][1][e]) * P.scale_log2e;
+        if (valid != 0xffffu) {
+          if (!((valid >> g) & 1u)) x[0] = x[1] = __int_as_float(0xff800000);
+          if (!((valid >> (g + 8)) & 1u)) x[2] = x[3] = __int_as_float(0xff800000);
         }
-      if (WEIGHTS) {
-        const int rows = min(P.group - at.pair % P.chunks * 16, 16), t = at.unit * kDpUnit + warp * kDpSlice + c0;
-        const int h0 = at.pair / P.chunks * P.group + at.pair % P.chunks * 16;
+        if (WEIGHTS) {
+          const int t = at.unit * kDpUnit + warp * kDpSlice + g;
+          float* const to = P.logits + ((long long)at.b * P.q_heads + h0 + 8 * i + c0) * P.capacity + t;
 #pragma unroll
-        for (int half = 0; half < ROWS / 8; ++half) {
-          const int r = (lane >> 2) + 8 * half;
-          if (r < rows) {
-            float* const to = P.logits + ((long long)at.b * P.q_heads + h0 + r) * P.capacity + t;
+          for (int e = 0; e < 4; ++e)
+            if (8 * i + c0 + (e & 1) < rows && t + 4 * (e & 2) < at.r.tokens) to[(e & 1) * P.capacity + 4 * (e & 2)] = x[e];
+        }
+        float top[2];
 #pragma unroll
-            for (int n = 0; n < 2; ++n) {
-              if (t + 8 * n < at.r.tokens) to[8 * n] = s[n][2 * half];
-              if (t + 8 * n + 1 < at.r.tokens) to[8 * n + 1] = s[n][2 * half + 1];
-            }
+        for (int e = 0; e < 2; ++e) {
+          top[e] = fmaxf(x[e], x[e + 2]);
+          top[e] = fmaxf(top[e], __shfl_xor_sync(0xffffffffu, top[e], 4));
+          top[e] = fmaxf(top[e], __shfl_xor_sync(0xffffffffu, top[e], 8));
+          top[e] = fmaxf(top[e], __shfl_xor_sync(0xffffffffu, top[e], 16));
+        }
+        if (__any_sync(0xffffffffu, top[0] > m[i][0] + kDpSlack || top[1] > m[i][1] + kDpSlack)) {
+          float factor[2];
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const float next = top[e] > m[i][e] + kDpSlack ? top[e] : m[i][e];
+            factor[e] = pf_exp2(m[i][e] - next);
+            m[i][e] = next;
+            l[i][e] *= factor[e];
+          }
+#pragma unroll
+          for (int kk = 0; kk < D / 16; ++kk) {
+            o[i][kk][0] *= factor[0];
+            o[i][kk][1] *= factor[1];
+            o[i][kk][2] *= factor[0];
+            o[i][kk][3] *= factor[1];
           }
         }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[e] = pf_exp2(x[e] - m[i][e & 1]);
+        l[i][0] += x[0] + x[2];
+        l[i][1] += x[1] + x[3];
+        // rounded once, the sums are not; tokens change from rows to columns
+        p[i][0] = dp_transpose(pf_pack2<QT>(x[0], x[1]));
+        p[i][1] = dp_transpose(pf_pack2<QT>(x[2], x[3]));
       }
-      unsigned p[2][2] = {};
+      // matrices of a transposed load: channels 16 kk .. and 16 kk + 8 .. of tokens 0-7, then of tokens 8-15
+      const int vrow = (lane & 7) + ((lane >> 4) << 3), vc = (lane >> 3) & 1;
 #pragma unroll
-      for (int half = 0; half < ROWS / 8; ++half) {
-        float top = fmaxf(fmaxf(s[0][2 * half], s[0][2 * half + 1]), fmaxf(s[1][2 * half], s[1][2 * half + 1]));
-        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-        const bool raise = top > m[half] + kDpSlack;
-        if (__any_sync(0xffffffffu, raise)) {
-          const float next = raise ? top : m[half], factor = pf_exp2(m[half] - next);
-          m[half] = next;
-          l[half] *= factor;
+      for (int kk = 0; kk < D / 16; ++kk) {
+        unsigned a[4];
+        dp_ldm4t(a, vbase + vrow * S::kRowBytes + (((2 * kk + vc) ^ (vrow & 7)) << 4));
 #pragma unroll
-          for (int i = 0; i < D / 8; ++i) {
-            o[i][2 * half] *= factor;
-            o[i][2 * half + 1] *= factor;
-          }
-        }
-#pragma unroll
-        for (int n = 0; n < 2; ++n) {
-          const float e0 = pf_exp2(s[n][2 * half] - m[half]), e1 = pf_exp2(s[n][2 * half + 1] - m[half]);
-          l[half] += e0 + e1;
-          p[n][half] = pf_pack2<QT>(e0, e1);      // rounded once, the sum is not
-        }
-      }
-      // matrices of a transposed load: tokens 0-7 and 8-15 of channels 16 i .. and 16 i + 8 ..
-      const int vrow = lane & 15, vc = lane >> 4;
-#pragma unroll
-      for (int i = 0; i < D / 16; ++i) {
-        unsigned b[4];
-        dp_ldm4t(b, vbase + vrow * S::kRowBytes + (((2 * i + vc) ^ (vrow & 7)) << 4));
-        dp_mma<QT>(o[2 * i], p[0][0], p[0][1], p[1][0], p[1][1], b[0], b[1]);
-        dp_mma<QT>(o[2 * i + 1], p[0][0], p[0][1], p[1][0], p[1][1], b[2], b[3]);
+        for (int i = 0; i < TILES; ++i) dp_mma<QT>(o[i][kk], a[0], a[1], a[2], a[3], p[i][0], p[i][1]);
       }
     }
     __syncwarp();        // the stage may be asked for again
+    stage = stage + 1 == kStages ? 0 : stage + 1;
     const bool pair_ends = at.unit + 1 == at.r.units;
     if (pair_ends || done + 1 == count) {
       // ---- this CTA's part of the pair: the warps' states joined, a record or, where it is the whole pair, the output
 #pragma unroll
-      for (int half = 0; half < ROWS / 8; ++half) {
-        l[half] += __shfl_xor_sync(0xffffffffu, l[half], 1);
-        l[half] += __shfl_xor_sync(0xffffffffu, l[half], 2);
-        if ((lane & 3) == 0) *(float2*)(ml + 2 * (warp * 16 + (lane >> 2) + 8 * half)) = make_float2(m[half], l[half]);
-      }
+      for (int i = 0; i < TILES; ++i)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          l[i][e] += __shfl_xor_sync(0xffffffffu, l[i][e], 4);
+          l[i][e] += __shfl_xor_sync(0xffffffffu, l[i][e], 8);
+          l[i][e] += __shfl_xor_sync(0xffffffffu, l[i][e], 16);
+          if (lane < 4) *(float2*)(ml + 2 * (warp * 16 + 8 * i + c0 + e)) = make_float2(m[i][e], l[i][e]);
+        }
       const bool alone = pair_ends && done >= at.unit;      // every unit of the pair was in this range
-      const int h0 = at.pair / P.chunks * P.group + at.pair % P.chunks * 16, rows = min(P.group - at.pair % P.chunks * 16, 16);
-      const long long record = blockIdx.x + (long long)at.b * P.kv_heads * P.chunks + at.pair;
+      const long long pair = (long long)at.b * P.kv_heads * P.chunks + at.pair;
 #pragma unroll
-      for (int half = 0; half < ROWS / 8; ++half) {
-        const int g = lane >> 2;
+      for (int i = 0; i < TILES; ++i) {
 #pragma unroll
-        for (int i = 0; i < D / 8; ++i)
-          *(float2*)(exchange + (warp * 8 + g) * D + ((8 * i + 2 * (lane & 3)) ^ (4 * g))) = make_float2(o[i][2 * half], o[i][2 * half + 1]);
+        for (int kk = 0; kk < D / 16; ++kk)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int r = c0 + (e & 1);
+            exchange[(warp * 8 + r) * D + ((16 * kk + g + 4 * (e & 2)) ^ (4 * r))] = o[i][kk][e];
+          }
         __syncthreads();
-        const int r = tid / (D / 4), c = 4 * (tid % (D / 4)), row = r + 8 * half;
+        const int r = tid / (D / 4), c = 4 * (tid % (D / 4)), row = r + 8 * i;
         if (r < 8 && row < rows) {
           float2 each[kDpWarps];
           float top = kDpNegBig;
@@ -405,7 +491,7 @@ __global__ void __launch_bounds__(kDpThreads, 1) paged_kernel(const DensePagedPa
             sum.z = fmaf(x.z, f, sum.z);
             sum.w = fmaf(x.w, f, sum.w);
           }
-          float* const rec = P.records + (record * 16 + row) * (D + 2);
+          float* const rec = P.records + ((blockIdx.x + pair) * 16 + row) * (D + 2);
           if (c == 0) *(float2*)(rec + D) = make_float2(top, weight);
           if (alone) {
             const float inv = weight == 0.f ? 0.f : 1.f / weight;
@@ -418,129 +504,80 @@ __global__ void __launch_bounds__(kDpThreads, 1) paged_kernel(const DensePagedPa
         }
         __syncthreads();
       }
+      if (!alone) {
+        // the CTA that hands in the last part joins them all, in their order, and leaves the counter as it found it
+        const long long u0 = w0 + done - at.unit;
+        const int part0 = range_of(total, u0, ctas), parts = range_of(total, u0 + at.r.units - 1, ctas) - part0 + 1;
+        __threadfence();
+        __syncthreads();
+        int* const last = (int*)ml;
+        if (tid == 0) {
+          const bool is_last = atomicAdd(P.counters + pair, 1) == parts - 1;
+          if (is_last) P.counters[pair] = 0;
+          *last = is_last;
+        }
+        __syncthreads();
+        const bool joins = *last != 0;
+        if (joins) {
+          __threadfence();
+          for (int row = warp; row < rows; row += kDpWarps)
+            join_row<QT, D>(P.records + ((part0 + pair) * 16 + row) * (D + 2), 16 * (D + 2), parts,
+                            (QT*)P.out + at.b * P.o_sb + (long long)(h0 + row) * P.o_sh);
+        }
+        __syncthreads();
+      }
       first = true;
     }
     if (done + 1 < count) advance(P, at);
   }
 }
 
-// Joins the parts of pairs that ranges cut.  The first requests x query heads blocks take a row each; with weights,
-// further blocks take 512 tokens of a KV head each.  A part's maximum and sum are read by a thread each, 32 at a time, and
-// its output by D / 4 threads, 512 / D parts at once.
-constexpr int kDpJoinThreads = 128, kDpJoinEach = 4, kDpJoinTokens = kDpJoinThreads * kDpJoinEach;
-// Reference maximum and sum of a row over its parts c0 .. c0 + n - 1, the same in every lane; the whole warp takes part.
-__device__ __forceinline__ float2 join_sums(const float* first, long long stride, int n) {
-  const int lane = threadIdx.x & 31;
-  float top = kDpNegBig, sum = 0.f;
-  for (int c = lane; c < n; c += 32) {
-    const float2 ml = __ldcg((const float2*)(first + c * stride));
-    const float next = fmaxf(top, ml.x);
-    sum = sum * pf_exp2(top - next) + ml.y * pf_exp2(ml.x - next);
-    top = next;
-  }
-#pragma unroll
-  for (int d = 16; d; d >>= 1) {
-    const float other_top = __shfl_xor_sync(0xffffffffu, top, d), other = __shfl_xor_sync(0xffffffffu, sum, d);
-    const float next = fmaxf(top, other_top);
-    sum = sum * pf_exp2(top - next) + other * pf_exp2(other_top - next);
-    top = next;
-  }
-  return make_float2(top, sum);
-}
-template <typename QT, int D>
-__global__ void __launch_bounds__(kDpJoinThreads) paged_join_kernel(const DensePagedParams P, int most_ctas, int weight_blocks) {
-  constexpr int kAtOnce = 4 * kDpJoinThreads / D, kStride = 16 * (D + 2);
-  __shared__ float4 partial[kAtOnce][D / 4];
+// Accumulated weights: out_w_t = w_t + sum_g 2^(s_gt - lse_g), from the logits that the launch before this one left and the
+// maxima and sums of its parts.  A block takes 512 tokens of a KV head.
+constexpr int kDpWeightThreads = 128, kDpWeightEach = 4, kDpWeightTokens = kDpWeightThreads * kDpWeightEach;
+template <int D>
+__global__ void __launch_bounds__(kDpWeightThreads) paged_weights_kernel(const DensePagedParams P, int most_ctas, int blocks) {
+  constexpr int kStride = 16 * (D + 2);
   __shared__ float lse_s[64];
   follow_stream();
-  const int tid = threadIdx.x, warp = tid >> 5, rows_in_all = P.requests * P.q_heads;
-  const bool row_block = (int)blockIdx.x < rows_in_all;
-  const int job = row_block ? blockIdx.x : blockIdx.x - rows_in_all;
-  const int b = row_block ? job / P.q_heads : job / (P.kv_heads * weight_blocks);
+  const int tid = threadIdx.x, warp = tid >> 5, kvh = blockIdx.x / blocks % P.kv_heads, b = blockIdx.x / (blocks * P.kv_heads);
+  const int t0 = blockIdx.x % blocks * kDpWeightTokens;
   const Request r = load_request(P, b);
-  const int per = P.kv_heads * P.chunks;
-  if (r.units == 0) {
-    // nothing to attend to: zeros, and no weight
-    const int head = job % P.q_heads;
-    if (row_block && tid < D) ((QT*)P.out)[b * P.o_sb + (long long)head * P.o_sh + tid] = from_float<QT>(0.f);
-    return;
-  }
-  const int t0 = row_block ? 0 : job % weight_blocks * kDpJoinTokens;
   if (t0 >= r.tokens) return;
+  float sums[kDpWeightEach];
+#pragma unroll
+  for (int i = 0; i < kDpWeightEach; ++i) {
+    const int t = t0 + tid + i * kDpWeightThreads;
+    sums[i] = P.weights && t < r.tokens && t != r.fresh ? P.weights[b * P.w_sb + kvh * P.w_sh + t] : 0.f;
+  }
   long long before;
   const long long total = count_units(P, b, before);
   const int ctas = range_count(total, most_ctas);
-  // parts of a pair: record of part c is c + pair
-  auto parts = [&](int pair, int& c0, int& n) {
-    const long long u0 = before + (long long)pair * r.units;
-    c0 = range_of(total, u0, ctas);
-    n = range_of(total, u0 + r.units - 1, ctas) - c0 + 1;
-  };
-  auto record = [&](int c0, int pair, int g) { return P.records + ((c0 + (long long)b * per + pair) * 16 + g % 16) * (D + 2); };
-  if (row_block) {
-    const int head = job % P.q_heads, g = head % P.group, pair = head / P.group * P.chunks + g / 16;
-    int c0, n;
-    parts(pair, c0, n);
-    if (n == 1) return;       // written by the CTA that had the whole pair
-    const float* const rec = record(c0, pair, g);
-    const float2 whole = join_sums(rec + D, kStride, n);
-    const int first = tid / (D / 4), c = tid % (D / 4);
-    float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-    for (int i = first; i < n; i += kAtOnce) {
-      const float f = pf_exp2(__ldcg(rec + (long long)i * kStride + D) - whole.x);
-      const float2 lo = __ldcg((const float2*)(rec + (long long)i * kStride + 4 * c)), hi = __ldcg((const float2*)(rec + (long long)i * kStride + 4 * c + 2));
-      sum.x = fmaf(lo.x, f, sum.x);
-      sum.y = fmaf(lo.y, f, sum.y);
-      sum.z = fmaf(hi.x, f, sum.z);
-      sum.w = fmaf(hi.y, f, sum.w);
-    }
-    partial[first][c] = sum;
-    __syncthreads();
-    if (tid < D / 4) {
-#pragma unroll
-      for (int i = 1; i < kAtOnce; ++i) {
-        const float4 x = partial[i][tid];
-        sum = make_float4(sum.x + x.x, sum.y + x.y, sum.z + x.z, sum.w + x.w);
-      }
-      const float inv = whole.y == 0.f ? 0.f : 1.f / whole.y;
-      *(uint2*)((QT*)P.out + b * P.o_sb + (long long)head * P.o_sh + 4 * tid) =
-          make_uint2(pf_pack2<QT>(sum.x * inv, sum.y * inv), pf_pack2<QT>(sum.z * inv, sum.w * inv));
-    }
-    return;
-  }
-  // ---- weights of 512 tokens of one KV head
-  const int kvh = job / weight_blocks % P.kv_heads;
-  float sums[kDpJoinEach];
-#pragma unroll
-  for (int i = 0; i < kDpJoinEach; ++i) {
-    const int t = t0 + tid + i * kDpJoinThreads;
-    sums[i] = P.weights && t < r.tokens && t != r.fresh ? P.weights[b * P.w_sb + kvh * P.w_sh + t] : 0.f;
-  }
   const float* const logits = P.logits + ((long long)b * P.q_heads + kvh * P.group) * P.capacity;
   for (int g0 = 0; g0 < P.group; g0 += 64) {
+    const int g1 = min(g0 + 64, P.group);
     __syncthreads();
-    for (int g = g0 + warp; g < min(g0 + 64, P.group); g += kDpJoinThreads / 32) {
+    for (int g = g0 + warp; g < g1; g += kDpWeightThreads / 32) {
       const int pair = kvh * P.chunks + g / 16;
-      int c0, n;
-      parts(pair, c0, n);
-      const float2 whole = join_sums(record(c0, pair, g) + D, kStride, n);
+      const long long u0 = before + (long long)pair * r.units;
+      const int c0 = range_of(total, u0, ctas), n = range_of(total, u0 + r.units - 1, ctas) - c0 + 1;
+      const float2 whole = join_sums(P.records + ((c0 + (long long)b * P.kv_heads * P.chunks + pair) * 16 + g % 16) * (D + 2) + D, kStride, n);
       if ((tid & 31) == 0) lse_s[g - g0] = whole.y == 0.f ? __int_as_float(0x7f800000) : whole.x + log2f(whole.y);
     }
     __syncthreads();
 #pragma unroll 4
-    for (int g = g0; g < min(g0 + 64, P.group); ++g) {
+    for (int g = g0; g < g1; ++g) {
       const float lse = lse_s[g - g0];
 #pragma unroll
-      for (int i = 0; i < kDpJoinEach; ++i) {
-        const int t = t0 + tid + i * kDpJoinThreads;
+      for (int i = 0; i < kDpWeightEach; ++i) {
+        const int t = t0 + tid + i * kDpWeightThreads;
         if (t < r.tokens) sums[i] += pf_exp2(__ldcg(logits + g * P.capacity + t) - lse);
       }
     }
   }
 #pragma unroll
-  for (int i = 0; i < kDpJoinEach; ++i) {
-    const int t = t0 + tid + i * kDpJoinThreads;
+  for (int i = 0; i < kDpWeightEach; ++i) {
+    const int t = t0 + tid + i * kDpWeightThreads;
     if (t < r.tokens) P.out_weights[b * P.ow_sb + kvh * P.ow_sh + t] = sums[i];
   }
 }
@@ -564,7 +601,7 @@ long long logit_floats(const inq_paged_attention_args_t* a) {
   return a->out_weights ? (long long)a->requests * a->q_heads * a->table_columns * a->page_tokens : 0;
 }
 int check_args(const inq_paged_attention_args_t* a) {
-  if (!a || !a->q || !a->k || !a->v || !a->out || !a->table || !a->lengths || !a->status) return INQ_ERR_ARGUMENT;
+  if (!a || !a->q || !a->k || !a->v || !a->out || !a->table || !a->lengths || !a->counters || !a->status) return INQ_ERR_ARGUMENT;
   if (a->requests < 1 || a->kv_heads < 1 || a->q_heads < 1 || a->q_heads % a->kv_heads || !(a->scale > 0.f)) return INQ_ERR_ARGUMENT;
   if (a->pages < 1 || a->page_tokens < 1 || a->table_columns < 1) return INQ_ERR_ARGUMENT;
   if ((a->new_k == nullptr) != (a->new_v == nullptr) || (a->weights && !a->out_weights)) return INQ_ERR_ARGUMENT;
@@ -578,19 +615,31 @@ int check_args(const inq_paged_attention_args_t* a) {
   if (((uintptr_t)a->q | (uintptr_t)a->k | (uintptr_t)a->v | (uintptr_t)a->out | (uintptr_t)a->new_k | (uintptr_t)a->new_v) & 15) return INQ_ERR_ARGUMENT;
   return INQ_OK;
 }
+// The limit belongs to a kernel on a device; a device that has it is not asked again.
+int allow_shared(const void* kernel, std::atomic<unsigned long long>& known, int bytes) {
+  int device = 0;
+  INQ_CUDA_CHECK(cudaGetDevice(&device));
+  const unsigned long long bit = device < 64 ? 1ull << device : 0ull;
+  if (known.load(std::memory_order_relaxed) & bit) return INQ_OK;
+  INQ_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+  known.fetch_or(bit, std::memory_order_relaxed);
+  return INQ_OK;
+}
+template <typename QT, int D, int TILES, bool WEIGHTS>
+int launch_kernel(const DensePagedParams& P, int ctas, cudaStream_t stream) {
+  static std::atomic<unsigned long long> known{0};
+  const int rc = allow_shared((const void*)paged_kernel<QT, D, TILES, WEIGHTS>, known, DensePagedShape<D>::kSmem);
+  if (rc != INQ_OK) return rc;
+  INQ_CUDA_CHECK(launch_following(paged_kernel<QT, D, TILES, WEIGHTS>, ctas, kDpThreads, DensePagedShape<D>::kSmem, stream, P));
+  return INQ_OK;
+}
 template <typename QT, int D>
 int launch(const DensePagedParams& P, int ctas, cudaStream_t stream) {
-  auto start = [&](void (*kernel)(DensePagedParams)) {
-    INQ_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, DensePagedShape<D>::kSmem));
-    INQ_CUDA_CHECK(launch_following(kernel, ctas, kDpThreads, DensePagedShape<D>::kSmem, stream, P));
-    return (int)INQ_OK;
-  };
-  const int rc = P.group <= 8 ? P.out_weights ? start(paged_kernel<QT, D, 8, true>) : start(paged_kernel<QT, D, 8, false>)
-                              : P.out_weights ? start(paged_kernel<QT, D, 16, true>) : start(paged_kernel<QT, D, 16, false>);
+  if (!P.out_weights) return P.group <= 8 ? launch_kernel<QT, D, 1, false>(P, ctas, stream) : launch_kernel<QT, D, 2, false>(P, ctas, stream);
+  const int rc = P.group <= 8 ? launch_kernel<QT, D, 1, true>(P, ctas, stream) : launch_kernel<QT, D, 2, true>(P, ctas, stream);
   if (rc != INQ_OK) return rc;
-  const int weight_blocks = P.out_weights ? (int)((P.capacity + kDpJoinTokens - 1) / kDpJoinTokens) : 0;
-  const long long blocks = (long long)P.requests * P.q_heads + (long long)P.requests * P.kv_heads * weight_blocks;
-  INQ_CUDA_CHECK(launch_following(paged_join_kernel<QT, D>, dim3((unsigned)blocks), kDpJoinThreads, 0, stream, P, ctas, weight_blocks));
+  const int blocks = (int)((P.capacity + kDpWeightTokens - 1) / kDpWeightTokens);
+  INQ_CUDA_CHECK(launch_following(paged_weights_kernel<D>, dim3((unsigned)(P.requests * P.kv_heads * blocks)), kDpWeightThreads, 0, stream, P, ctas, blocks));
   return INQ_OK;
 }
 }  // namespace
@@ -607,9 +656,9 @@ extern "C" int inq_paged_attention(const inq_paged_attention_args_t* a, inq_stre
   int n_sm = 0;
   rc = ranges(&n_sm);
   if (rc != INQ_OK) return rc;
-  const long long records = record_floats(a, n_sm), blocks = (long long)a->requests * (a->q_heads +
-                  (a->out_weights ? a->kv_heads * (((long long)a->table_columns * a->page_tokens + kDpJoinTokens - 1) / kDpJoinTokens) : 0));
-  if (blocks > 0x7fffffffLL) return INQ_ERR_CAPACITY;
+  const long long records = record_floats(a, n_sm);
+  if ((long long)a->requests * a->kv_heads * (((long long)a->table_columns * a->page_tokens + kDpWeightTokens - 1) / kDpWeightTokens) > 0x7fffffffLL)
+    return INQ_ERR_CAPACITY;
   if (!a->workspace || ((uintptr_t)a->workspace & 15) || a->workspace_bytes < 4 * (records + logit_floats(a))) return INQ_ERR_CAPACITY;
   DensePagedParams P = {};
   P.q = a->q; P.k = a->k; P.v = a->v; P.out = a->out; P.new_k = a->new_k; P.new_v = a->new_v;
@@ -629,6 +678,7 @@ extern "C" int inq_paged_attention(const inq_paged_attention_args_t* a, inq_stre
   P.w_sb = a->w_stride_b; P.w_sh = a->w_stride_h; P.ow_sb = a->ow_stride_b; P.ow_sh = a->ow_stride_h;
   P.records = (float*)a->workspace;
   P.logits = P.records + records;
+  P.counters = a->counters;
   P.scale_log2e = a->scale * 1.4426950408889634f;
   P.status = a->status;
   cudaStream_t stream = (cudaStream_t)stream_;

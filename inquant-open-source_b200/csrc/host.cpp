@@ -471,14 +471,16 @@ bool state(const at::Tensor& t, at::ScalarType type, int64_t requests, int64_t h
 }
 
 // paged_attention(query, key_pages, value_pages, block_table, lengths, scale | None, new_key | None, new_value | None, weights | None,
-//                 out_weights | None, out | None, status) -> output or (output, out_weights), a return code, or None
+//                 out_weights | None, out | None, status, counters) -> output or (output, out_weights), a return code, or None
 PyObject* paged_attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
-  if (n != 12) return PyErr_Format(PyExc_TypeError, "paged_attention takes 12 arguments");
+  if (n != 13) return PyErr_Format(PyExc_TypeError, "paged_attention takes 13 arguments");
   const int at[] = {11};
   long long v[1];
   if (!integers(args, at, 1, v)) return nullptr;
   return guarded([&]() -> PyObject* {
     inq_paged_attention_args_t a = {};
+    const at::Tensor* const counters = plain(args[12]);
+    if (!counters || counters->scalar_type() != at::kInt || !counters->is_contiguous()) return none();
     const at::Tensor *q = plain(args[0]), *k = plain(args[1]), *new_k, *new_v, *w, *out_w, *out;
     if (!q || !paged(k, plain(args[2]), plain(args[3]), plain(args[4]), a)) return none();
     if (!optional(args[6], new_k) || !optional(args[7], new_v) || !optional(args[8], w) || !optional(args[9], out_w) || !optional(args[10], out)) return none();
@@ -519,6 +521,8 @@ PyObject* paged_attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
     a.q_heads = (int32_t)q->size(1);
     a.dtype = q->scalar_type() == at::kHalf ? INQ_F16 : INQ_BF16;
     a.status = reinterpret_cast<int32_t*>(v[0]);
+    if (counters->device() != q->device() || counters->numel() < (int64_t)a.requests * a.kv_heads * ((a.q_heads / a.kv_heads + 15) / 16)) return none();
+    a.counters = static_cast<int32_t*>(counters->data_ptr());
     a.workspace_bytes = g_dense.paged_bytes(&a);
     const at::Tensor scratch = bytes_on(*k, a.workspace_bytes);
     a.workspace = scratch.data_ptr();

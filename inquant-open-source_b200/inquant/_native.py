@@ -168,7 +168,7 @@ class PagedAttentionArgs(ctypes.Structure):
                 ("w_stride_b", c_int64), ("w_stride_h", c_int64), ("ow_stride_b", c_int64), ("ow_stride_h", c_int64),
                 ("table", c_void_p), ("lengths", c_void_p), ("table_stride", c_int64), ("pages", c_int64),
                 ("requests", c_int32), ("q_heads", c_int32), ("kv_heads", c_int32), ("head_dim", c_int32), ("page_tokens", c_int32),
-                ("table_columns", c_int32), ("dtype", c_int32), ("scale", ctypes.c_float), ("status", c_void_p),
+                ("table_columns", c_int32), ("dtype", c_int32), ("scale", ctypes.c_float), ("status", c_void_p), ("counters", c_void_p),
                 ("workspace", c_void_p), ("workspace_bytes", c_int64)]
 
 
@@ -456,6 +456,14 @@ def decode_counters(device: torch.device, count: int, handle: int | None = None)
         tensor = torch.zeros(max(count + 1, 1024), dtype=torch.int32, device=device)
         _counters[key] = tensor
     return tensor
+
+
+def launch_counters(device: torch.device, count: int) -> torch.Tensor:
+    """``decode_counters`` of the current stream; a call that is being captured gets zeroed ones of its own, because two
+    graphs that were captured on one stream may be replayed at the same time."""
+    if torch.cuda.is_current_stream_capturing():
+        return torch.zeros(count, dtype=torch.int32, device=device)
+    return decode_counters(device, count)
 
 
 def dense_rows_aligned(tensor: torch.Tensor) -> bool:

@@ -44,6 +44,14 @@ def _check_pages(what: str, key_pages, value_pages, block_table, lengths) -> Non
         raise ValueError("pages, block_table and lengths must share a device")
 
 
+def _pairs(query: torch.Tensor, key_pages: torch.Tensor) -> int:
+    """Pairs of a request and up to 16 query heads of a KV head (of shapes that may not have been checked yet)."""
+    if query.ndim != 3 or key_pages.ndim != 4 or key_pages.shape[1] < 1:
+        return 1
+    heads = key_pages.shape[1]
+    return max(query.shape[0] * heads * ((query.shape[1] // heads + 15) // 16), 1)
+
+
 def _check_state(name: str, t: torch.Tensor, dtype: torch.dtype, requests: int, heads: int, columns: int, device) -> None:
     if t.ndim != 3 or t.shape[0] != requests or t.shape[1] != heads or t.shape[2] < columns or t.dtype != dtype or t.device != device \
             or (t.shape[2] > 1 and t.stride(2) != 1):
@@ -68,8 +76,10 @@ def paged_attention(query: torch.Tensor, key_pages: torch.Tensor, value_pages: t
     stores into them.  Returns the output [B, Hq, D], and with weights ``(output, out_weights)``."""
     host = N.native_call(query)      # the ordinary call in native code, the rest takes the checks and copies below
     if host is not None:
+        device = query.device
+        counters = N.launch_counters(device, _pairs(query, key_pages))
         result = host.paged_attention(query, key_pages, value_pages, block_table, lengths, scale, new_key, new_value, weights, out_weights, out,
-                                      N.status_word(query.device).data_ptr())
+                                      N.status_word(device).data_ptr(), counters)
         if type(result) is int:
             N.check(result, "inq_paged_attention")
         if result is not None:
@@ -131,6 +141,8 @@ def _paged_attention(query, key_pages, value_pages, block_table, lengths, scale,
         need = N.library().inq_paged_attention_workspace_bytes(ctypes.byref(args))
         scratch = torch.empty(need, dtype=torch.uint8, device=device)
         args.workspace, args.workspace_bytes = scratch.data_ptr(), need
+        counters = N.launch_counters(device, _pairs(query, key_pages))
+        args.counters = counters.data_ptr()
         N.check(N.library().inq_paged_attention(ctypes.byref(args), N.stream_pointer(device)), "inq_paged_attention")
     return out if out_weights is None else (out, out_weights)
 
