@@ -21,7 +21,7 @@
 
 namespace inq {
 
-constexpr int kDpWarps = 8, kDpThreads = 32 * kDpWarps;
+constexpr int kDpWarps = 4, kDpThreads = 32 * kDpWarps, kDpPerSm = 2;
 constexpr int kDpSlice = 16;                       // tokens of a unit per warp
 constexpr int kDpUnit = kDpWarps * kDpSlice;
 constexpr float kDpNegBig = -3.0e38f;              // the maximum of nothing
@@ -36,11 +36,14 @@ struct DensePagedParams {
   long long table_stride;
   long long pages;
   int requests, q_heads, kv_heads, group, chunks, page_tokens, page_shift, table_columns;
+  int even_ctas;       // CTAs that run at a time: the ranges of an even cut
+  int late_join;       // whether a launch of its own joins the parts
   const float* weights;
   float* out_weights;
   long long w_sb, w_sh, ow_sb, ow_sh;
   float* records;      // [part + pair][rows][D + 2]: unnormalised output, maximum, sum
   float* logits;       // [request][query head][capacity], base 2
+  float* lse;          // [request][query head], base 2, where weights are asked for
   int* counters;       // [pair]: parts handed in, zero between launches
   long long capacity;
   float scale_log2e;
@@ -70,28 +73,61 @@ __device__ __forceinline__ Request load_request(const DensePagedParams& P, int b
   return r;
 }
 // Units of all pairs, and those in front of request `upto`.  The whole warp takes part.
-__device__ __forceinline__ long long count_units(const DensePagedParams& P, int upto, long long& before) {
+__device__ __forceinline__ unsigned count_units(const DensePagedParams& P, int upto, unsigned& before) {
   const int lane = threadIdx.x & 31;
-  long long all = 0, front = 0;
+  unsigned all = 0, front = 0;
   for (int b = lane; b < P.requests; b += 32) {
-    const int n = load_request(P, b).units;
+    const unsigned n = load_request(P, b).units;
     all += n;
     if (b < upto) front += n;
   }
-#pragma unroll
-  for (int d = 16; d; d >>= 1) {
-    all += __shfl_xor_sync(0xffffffffu, all, d);
-    front += __shfl_xor_sync(0xffffffffu, front, d);
-  }
-  const long long per = (long long)P.kv_heads * P.chunks;
-  before = front * per;
-  return all * per;
+  const unsigned per = P.kv_heads * P.chunks;
+  before = __reduce_add_sync(0xffffffffu, front) * per;
+  return __reduce_add_sync(0xffffffffu, all) * per;
 }
-// Range c of `ctas` is [range_start(c), range_start(c + 1)); there are no more ranges than units, so that none is empty.
-__device__ __forceinline__ int range_count(long long total, int most) { return (int)min(total, (long long)most); }
-__device__ __forceinline__ long long range_start(long long total, int cta, int ctas) { return total * cta / ctas; }
-__device__ __forceinline__ int range_of(long long total, long long unit, int ctas) { return (int)(((unit + 1) * ctas - 1) / total); }
 
+// How the list of units is cut into ranges, one CTA each.  CTAs do not stream alike (64 requests in equal ranges: half of
+// them had finished after 135 us, the last after 160), so the first CTAs get three quarters of an even share and those that
+// take their places ever smaller ranges of the rest.  Few units are cut evenly: what joins the parts costs more.
+constexpr unsigned kDpLeast = 4;         // units of a range, where there are many
+constexpr unsigned kDpEven = 48;         // an even share of fewer units than this is not cut further
+constexpr int kDpMostRanges = 5;         // ranges per CTA of an even cut, at most
+struct Ranges {
+  unsigned total, ctas, size0, extra;    // the first `ctas` ranges: size0 units, the first `extra` of them one more
+  unsigned size1, count1, size2, count;  // then count1 ranges of size1, then ranges of size2; count: all
+  __host__ __device__ __forceinline__ Ranges(unsigned units, unsigned most) : total(units) {
+    ctas = units < most ? units : most;
+    count = ctas;
+    size0 = size1 = size2 = extra = count1 = 0;
+    if (ctas == 0) return;
+    const unsigned even = units / ctas;
+    if (even < kDpEven) {
+      size0 = even;
+      extra = units - even * ctas;
+      return;
+    }
+    size0 = even - even / 4;
+    unsigned rest = units - size0 * ctas;
+    size1 = rest / (2 * ctas) > kDpLeast ? rest / (2 * ctas) : kDpLeast;
+    count1 = (rest + size1 - 1) / size1 < ctas ? (rest + size1 - 1) / size1 : ctas;
+    rest -= rest < count1 * size1 ? rest : count1 * size1;
+    size2 = size1 / 2 > kDpLeast ? size1 / 2 : kDpLeast;
+    count = ctas + count1 + (rest + size2 - 1) / size2;
+  }
+  __device__ __forceinline__ unsigned start(unsigned range) const {
+    if (range < ctas) return range * size0 + min(range, extra);
+    const unsigned behind = ctas * size0 + extra, r = range - ctas;
+    return min(r < count1 ? behind + r * size1 : behind + count1 * size1 + (r - count1) * size2, total);
+  }
+  // The range that holds a unit
+  __device__ __forceinline__ unsigned of(unsigned unit) const {
+    const unsigned longer = extra * (size0 + 1), behind = ctas * size0 + extra;
+    if (unit < longer) return unit / (size0 + 1);
+    if (unit < behind) return extra + (unit - longer) / size0;
+    const unsigned r = unit - behind;
+    return r < count1 * size1 ? ctas + r / size1 : ctas + count1 + (r - count1 * size1) / size2;
+  }
+};
 // A place in the list of units: request, pair inside the request, unit inside the pair.
 struct Cursor {
   int b, pair, unit;
@@ -101,16 +137,17 @@ __device__ __forceinline__ void skip_empty(const DensePagedParams& P, Cursor& c)
   while (c.r.units == 0 && ++c.b < P.requests) c.r = load_request(P, c.b);
 }
 // The place of unit `unit`, which exists.  The whole warp takes part.
-__device__ __forceinline__ Cursor seek(const DensePagedParams& P, long long unit) {
-  const int lane = threadIdx.x & 31, per = P.kv_heads * P.chunks;
+__device__ __forceinline__ Cursor seek(const DensePagedParams& P, unsigned unit) {
+  const int lane = threadIdx.x & 31;
+  const unsigned per = P.kv_heads * P.chunks;
   Cursor c = {0, 0, 0, {0, -1, 0}};
   for (int b0 = 0; b0 < P.requests; b0 += 32) {
     Request r = {0, -1, 0};
     if (b0 + lane < P.requests) r = load_request(P, b0 + lane);
-    long long sum = (long long)r.units * per;
+    unsigned sum = r.units * per;
 #pragma unroll
     for (int d = 1; d < 32; d <<= 1) {
-      const long long other = __shfl_up_sync(0xffffffffu, sum, d);
+      const unsigned other = __shfl_up_sync(0xffffffffu, sum, d);
       if (lane >= d) sum += other;
     }
     const unsigned found = __ballot_sync(0xffffffffu, sum > unit);
@@ -119,10 +156,10 @@ __device__ __forceinline__ Cursor seek(const DensePagedParams& P, long long unit
       c.r.tokens = __shfl_sync(0xffffffffu, r.tokens, who);
       c.r.fresh = __shfl_sync(0xffffffffu, r.fresh, who);
       c.r.units = __shfl_sync(0xffffffffu, r.units, who);
-      const long long inside = unit - (__shfl_sync(0xffffffffu, sum, who) - (long long)c.r.units * per);
+      const unsigned inside = unit - (__shfl_sync(0xffffffffu, sum, who) - c.r.units * per);
       c.b = b0 + who;
       c.pair = (int)(inside / c.r.units);
-      c.unit = (int)(inside % c.r.units);
+      c.unit = (int)(inside - c.pair * c.r.units);
       return c;
     }
     unit -= __shfl_sync(0xffffffffu, sum, 31);
@@ -174,80 +211,76 @@ struct DensePagedShape {
   static constexpr int kSliceBytes = 2 * kDpSlice * kRowBytes;          // K rows, then V rows
   static constexpr int kStages = D == 128 ? 3 : 4;
   static constexpr int kRing = kDpWarps * kStages * kSliceBytes;
-  static constexpr int kExchange = kDpWarps * 8 * D * 4;                // eight rows of every warp's output
+  static constexpr int kExchange = kDpWarps * 4 * D * 4;                // four rows of every warp's output
   static constexpr int kSmem = kRing + kExchange + kDpWarps * 16 * 2 * 4;
 };
 
-// Reference maximum and sum of a row over n parts, the same in every lane; the whole warp takes part.
-__device__ __forceinline__ float2 join_sums(const float* first, long long stride, int n) {
-  const int lane = threadIdx.x & 31;
+// Log-sum-exp of a row to base 2; a row without weight, for what divides by it.
+__device__ __forceinline__ float join_lse(float top, float sum) { return sum == 0.f ? __int_as_float(0x7f800000) : top + log2f(sum); }
+// Parts c0 .. c1 - 1 of a row in their order: reference maximum, sum and, D / 32 channels a lane, unnormalised output.  A warp;
+// all it reads of 16 parts is asked for at once, since a trip to memory is what this costs.
+template <int D>
+struct Joined {
+  static constexpr int kPairs = D / 64, kAtOnce = 16;
   float top = kDpNegBig, sum = 0.f;
-  for (int c = lane; c < n; c += 32) {
-    const float2 ml = __ldcg((const float2*)(first + c * stride));
-    const float next = fmaxf(top, ml.x);
-    sum = sum * pf_exp2(top - next) + ml.y * pf_exp2(ml.x - next);
-    top = next;
-  }
+  float2 out[kPairs] = {};
+  __device__ __forceinline__ void add(const float* rec, long long stride, int c0, int c1) {
+    const int lane = threadIdx.x & 31;
+    for (int c = c0; c < c1; c += kAtOnce) {
+      const float2 ml = lane < kAtOnce && c + lane < c1 ? __ldcg((const float2*)(rec + (c + lane) * stride + D)) : make_float2(kDpNegBig, 0.f);
+      float2 x[kAtOnce][kPairs];
 #pragma unroll
-  for (int d = 16; d; d >>= 1) {
-    const float other_top = __shfl_xor_sync(0xffffffffu, top, d), other = __shfl_xor_sync(0xffffffffu, sum, d);
-    const float next = fmaxf(top, other_top);
-    sum = sum * pf_exp2(top - next) + other * pf_exp2(other_top - next);
-    top = next;
-  }
-  return make_float2(top, sum);
-}
-// A row of a cut pair: out = sum_c O_c 2^(m_c - m) / sum_c l_c 2^(m_c - m) over its n parts.  A warp, D / 32 channels a lane.
-template <typename QT, int D>
-__device__ __forceinline__ void join_row(const float* rec, long long stride, int n, QT* out) {
-  constexpr int kEach = D / 32;
-  const int lane = threadIdx.x & 31;
-  const float2 whole = join_sums(rec + D, stride, n);
-  float sum[kEach] = {};
-#pragma unroll 8
-  for (int c = 0; c < n; ++c) {
-    const float f = pf_exp2(__ldcg(rec + c * stride + D) - whole.x);
+      for (int i = 0; i < kAtOnce; ++i)
 #pragma unroll
-    for (int i = 0; i < kEach; i += 2) {
-      const float2 x = __ldcg((const float2*)(rec + c * stride + kEach * lane + i));
-      sum[i] = fmaf(x.x, f, sum[i]);
-      sum[i + 1] = fmaf(x.y, f, sum[i + 1]);
+        for (int k = 0; k < kPairs; ++k) x[i][k] = c + i < c1 ? __ldcg((const float2*)(rec + (c + i) * stride) + 32 * k + lane) : make_float2(0.f, 0.f);
+      float next = ml.x;
+#pragma unroll
+      for (int d = 8; d; d >>= 1) next = fmaxf(next, __shfl_xor_sync(0xffffffffu, next, d));
+      next = fmaxf(top, __shfl_sync(0xffffffffu, next, 0));
+      const float before = pf_exp2(top - next), factor = pf_exp2(ml.x - next);
+      top = next;
+      sum *= before;
+#pragma unroll
+      for (int k = 0; k < kPairs; ++k) out[k] = make_float2(out[k].x * before, out[k].y * before);
+#pragma unroll
+      for (int i = 0; i < kAtOnce; ++i) {
+        const float f = __shfl_sync(0xffffffffu, factor, i);
+        sum = fmaf(__shfl_sync(0xffffffffu, ml.y, i), f, sum);
+#pragma unroll
+        for (int k = 0; k < kPairs; ++k) {
+          out[k].x = fmaf(x[i][k].x, f, out[k].x);
+          out[k].y = fmaf(x[i][k].y, f, out[k].y);
+        }
+      }
     }
   }
-  const float inv = whole.y == 0.f ? 0.f : 1.f / whole.y;
+  template <typename QT>
+  __device__ __forceinline__ void store(QT* to, float* lse) const {
+    const int lane = threadIdx.x & 31;
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;
 #pragma unroll
-  for (int i = 0; i < kEach; i += 2) *(unsigned*)(out + kEach * lane + i) = pf_pack2<QT>(sum[i] * inv, sum[i + 1] * inv);
-}
+    for (int k = 0; k < kPairs; ++k) *(unsigned*)(to + 64 * k + 2 * lane) = pf_pack2<QT>(out[k].x * inv, out[k].y * inv);
+    if (lse && lane == 0) *lse = join_lse(top, sum);
+  }
+};
 
 // TILES: query heads of a pair that the kernel holds, in eights.  Both contractions take the cache as their left operand,
 // S^T = K Q^T (16 tokens x 8 heads) and O^T = V^T P^T (16 channels x 8 heads): the query heads of one KV head are few, and as
 // rows of a 16-row operand half of them would be empty.  The probabilities change places between the two by movmatrix.
 template <typename QT, int D, int TILES, bool WEIGHTS>
-__global__ void __launch_bounds__(kDpThreads, 1) paged_kernel(const DensePagedParams P) {
+__global__ void __launch_bounds__(kDpThreads, kDpPerSm) paged_kernel(const DensePagedParams P) {
   using S = DensePagedShape<D>;
   constexpr int kStages = S::kStages, kCopies = kDpSlice * S::kChunks / 32;      // 16-byte copies of a lane per K or V slice
   constexpr int kRowsAtOnce = 32 / S::kChunks;
   extern __shared__ __align__(1024) unsigned char dp_raw[];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const unsigned ring = tc_smem(dp_raw) + warp * kStages * S::kSliceBytes;
-  float* const exchange = (float*)(dp_raw + S::kRing);                           // [warp][8][D], columns swizzled
+  float* const exchange = (float*)(dp_raw + S::kRing);                           // [warp][4][D], columns swizzled
   float* const ml = (float*)(dp_raw + S::kRing + S::kExchange);                  // [warp][16][maximum, sum]
   follow_stream();
-  if (blockIdx.x == 0 && tid < 32)
-    for (int b = tid; b < P.requests; b += 32) load_request(P, b, true);
-  // requests with nothing to attend to: zeros
-  for (int b = blockIdx.x; b < P.requests; b += gridDim.x)
-    if (load_request(P, b).units == 0)
-      for (int i = tid; i < P.q_heads * S::kChunks; i += kDpThreads)
-        *(uint4*)((QT*)P.out + b * P.o_sb + (long long)(i / S::kChunks) * P.o_sh + i % S::kChunks * 8) = make_uint4(0u, 0u, 0u, 0u);
-  long long unused;
-  const long long total = count_units(P, 0, unused);
-  const int ctas = range_count(total, gridDim.x);
+  unsigned unused;
+  const Ranges ranges(count_units(P, 0, unused), P.even_ctas);
   allow_next();
-  if ((int)blockIdx.x >= ctas) return;
-  const long long w0 = range_start(total, blockIdx.x, ctas), w1 = range_start(total, blockIdx.x + 1, ctas);
-  Cursor at = seek(P, w0), ahead = at;         // the unit in work and the one to ask for next
-  const int count = (int)(w1 - w0);
   const bool whole = P.page_tokens % kDpSlice == 0;     // a slice lies in one page
 
   // Physical page of the row that lane & 15 stands for, or -1.
@@ -322,9 +355,25 @@ __global__ void __launch_bounds__(kDpThreads, 1) paged_kernel(const DensePagedPa
     return valid;
   };
 
+  // requests with nothing to attend to: zeros; lengths that the table cannot hold are reported
+  auto settle = [&]() {
+    for (int b = blockIdx.x; b < P.requests; b += gridDim.x)
+      if (load_request(P, b, tid == 0).units == 0)
+        for (int i = tid; i < P.q_heads * S::kChunks; i += kDpThreads)
+          *(uint4*)((QT*)P.out + b * P.o_sb + (long long)(i / S::kChunks) * P.o_sh + i % S::kChunks * 8) = make_uint4(0u, 0u, 0u, 0u);
+  };
+  const unsigned range = blockIdx.x;
+  if (range >= ranges.count) {
+    settle();
+    return;
+  }
+  const unsigned begin = ranges.start(range);
+  const int count = (int)(ranges.start(range + 1) - begin);
+
   unsigned long long rows_ahead = 0;        // 16 bits per requested slice, the oldest lowest
   constexpr int kAhead = kStages - 1;      // slices requested in front of the one in work
   static_assert(kAhead <= 3, "16 bits per slice, and the one in work");
+  Cursor at = seek(P, begin), ahead = at;         // the unit in work and the one to ask for next
   int page = look_up(ahead), asked = 0, ask_stage = 0, stage = 0;
   auto ask = [&]() {
     if (asked < count) {
@@ -343,12 +392,13 @@ __global__ void __launch_bounds__(kDpThreads, 1) paged_kernel(const DensePagedPa
     ask();
     rows_ahead >>= 16;
   }
+  settle();
 
   unsigned qf[TILES][D / 16][2];                // query heads as right operands
   float o[TILES][D / 16][4], m[TILES][2], l[TILES][2];      // heads 8 i + 2 (lane & 3) (+ 1)
   const int c0 = 2 * (lane & 3), g = lane >> 2;
   bool first = true;
-  for (int done = 0; done < count; ++done) {
+  for (int done = 1; done <= count; ++done) {
     const int h0 = at.pair / P.chunks * P.group + at.pair % P.chunks * 16, rows = min(P.group - at.pair % P.chunks * 16, 16);
     if (first) {
       // a new pair: its query rows (those beyond the group are zero), an empty state
@@ -447,7 +497,7 @@ __global__ void __launch_bounds__(kDpThreads, 1) paged_kernel(const DensePagedPa
     __syncwarp();        // the stage may be asked for again
     stage = stage + 1 == kStages ? 0 : stage + 1;
     const bool pair_ends = at.unit + 1 == at.r.units;
-    if (pair_ends || done + 1 == count) {
+    if (pair_ends || done == count) {
       // ---- this CTA's part of the pair: the warps' states joined, a record or, where it is the whole pair, the output
 #pragma unroll
       for (int i = 0; i < TILES; ++i)
@@ -458,20 +508,22 @@ __global__ void __launch_bounds__(kDpThreads, 1) paged_kernel(const DensePagedPa
           l[i][e] += __shfl_xor_sync(0xffffffffu, l[i][e], 16);
           if (lane < 4) *(float2*)(ml + 2 * (warp * 16 + 8 * i + c0 + e)) = make_float2(m[i][e], l[i][e]);
         }
-      const bool alone = pair_ends && done >= at.unit;      // every unit of the pair was in this range
+      const bool alone = pair_ends && done > at.unit;      // every unit of the pair was in this range
       const long long pair = (long long)at.b * P.kv_heads * P.chunks + at.pair;
 #pragma unroll
-      for (int i = 0; i < TILES; ++i) {
+      for (int four = 0; four < 2 * TILES; ++four) {      // rows 4 four .. of the pair, which half of the lanes hold
+        if ((lane & 2) == 2 * (four & 1)) {
 #pragma unroll
-        for (int kk = 0; kk < D / 16; ++kk)
+          for (int kk = 0; kk < D / 16; ++kk)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const int r = c0 + (e & 1);
-            exchange[(warp * 8 + r) * D + ((16 * kk + g + 4 * (e & 2)) ^ (4 * r))] = o[i][kk][e];
-          }
+            for (int e = 0; e < 4; ++e) {
+              const int r = (c0 & 2) + (e & 1);
+              exchange[(warp * 4 + r) * D + ((16 * kk + g + 4 * (e & 2)) ^ (8 * r))] = o[four >> 1][kk][e];
+            }
+        }
         __syncthreads();
-        const int r = tid / (D / 4), c = 4 * (tid % (D / 4)), row = r + 8 * i;
-        if (r < 8 && row < rows) {
+        const int r = tid / (D / 4), c = 4 * (tid % (D / 4)), row = r + 4 * four;
+        if (r < 4 && row < rows) {
           float2 each[kDpWarps];
           float top = kDpNegBig;
 #pragma unroll
@@ -484,16 +536,17 @@ __global__ void __launch_bounds__(kDpThreads, 1) paged_kernel(const DensePagedPa
 #pragma unroll
           for (int w = 0; w < kDpWarps; ++w) {
             const float f = pf_exp2(each[w].x - top);
-            const float4 x = *(const float4*)(exchange + (w * 8 + r) * D + (c ^ (4 * r)));
+            const float4 x = *(const float4*)(exchange + (w * 4 + r) * D + (c ^ (8 * r)));
             weight = fmaf(each[w].y, f, weight);
             sum.x = fmaf(x.x, f, sum.x);
             sum.y = fmaf(x.y, f, sum.y);
             sum.z = fmaf(x.z, f, sum.z);
             sum.w = fmaf(x.w, f, sum.w);
           }
-          float* const rec = P.records + ((blockIdx.x + pair) * 16 + row) * (D + 2);
+          float* const rec = P.records + ((range + pair) * 16 + row) * (D + 2);
           if (c == 0) *(float2*)(rec + D) = make_float2(top, weight);
           if (alone) {
+            if (WEIGHTS && c == 0) P.lse[at.b * P.q_heads + h0 + row] = join_lse(top, weight);
             const float inv = weight == 0.f ? 0.f : 1.f / weight;
             *(uint2*)((QT*)P.out + at.b * P.o_sb + (long long)(h0 + row) * P.o_sh + c) =
                 make_uint2(pf_pack2<QT>(sum.x * inv, sum.y * inv), pf_pack2<QT>(sum.z * inv, sum.w * inv));
@@ -504,10 +557,10 @@ __global__ void __launch_bounds__(kDpThreads, 1) paged_kernel(const DensePagedPa
         }
         __syncthreads();
       }
-      if (!alone) {
+      if (!alone && !P.late_join) {
         // the CTA that hands in the last part joins them all, in their order, and leaves the counter as it found it
-        const long long u0 = w0 + done - at.unit;
-        const int part0 = range_of(total, u0, ctas), parts = range_of(total, u0 + at.r.units - 1, ctas) - part0 + 1;
+        const unsigned u0 = begin + done - 1 - at.unit;
+        const int part0 = (int)ranges.of(u0), parts = (int)ranges.of(u0 + at.r.units - 1) - part0 + 1;
         __threadfence();
         __syncthreads();
         int* const last = (int*)ml;
@@ -520,27 +573,66 @@ __global__ void __launch_bounds__(kDpThreads, 1) paged_kernel(const DensePagedPa
         const bool joins = *last != 0;
         if (joins) {
           __threadfence();
-          for (int row = warp; row < rows; row += kDpWarps)
-            join_row<QT, D>(P.records + ((part0 + pair) * 16 + row) * (D + 2), 16 * (D + 2), parts,
-                            (QT*)P.out + at.b * P.o_sb + (long long)(h0 + row) * P.o_sh);
+          for (int row = warp; row < rows; row += kDpWarps) {
+            Joined<D> all;
+            all.add(P.records + ((part0 + pair) * 16 + row) * (D + 2), 16 * (D + 2), 0, parts);
+            all.template store<QT>((QT*)P.out + at.b * P.o_sb + (long long)(h0 + row) * P.o_sh, WEIGHTS ? P.lse + at.b * P.q_heads + h0 + row : nullptr);
+          }
         }
         __syncthreads();
       }
       first = true;
     }
-    if (done + 1 < count) advance(P, at);
+    if (done < count) advance(P, at);
   }
 }
 
-// Accumulated weights: out_w_t = w_t + sum_g 2^(s_gt - lse_g), from the logits that the launch before this one left and the
-// maxima and sums of its parts.  A block takes 512 tokens of a KV head.
-constexpr int kDpWeightThreads = 128, kDpWeightEach = 4, kDpWeightTokens = kDpWeightThreads * kDpWeightEach;
-template <int D>
-__global__ void __launch_bounds__(kDpWeightThreads) paged_weights_kernel(const DensePagedParams P, int most_ctas, int blocks) {
-  constexpr int kStride = 16 * (D + 2);
-  __shared__ float lse_s[64];
+// Joins the parts of all pairs, a block per row, its warps neighbouring parts each: where a pair has many parts, one CTA of the
+// launch above would take longer over its rows than this launch does.
+constexpr int kDpJoinWarps = 8;
+template <typename QT, int D>
+__global__ void __launch_bounds__(32 * kDpJoinWarps) paged_join_kernel(const DensePagedParams P) {
+  __shared__ float2 ml[kDpJoinWarps], outs[kDpJoinWarps][D / 2];
   follow_stream();
-  const int tid = threadIdx.x, warp = tid >> 5, kvh = blockIdx.x / blocks % P.kv_heads, b = blockIdx.x / (blocks * P.kv_heads);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, b = blockIdx.x / P.q_heads, head = blockIdx.x % P.q_heads;
+  const Request r = load_request(P, b);
+  if (r.units == 0) return;
+  unsigned before;
+  const Ranges ranges(count_units(P, b, before), P.even_ctas);
+  const int g = head % P.group, pair = head / P.group * P.chunks + g / 16;
+  const unsigned u0 = before + pair * r.units;
+  const int part0 = (int)ranges.of(u0), parts = (int)ranges.of(u0 + r.units - 1) - part0 + 1;
+  if (parts == 1) return;       // written by the CTA that had the whole pair
+  Joined<D> mine;
+  mine.add(P.records + ((part0 + (long long)b * P.kv_heads * P.chunks + pair) * 16 + g % 16) * (D + 2), 16 * (D + 2), parts * warp / kDpJoinWarps,
+           parts * (warp + 1) / kDpJoinWarps);
+  if (lane == 0) ml[warp] = make_float2(mine.top, mine.sum);
+#pragma unroll
+  for (int k = 0; k < D / 64; ++k) outs[warp][32 * k + lane] = mine.out[k];
+  __syncthreads();
+  if (warp) return;
+  Joined<D> all;
+#pragma unroll
+  for (int w = 0; w < kDpJoinWarps; ++w) all.top = fmaxf(all.top, ml[w].x);
+#pragma unroll
+  for (int w = 0; w < kDpJoinWarps; ++w) {
+    const float f = pf_exp2(ml[w].x - all.top);
+    all.sum = fmaf(ml[w].y, f, all.sum);
+#pragma unroll
+    for (int k = 0; k < D / 64; ++k) {
+      const float2 x = outs[w][32 * k + lane];
+      all.out[k] = make_float2(fmaf(x.x, f, all.out[k].x), fmaf(x.y, f, all.out[k].y));
+    }
+  }
+  all.template store<QT>((QT*)P.out + b * P.o_sb + (long long)head * P.o_sh, P.out_weights ? P.lse + blockIdx.x : nullptr);
+}
+
+// Accumulated weights: out_w_t = w_t + sum_g 2^(s_gt - lse_g), from the logits and log-sum-exps that the launches before this
+// one left.  A block takes 512 tokens of a KV head.
+constexpr int kDpWeightThreads = 128, kDpWeightEach = 4, kDpWeightTokens = kDpWeightThreads * kDpWeightEach;
+__global__ void __launch_bounds__(kDpWeightThreads) paged_weights_kernel(const DensePagedParams P, int blocks) {
+  follow_stream();
+  const int tid = threadIdx.x, kvh = blockIdx.x / blocks % P.kv_heads, b = blockIdx.x / (blocks * P.kv_heads);
   const int t0 = blockIdx.x % blocks * kDpWeightTokens;
   const Request r = load_request(P, b);
   if (t0 >= r.tokens) return;
@@ -550,29 +642,15 @@ __global__ void __launch_bounds__(kDpWeightThreads) paged_weights_kernel(const D
     const int t = t0 + tid + i * kDpWeightThreads;
     sums[i] = P.weights && t < r.tokens && t != r.fresh ? P.weights[b * P.w_sb + kvh * P.w_sh + t] : 0.f;
   }
-  long long before;
-  const long long total = count_units(P, b, before);
-  const int ctas = range_count(total, most_ctas);
+  const float* const lse = P.lse + b * P.q_heads + kvh * P.group;
   const float* const logits = P.logits + ((long long)b * P.q_heads + kvh * P.group) * P.capacity;
-  for (int g0 = 0; g0 < P.group; g0 += 64) {
-    const int g1 = min(g0 + 64, P.group);
-    __syncthreads();
-    for (int g = g0 + warp; g < g1; g += kDpWeightThreads / 32) {
-      const int pair = kvh * P.chunks + g / 16;
-      const long long u0 = before + (long long)pair * r.units;
-      const int c0 = range_of(total, u0, ctas), n = range_of(total, u0 + r.units - 1, ctas) - c0 + 1;
-      const float2 whole = join_sums(P.records + ((c0 + (long long)b * P.kv_heads * P.chunks + pair) * 16 + g % 16) * (D + 2) + D, kStride, n);
-      if ((tid & 31) == 0) lse_s[g - g0] = whole.y == 0.f ? __int_as_float(0x7f800000) : whole.x + log2f(whole.y);
-    }
-    __syncthreads();
 #pragma unroll 4
-    for (int g = g0; g < g1; ++g) {
-      const float lse = lse_s[g - g0];
+  for (int g = 0; g < P.group; ++g) {
+    const float minus = __ldcg(lse + g);
 #pragma unroll
-      for (int i = 0; i < kDpWeightEach; ++i) {
-        const int t = t0 + tid + i * kDpWeightThreads;
-        if (t < r.tokens) sums[i] += pf_exp2(__ldcg(logits + g * P.capacity + t) - lse);
-      }
+    for (int i = 0; i < kDpWeightEach; ++i) {
+      const int t = t0 + tid + i * kDpWeightThreads;
+      if (t < r.tokens) sums[i] += pf_exp2(__ldcg(logits + g * P.capacity + t) - minus);
     }
   }
 #pragma unroll
@@ -595,10 +673,10 @@ int ranges(int* n) {
 }
 long long record_floats(const inq_paged_attention_args_t* a, int ctas) {
   const long long chunks = (a->q_heads / a->kv_heads + 15) / 16;
-  return ((long long)a->requests * a->kv_heads * chunks + ctas) * 16 * (a->head_dim + 2);
+  return ((long long)a->requests * a->kv_heads * chunks + (long long)ctas * kDpPerSm * kDpMostRanges) * 16 * (a->head_dim + 2);
 }
 long long logit_floats(const inq_paged_attention_args_t* a) {
-  return a->out_weights ? (long long)a->requests * a->q_heads * a->table_columns * a->page_tokens : 0;
+  return a->out_weights ? (long long)a->requests * a->q_heads * ((long long)a->table_columns * a->page_tokens + 1) : 0;      // and lse
 }
 int check_args(const inq_paged_attention_args_t* a) {
   if (!a || !a->q || !a->k || !a->v || !a->out || !a->table || !a->lengths || !a->counters || !a->status) return INQ_ERR_ARGUMENT;
@@ -635,11 +713,14 @@ int launch_kernel(const DensePagedParams& P, int ctas, cudaStream_t stream) {
 }
 template <typename QT, int D>
 int launch(const DensePagedParams& P, int ctas, cudaStream_t stream) {
-  if (!P.out_weights) return P.group <= 8 ? launch_kernel<QT, D, 1, false>(P, ctas, stream) : launch_kernel<QT, D, 2, false>(P, ctas, stream);
-  const int rc = P.group <= 8 ? launch_kernel<QT, D, 1, true>(P, ctas, stream) : launch_kernel<QT, D, 2, true>(P, ctas, stream);
+  const int rc = P.out_weights ? P.group <= 8 ? launch_kernel<QT, D, 1, true>(P, ctas, stream) : launch_kernel<QT, D, 2, true>(P, ctas, stream)
+                 : P.group <= 8 ? launch_kernel<QT, D, 1, false>(P, ctas, stream) : launch_kernel<QT, D, 2, false>(P, ctas, stream);
   if (rc != INQ_OK) return rc;
-  const int blocks = (int)((P.capacity + kDpWeightTokens - 1) / kDpWeightTokens);
-  INQ_CUDA_CHECK(launch_following(paged_weights_kernel<D>, dim3((unsigned)(P.requests * P.kv_heads * blocks)), kDpWeightThreads, 0, stream, P, ctas, blocks));
+  if (P.late_join) INQ_CUDA_CHECK(launch_following(paged_join_kernel<QT, D>, dim3(P.requests * P.q_heads), 32 * kDpJoinWarps, 0, stream, P));
+  if (P.out_weights) {
+    const int blocks = (int)((P.capacity + kDpWeightTokens - 1) / kDpWeightTokens);
+    INQ_CUDA_CHECK(launch_following(paged_weights_kernel, dim3((unsigned)(P.requests * P.kv_heads * blocks)), kDpWeightThreads, 0, stream, P, blocks));
+  }
   return INQ_OK;
 }
 }  // namespace
@@ -657,8 +738,11 @@ extern "C" int inq_paged_attention(const inq_paged_attention_args_t* a, inq_stre
   rc = ranges(&n_sm);
   if (rc != INQ_OK) return rc;
   const long long records = record_floats(a, n_sm);
+  const long long most_units = (long long)a->requests * a->kv_heads * ((a->q_heads / a->kv_heads + 15) / 16) *
+                               (((long long)a->table_columns * a->page_tokens + kDpUnit - 1) / kDpUnit);
   if ((long long)a->requests * a->kv_heads * (((long long)a->table_columns * a->page_tokens + kDpWeightTokens - 1) / kDpWeightTokens) > 0x7fffffffLL)
     return INQ_ERR_CAPACITY;
+  if (most_units > 0x7fffffffLL) return INQ_ERR_CAPACITY;      // units are counted in 32 bits
   if (!a->workspace || ((uintptr_t)a->workspace & 15) || a->workspace_bytes < 4 * (records + logit_floats(a))) return INQ_ERR_CAPACITY;
   DensePagedParams P = {};
   P.q = a->q; P.k = a->k; P.v = a->v; P.out = a->out; P.new_k = a->new_k; P.new_v = a->new_v;
@@ -678,10 +762,17 @@ extern "C" int inq_paged_attention(const inq_paged_attention_args_t* a, inq_stre
   P.w_sb = a->w_stride_b; P.w_sh = a->w_stride_h; P.ow_sb = a->ow_stride_b; P.ow_sh = a->ow_stride_h;
   P.records = (float*)a->workspace;
   P.logits = P.records + records;
+  P.lse = P.logits + (long long)a->requests * a->q_heads * P.capacity;
   P.counters = a->counters;
+  P.even_ctas = kDpPerSm * n_sm;
+  // parts of a pair if all are alike: a CTA joins up to sixteen in one trip to memory
+  P.late_join = P.even_ctas > 16LL * a->requests * a->kv_heads * P.chunks && most_units > 16LL * a->requests * a->kv_heads * P.chunks;
   P.scale_log2e = a->scale * 1.4426950408889634f;
   P.status = a->status;
+  // the lengths are not known here: as many CTAs as any would need
+  const long long even = most_units / P.even_ctas;
+  const int ctas = (int)std::max<long long>(1, std::min<long long>(most_units, even < kDpEven ? P.even_ctas : (long long)P.even_ctas * kDpMostRanges));
   cudaStream_t stream = (cudaStream_t)stream_;
-  if (a->dtype == INQ_F16) return a->head_dim == 64 ? launch<__half, 64>(P, n_sm, stream) : launch<__half, 128>(P, n_sm, stream);
-  return a->head_dim == 64 ? launch<__nv_bfloat16, 64>(P, n_sm, stream) : launch<__nv_bfloat16, 128>(P, n_sm, stream);
+  if (a->dtype == INQ_F16) return a->head_dim == 64 ? launch<__half, 64>(P, ctas, stream) : launch<__half, 128>(P, ctas, stream);
+  return a->head_dim == 64 ? launch<__nv_bfloat16, 64>(P, ctas, stream) : launch<__nv_bfloat16, 128>(P, ctas, stream);
 }
