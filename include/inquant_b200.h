@@ -456,15 +456,15 @@ typedef struct {
   float scale;
   int32_t reserved;
   int32_t* status;
-  void* workspace;            /* scratch of one launch at a time, or NULL (items are then not cut) */
+  void* workspace;            /* scratch of one call at a time; without it inq_prompt_attention does not cut its items */
   int64_t workspace_bytes;
 } inq_prompt_args_t;
 int inq_prompt_attention(const inq_prompt_args_t* args /* host */, inq_stream_t stream);
 /* weights[h][j] = sum over the query heads of KV head h and the counted queries i that see key j of
  * exp(scale * q_i k_j - lse_i) */
 int inq_prompt_weights(const inq_prompt_args_t* args /* host */, inq_stream_t stream);
-/* Scratch with which inq_prompt_attention (weights = 0) or inq_prompt_weights (weights = 1) cuts its items as it would
- * on the current device; 0 where it does not cut. */
+/* Scratch with which inq_prompt_attention (weights = 0) cuts its items as it would on the current device, and that
+ * inq_prompt_weights (weights = 1) needs; 0 where nothing is cut. */
 int64_t inq_prompt_workspace_bytes(int32_t q_heads, int32_t kv_heads, int32_t head_dim, int64_t q_rows, int64_t k_rows, int32_t n_seq,
                                    int32_t weights, int32_t window);
 

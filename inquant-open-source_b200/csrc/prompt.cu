@@ -43,6 +43,7 @@ struct PromptParams {
   int n_seq, q_rows, k_rows, q_heads, kv_heads;
   int splits;
   int window;                       // weights: queries per sequence that count, 0 = all
+  int width;                        // weights: columns of a step per query head
   float* records;                   // partial results of cut items
   float scale_log2e;
   int* status;
@@ -65,43 +66,26 @@ __device__ __forceinline__ bool bad_sequence(const PromptParams& P, int b) {
   return q0 < 0 || q1 < q0 || q1 > P.q_rows || k0 < 0 || k1 < k0 || k1 > P.k_rows;
 }
 
-// Items of one sequence that cost at least c.  Costs fall or rise monotonously with the item's index, so that
-// this is an interval and its size a closed form.
-struct AttentionCost {   // item i: 256 query rows; cost: tiles of 128 keys that its last row sees
-  __device__ static int at_least(const Sequence& s, int, int c) {
-    const int n = (s.nq + kPrRows - 1) / kPrRows;
-    if (c <= 0) return n;
-    const int keys = (c - 1) * kPrTile;                       // more than these have to be visible
-    if (s.nk <= keys) return 0;
-    return n - min(max((keys - (s.nk - s.nq)) >> 8, 0), n);
-  }
-  static constexpr bool kFromBack = true;                     // the last items are the dear ones
-};
-struct WeightsCost {     // item i: 256 keys; cost: tiles of 128 queries with one that sees its first key
-  __device__ static int at_least(const Sequence& s, int window, int c) {
-    const int n = (s.nk + kPrRows - 1) / kPrRows;
-    if (c <= 0) return n;
-    const int nw = window > 0 ? min(window, s.nq) : s.nq, tiles = (nw + kPrTile - 1) / kPrTile;
-    if (tiles < c) return 0;
-    // first tile with a query that sees key 256 i: (256 i - (nk - nw)) >> 7 <= tiles - c
-    const int limit = (tiles - c + 1) * kPrTile + (s.nk - nw);
-    return min(max((limit + kPrRows - 1) >> 8, 0), n);
-  }
-  static constexpr bool kFromBack = false;
-};
-
+// Items (256 query rows) of one sequence that cost at least c, cost being the tiles of 128 keys that the last row sees.
+// Costs rise with the item's index, so that these are the last ones and their number a closed form.
+__device__ __forceinline__ int items_at_least(const Sequence& s, int c) {
+  const int n = (s.nq + kPrRows - 1) / kPrRows;
+  if (c <= 0) return n;
+  const int keys = (c - 1) * kPrTile;                       // more than these have to be visible
+  if (s.nk <= keys) return 0;
+  return n - min(max((keys - (s.nk - s.nq)) >> 8, 0), n);
+}
 // The item of rank `rank` in the order of falling cost (sequences in order among equals).  The whole warp takes
 // part: a binary search over the cost, each lane counting the items of its sequences; the sequence and the item
 // inside it follow from prefix sums.  32 sequences stay in registers, further ones are read again (from L1) in
 // every turn.  Returns the sequence, or -1 where there are fewer items.
-template <typename Cost>
 __device__ __forceinline__ int find_item(const PromptParams& P, int rank, int max_cost, Sequence& seq, int& index) {
   const int lane = threadIdx.x & 31;
   Sequence mine = {0, 0, 0, 0};
   if (lane < P.n_seq) mine = load_sequence(P, lane);
   auto count = [&](int c) {
-    int n = Cost::at_least(mine, P.window, c);
-    for (int b = 32 + lane; b < P.n_seq; b += 32) n += Cost::at_least(load_sequence(P, b), P.window, c);
+    int n = items_at_least(mine, c);
+    for (int b = 32 + lane; b < P.n_seq; b += 32) n += items_at_least(load_sequence(P, b), c);
     return __reduce_add_sync(0xffffffffu, n);
   };
   if (rank >= count(0)) return -1;
@@ -114,7 +98,7 @@ __device__ __forceinline__ int find_item(const PromptParams& P, int rank, int ma
   int left = rank - count(lo + 1);
   for (int b0 = 0; b0 < P.n_seq; b0 += 32) {
     const Sequence s = b0 == 0 ? mine : b0 + lane < P.n_seq ? load_sequence(P, b0 + lane) : Sequence{0, 0, 0, 0};
-    const int ge = Cost::at_least(s, P.window, lo), more = Cost::at_least(s, P.window, lo + 1), equal = ge - more;
+    const int ge = items_at_least(s, lo), equal = ge - items_at_least(s, lo + 1);
     int before = equal;
 #pragma unroll
     for (int d = 1; d < 32; d <<= 1) {
@@ -125,9 +109,7 @@ __device__ __forceinline__ int find_item(const PromptParams& P, int rank, int ma
     if (found) {
       const int who = __ffs(found) - 1;
       left -= __shfl_sync(0xffffffffu, before - equal, who);
-      const int n = __shfl_sync(0xffffffffu, Cost::at_least(s, P.window, 0), who);
-      const int ge_w = __shfl_sync(0xffffffffu, ge, who), more_w = __shfl_sync(0xffffffffu, more, who);
-      index = Cost::kFromBack ? n - ge_w + left : more_w + left;
+      index = __shfl_sync(0xffffffffu, items_at_least(s, 0) - ge, who) + left;
       seq.q0 = __shfl_sync(0xffffffffu, s.q0, who);
       seq.nq = __shfl_sync(0xffffffffu, s.nq, who);
       seq.k0 = __shfl_sync(0xffffffffu, s.k0, who);
@@ -185,7 +167,7 @@ __global__ void __launch_bounds__(kPrThreads, 1) prompt_kernel(const PromptParam
   if (warp == 8) {
     Sequence s;
     int index = 0;
-    const int b = find_item<AttentionCost>(P, unit / P.q_heads, (P.k_rows + kPrTile - 1) / kPrTile, s, index);
+    const int b = find_item(P, unit / P.q_heads, (P.k_rows + kPrTile - 1) / kPrTile, s, index);
     if (lane == 0) {
       item_p[0] = b;
       item_p[1] = index;
@@ -572,7 +554,7 @@ __global__ void __launch_bounds__(256) prompt_merge_kernel(const PromptParams P)
   const int unit = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, head = unit % P.q_heads;
   Sequence s;
   int index = 0;
-  if (find_item<AttentionCost>(P, unit / P.q_heads, (P.k_rows + kPrTile - 1) / kPrTile, s, index) < 0) return;
+  if (find_item(P, unit / P.q_heads, (P.k_rows + kPrTile - 1) / kPrTile, s, index) < 0) return;
 #pragma unroll 1
   for (int r = warp; r < kPrMergeRows; r += 8) {
     const int row = blockIdx.y * kPrMergeRows + r, q_row = index * kPrRows + row;
@@ -617,48 +599,153 @@ __global__ void __launch_bounds__(256) prompt_merge_kernel(const PromptParams P)
 }
 
 // ---------------------------------------------------------------------------------------- attention weights of keys
-// An item is 256 keys (tiles A and B, one softmax warpgroup each) of one KV head, or one of P.splits shares of its
-// steps; a step is one query head of the group and 128 queries.  The grid is persistent: the keys and queries of the
-// next item are on their way while this one's are used.  Score tiles are double buffered in tensor memory
-// (x * 256 + 128 * (step % 2)), so that contraction and exponentials run side by side; the exponentials bound it
-// (128 x 128 of them take 1024 cycles of their unit, the contraction 512).
+// An item is 256 keys (tiles A and B, one softmax warpgroup each) of one KV head; a step of it is 128 columns of queries:
+// a tile of 128 queries of one query head of the group or, with a window of at most 64, the windows of 128 / width heads
+// side by side.  The steps of all items form one list (request, KV head, keys rising, then query heads and queries), cut
+// into equal ranges, one per CTA: what an item costs, 256 keys near the end of a sequence a fraction of the first ones,
+// then does not matter.  An item that a range cuts leaves its sums to a second launch; items of few steps are not cut.
+// The keys and queries of the steps to come are on their way while this one's are used; score tiles are double
+// buffered in tensor memory (x * 256 + 128 * (step % 2)), so that contraction and exponentials run side by side.  The
+// exponentials bound it (128 x 128 of them take 1024 cycles of their unit, the contraction 512).
+constexpr int kPwColumns = 4;                                 // steps whose columns are described ahead
+constexpr int kPwColumnBytes = kPrTile * 4 + 32;              // the exponents of 128 columns, and a StepNote
+// What a softmax thread has to know of a step.  Key row r of the item is seen by queries lo + r .. hi - 1 of a window, the
+// columns from `columns` on belong to no head.  The last step of a range in an item tells where its sums go: `keys` rows
+// of them, at weights + at or, of an item that is cut, at records + at.
+struct StepNote {
+  int lo, hi, columns, keys;
+  long long at;
+  int last, cut;
+};
+static_assert(sizeof(StepNote) == 32, "behind 128 exponents");
 template <int D>
 struct WeightsShape {
   static constexpr int kSlabs = D / 64;
   static constexpr int kTileBytes = kSlabs * kPrSlab;
   static constexpr int kStages = D == 128 ? 2 : 4;            // query tiles in flight
   static constexpr int kTiles = (4 + kStages) * kTileBytes;   // two items' key tiles A and B, the query tiles
-  static constexpr int kBars = 4 + 2 * kStages + 8 + 1;
-  static constexpr int kBarOffset = kTiles + 64, kLseOffset = kBarOffset + 8 * kBars + 8;
-  static constexpr int kSmem = kLseOffset + 2 * 2 * kPrTile * 4;
+  static constexpr int kBars = 4 + 2 * kStages + 8 + 2 * kPwColumns + 1;
+  // after the tiles: TMEM base, abort flag, request counts; the range; barriers; what the columns of the next steps are
+  static constexpr int kRangeOffset = kTiles + 16, kBarOffset = kTiles + 128, kColumnsOffset = kBarOffset + 8 * kBars + 8;
+  static constexpr int kSmem = kColumnsOffset + kPwColumns * kPwColumnBytes;
 };
+constexpr int kPwWhole = 8;       // items of at most so many steps are not cut
+constexpr int kPwEvery = 8;       // a pair of columns in so many takes the FMA units
 
-struct WeightsItem {
-  Sequence s;
-  int kvh, key0, w0, nw, qt0, first, steps;      // first: of this share among all steps of the item
-  long long unit;
+// The steps of one KV head of a sequence.  Key tile t costs `groups` x (tiles - first(t)) steps, first(t) being its first
+// tile of queries with one that sees its first key: min(max(2 t - lag, 0), tiles).
+struct KeySteps {
+  int nw, w0, tiles, lag, items, groups;
+  __device__ __forceinline__ KeySteps(const PromptParams& P, const Sequence& s) {
+    nw = P.window > 0 ? min(P.window, s.nq) : s.nq;      // queries that count, behind the first w0
+    w0 = s.nq - nw;
+    tiles = (nw + kPrTile - 1) / kPrTile;
+    lag = (s.nk - nw + kPrTile - 1) >> 7;
+    items = tiles > 0 ? (s.nk + kPrRows - 1) / kPrRows : 0;      // without queries there are no steps
+    groups = (P.q_heads / P.kv_heads * P.width + kPrTile - 1) / kPrTile;
+  }
+  __device__ __forceinline__ int first(int t) const { return min(max(2 * t - lag, 0), tiles); }
+  __device__ __forceinline__ int cost(int t) const { return groups * (tiles - first(t)); }
+  __device__ __forceinline__ long long before(int t) const {
+    // the sum of first() from 0 to t - 1: zero up to lag / 2, then rising by two, then `tiles`
+    const long long full = min(t, max((tiles + lag + 1) >> 1, 0)), start = min((long long)max((lag >> 1) + 1, 0), full);
+    const long long sum = full * (full - 1) - start * (start - 1) - (full - start) * lag + (t - full) * tiles;
+    return groups * ((long long)t * tiles - sum);
+  }
 };
-// The n-th item of this CTA.  Ranks fall in cost; every other round goes through the CTAs backwards.
-__device__ __forceinline__ bool weights_item(const PromptParams& P, int n, WeightsItem& it) {
-  const int g = gridDim.x;
-  const long long unit = (long long)n * g + ((n & 1) ? g - 1 - (int)blockIdx.x : (int)blockIdx.x);
-  const int per_tile = P.kv_heads * P.splits;
-  int index = 0;
-  if (unit / per_tile > 0x3fffffff ||
-      find_item<WeightsCost>(P, (int)(unit / per_tile), (P.q_rows + kPrTile - 1) / kPrTile, it.s, index) < 0)
-    return false;
-  const int rest = (int)(unit % per_tile), share = rest % P.splits;
-  it.unit = unit;
-  it.kvh = rest / P.splits;
-  it.key0 = index * kPrRows;
-  it.nw = P.window > 0 ? min(P.window, it.s.nq) : it.s.nq;
-  it.w0 = it.s.nq - it.nw;
-  const int tiles = (it.nw + kPrTile - 1) / kPrTile;
-  it.qt0 = min(max((it.key0 - (it.s.nk - it.nw)) >> 7, 0), tiles);
-  const long long all = (long long)(tiles - it.qt0) * (P.q_heads / P.kv_heads);
-  it.first = (int)(all * share / P.splits);
-  it.steps = (int)(all * (share + 1) / P.splits) - it.first;
-  return true;
+__device__ __forceinline__ long long shuffle64(long long v, int lane) {
+  return (long long)__shfl_sync(0xffffffffu, (unsigned long long)v, lane);
+}
+// Steps of all items; the whole warp takes part.
+__device__ __forceinline__ long long count_steps(const PromptParams& P) {
+  long long n = 0;
+  for (int b = threadIdx.x & 31; b < P.n_seq; b += 32) {
+    const KeySteps k(P, load_sequence(P, b));
+    n += k.before(k.items);
+  }
+#pragma unroll
+  for (int d = 16; d; d >>= 1) n += (long long)__shfl_xor_sync(0xffffffffu, (unsigned long long)n, d);
+  return n * P.kv_heads;
+}
+// A place in the list of steps.
+struct StepCursor {
+  int b, kvh, tile, step, cost;      // step: inside the item, of `cost`
+  Sequence s;
+};
+// The place of step u, which exists; the whole warp takes part.
+__device__ __forceinline__ StepCursor seek_step(const PromptParams& P, long long u) {
+  const int lane = threadIdx.x & 31;
+  StepCursor c = {};
+  for (int b0 = 0; b0 < P.n_seq; b0 += 32) {
+    const Sequence s = b0 + lane < P.n_seq ? load_sequence(P, b0 + lane) : Sequence{0, 0, 0, 0};
+    const KeySteps k(P, s);
+    const long long mine = k.before(k.items) * P.kv_heads;
+    long long sum = mine;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const long long other = (long long)__shfl_up_sync(0xffffffffu, (unsigned long long)sum, d);
+      if (lane >= d) sum += other;
+    }
+    const unsigned found = __ballot_sync(0xffffffffu, sum > u);
+    if (found) {
+      const int who = __ffs(found) - 1;
+      c.b = b0 + who;
+      c.s.q0 = __shfl_sync(0xffffffffu, s.q0, who);
+      c.s.nq = __shfl_sync(0xffffffffu, s.nq, who);
+      c.s.k0 = __shfl_sync(0xffffffffu, s.k0, who);
+      c.s.nk = __shfl_sync(0xffffffffu, s.nk, who);
+      u -= shuffle64(sum - mine, who);
+      break;
+    }
+    u -= shuffle64(sum, 31);
+  }
+  const KeySteps k(P, c.s);
+  const long long per_head = k.before(k.items);
+  c.kvh = (int)(u / per_head);
+  u -= c.kvh * per_head;
+  int lo = 0, hi = k.items;      // before(lo) <= u < before(hi)
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (k.before(mid) <= u) lo = mid;
+    else hi = mid;
+  }
+  c.tile = lo;
+  c.step = (int)(u - k.before(lo));
+  c.cost = k.cost(lo);
+  return c;
+}
+// The first step of the item behind the one of `c`.
+__device__ __forceinline__ void next_item(const PromptParams& P, StepCursor& c) {
+  c.step = 0;
+  if (++c.tile == KeySteps(P, c.s).items) {
+    c.tile = 0;
+    if (++c.kvh == P.kv_heads) {
+      c.kvh = 0;
+      do {
+        if (++c.b >= P.n_seq) return;      // behind the last step
+        c.s = load_sequence(P, c.b);
+      } while (KeySteps(P, c.s).items == 0);
+    }
+  }
+  c.cost = KeySteps(P, c.s).cost(c.tile);
+}
+// The ranges: as equal as whole steps and uncut small items allow.
+__device__ __forceinline__ int range_count(long long total, int ctas) { return (int)min(total, (long long)ctas); }
+__device__ __forceinline__ long long range_start(long long total, int range, int ranges) { return (long long)((double)total / ranges * range); }
+__device__ __forceinline__ int range_of(long long total, long long step, int ranges) {
+  int r = (int)min((long long)((double)step / ((double)total / ranges)), (long long)ranges - 1);
+  while (r > 0 && range_start(total, r, ranges) > step) --r;
+  while (r + 1 < ranges && range_start(total, r + 1, ranges) <= step) ++r;
+  return r;
+}
+__device__ __forceinline__ StepCursor range_cursor(const PromptParams& P, long long total, int range, int ranges, long long& step) {
+  step = range_start(total, range, ranges);
+  StepCursor c = seek_step(P, step);
+  if (c.cost <= kPwWhole) {
+    step -= c.step;
+    c.step = 0;
+  }
+  return c;
 }
 
 template <typename QT, int D>
@@ -674,37 +761,74 @@ __global__ void __launch_bounds__(kPrThreads, 1) prompt_weights_kernel(const Pro
   volatile int* const requested = abort_flag + 1;       // key pairs and query tiles that the TMA warp asked for in all
   const unsigned bars = smem0 + S::kBarOffset;
   const unsigned bar_k = bars /* two items */, bar_kfree = bars + 16, bar_q = bars + 32, bar_qfree = bar_q + 8 * kStages;
-  const unsigned bar_s = bar_qfree + 8 * kStages /* [x][buffer] */, bar_f = bar_s + 32 /* [x][buffer] */, bar_e = bar_f + 32;
+  const unsigned bar_s = bar_qfree + 8 * kStages /* [x][buffer] */, bar_f = bar_s + 32 /* [x][buffer] */;
+  const unsigned bar_c = bar_f + 32 /* columns described */, bar_cfree = bar_c + 8 * kPwColumns, bar_e = bar_cfree + 8 * kPwColumns;
   const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
   follow_stream();
   if (smem0 & 1023u) {
     if (tid == 0) atomicOr(P.status, INQ_STATUS_BAD_INDEX);
     return;
   }
-  if (tid == 0) {
-    *abort_flag = requested[0] = requested[1] = 0;
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      tc_bar_init(bar_k + 8 * i, 1);
-      tc_bar_init(bar_kfree + 8 * i, 1);
+  // One warp each finds the first step of the range and the one behind it, while others set up.
+  struct Range {
+    StepCursor at;
+    long long first, end;
+  };
+  static_assert(sizeof(Range) <= 96, "between the flags and the barriers");
+  Range* const range = (Range*)(pr_raw + S::kRangeOffset);
+  if (warp < 2) {
+    const long long total = count_steps(P);
+    const int ranges = range_count(total, gridDim.x);
+    long long step = 0;
+    StepCursor c = {};
+    const int r = blockIdx.x + warp;
+    if (r < ranges) c = range_cursor(P, total, r, ranges, step);
+    else step = total;
+    if (lane == 0) {
+      if (warp == 0) {
+        range->at = c;
+        range->first = step;
+      } else {
+        range->end = step;
+      }
     }
+  } else if (warp == 2) {
+    if (lane == 0) {
+      *abort_flag = requested[0] = requested[1] = 0;
 #pragma unroll
-    for (int i = 0; i < kStages; ++i) {
-      tc_bar_init(bar_q + 8 * i, 1);
-      tc_bar_init(bar_qfree + 8 * i, 1);
-    }
+      for (int i = 0; i < 2; ++i) {
+        tc_bar_init(bar_k + 8 * i, 1);
+        tc_bar_init(bar_kfree + 8 * i, 1);
+      }
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      tc_bar_init(bar_s + 8 * i, 1);
-      tc_bar_init(bar_f + 8 * i, kPrTile);
+      for (int i = 0; i < kStages; ++i) {
+        tc_bar_init(bar_q + 8 * i, 1);
+        tc_bar_init(bar_qfree + 8 * i, 1);
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        tc_bar_init(bar_s + 8 * i, 1);
+        tc_bar_init(bar_f + 8 * i, kPrTile);
+      }
+#pragma unroll
+      for (int i = 0; i < kPwColumns; ++i) {
+        tc_bar_init(bar_c + 8 * i, 32);
+        tc_bar_init(bar_cfree + 8 * i, 8);
+      }
+      tc_bar_init(bar_e, 1);
+      asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    tc_bar_init(bar_e, 1);
-    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-  }
-  if (blockIdx.x == 0)
-    for (int b = tid; b < P.n_seq; b += kPrThreads)
-      if (bad_sequence(P, b)) atomicOr(P.status, INQ_STATUS_BAD_INDEX);
-  if (warp == 8) {
+  } else if (warp < 8) {
+    // offsets that the tensors do not hold, and keys of a sequence without queries
+    const int t = tid - 96;
+    for (int b = blockIdx.x; b < P.n_seq; b += gridDim.x) {
+      if (t == 0 && bad_sequence(P, b)) atomicOr(P.status, INQ_STATUS_BAD_INDEX);
+      const Sequence s = load_sequence(P, b);
+      if (s.nq == 0)
+        for (int h = 0; h < P.kv_heads; ++h)
+          for (int i = t; i < s.nk; i += 160) P.weights[h * P.weights_stride + s.k0 + i] = 0.f;
+    }
+  } else if (warp == 8) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(tc_smem(tmem_base_p)), "r"(512) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
@@ -713,15 +837,19 @@ __global__ void __launch_bounds__(kPrThreads, 1) prompt_weights_kernel(const Pro
   tc_fence_after();
   const unsigned tmem = *tmem_base_p;
   allow_next();
-  const int group = P.q_heads / P.kv_heads;
-  WeightsItem it;
+  const int group = P.q_heads / P.kv_heads, heads_per_step = kPrTile / P.width;
+  int left = (int)(range->end - range->first);           // steps of this range
 
+  if (warp >= 8) {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kPrIssueRegs));
+  StepCursor at = range->at;
   if (warp == 9) {
     // ================================================================ TMA warp
     int pairs = 0, tiles = 0;      // key pairs and query tiles requested so far
-    for (int n = 0; weights_item(P, n, it); ++n) {
-      if (it.steps == 0) continue;
-      const int kb = pairs & 1;
+    bool go = true;
+    while (go && left > 0) {
+      const KeySteps k(P, at.s);
+      const int kb = pairs & 1, steps = min(left, at.cost - at.step);
       if (pairs >= 2) tc_wait(bar_kfree + 8 * kb, (unsigned)((pairs >> 1) - 1) & 1u, abort_flag);
       if (__any_sync(0xffffffffu, *abort_flag != 0)) break;      // nothing more is asked for; the others run through
       if (lane == 0) {
@@ -730,34 +858,41 @@ __global__ void __launch_bounds__(kPrThreads, 1) prompt_weights_kernel(const Pro
         for (int x = 0; x < 2; ++x)
 #pragma unroll
           for (int c = 0; c < S::kSlabs; ++c)
-            pf_tma(sKb + (2 * kb + x) * kTileBytes + c * kPrSlab, &map_k, 64 * c, it.s.k0 + it.key0 + x * kPrTile, it.kvh, bar_k + 8 * kb);
+            pf_tma(sKb + (2 * kb + x) * kTileBytes + c * kPrSlab, &map_k, 64 * c, at.s.k0 + at.tile * kPrRows + x * kPrTile, at.kvh, bar_k + 8 * kb);
       }
       ++pairs;
-      const int tiles_per_head = (it.nw + kPrTile - 1) / kPrTile - it.qt0;
-      for (int i = 0; i < it.steps; ++i, ++tiles) {
-        const int st = tiles % kStages, step = it.first + i, g = step / tiles_per_head, qt = it.qt0 + step % tiles_per_head;
+      const int qt0 = k.first(at.tile), per_group = k.tiles - qt0;
+      for (int i = 0; i < steps; ++i, ++tiles) {
+        const int st = tiles % kStages, step = at.step + i, g = step / per_group, qt = qt0 + step - g * per_group;
         const bool free = tiles < kStages || tc_wait(bar_qfree + 8 * st, (unsigned)(tiles / kStages - 1) & 1u, abort_flag);
-        if (__any_sync(0xffffffffu, !free)) break;
+        if (__any_sync(0xffffffffu, !free)) {
+          go = false;
+          break;
+        }
         if (lane == 0) {
           requested[1] = tiles + 1;
-          pf_expect(bar_q + 8 * st, kTileBytes);
+          const int heads = min(heads_per_step, group - g * heads_per_step);
+          pf_expect(bar_q + 8 * st, heads * P.width * 2 * D);
+          for (int j = 0; j < heads; ++j)
 #pragma unroll
-          for (int c = 0; c < S::kSlabs; ++c)
-            pf_tma(sQb + st * kTileBytes + c * kPrSlab, &map_q, 64 * c, it.s.q0 + it.w0 + qt * kPrTile, it.kvh * group + g, bar_q + 8 * st);
+            for (int c = 0; c < S::kSlabs; ++c)
+              pf_tma(sQb + st * kTileBytes + c * kPrSlab + j * P.width * 128, &map_q, 64 * c, at.s.q0 + k.w0 + qt * kPrTile,
+                     at.kvh * group + g * heads_per_step + j, bar_q + 8 * st);
         }
       }
+      left -= steps;
+      if (left > 0) next_item(P, at);
     }
   } else if (warp == 8) {
     // ================================================================ MMA warp
     constexpr bool kBf16 = !std::is_same<QT, __half>::value;
     constexpr unsigned idesc = tc_idesc<kBf16, 128, 128, false>();
     int pairs = 0, step = 0;
-    for (int n = 0; weights_item(P, n, it); ++n) {
-      if (it.steps == 0) continue;
-      const int kb = pairs & 1;
+    while (left > 0) {
+      const int kb = pairs & 1, steps = min(left, at.cost - at.step);
       tc_wait(bar_k + 8 * kb, (unsigned)(pairs >> 1) & 1u, abort_flag);
       ++pairs;
-      for (int i = 0; i < it.steps; ++i, ++step) {
+      for (int i = 0; i < steps; ++i, ++step) {
         const int st = step % kStages, buffer = step & 1;
         tc_wait(bar_q + 8 * st, (unsigned)(step / kStages) & 1u, abort_flag);
         for (int x = 0; x < 2; ++x) {
@@ -774,73 +909,135 @@ __global__ void __launch_bounds__(kPrThreads, 1) prompt_weights_kernel(const Pro
             tc_commit(bar_s + 16 * x + 8 * buffer);
             if (x == 1) {
               tc_commit(bar_qfree + 8 * st);
-              if (i + 1 == it.steps) tc_commit(bar_kfree + 8 * kb);
+              if (i + 1 == steps) tc_commit(bar_kfree + 8 * kb);
             }
           }
           __syncwarp();
         }
       }
+      left -= steps;
+      if (left > 0) next_item(P, at);
     }
-  } else if (warp < 8) {
-    // ================================================================ one thread per key row
-    const int x = warp >> 2, row = tid & (kPrTile - 1);
-    const unsigned tS = tmem + ((unsigned)((warp & 3) * 32) << 16) + 256 * x;
-    float* const lse_s = (float*)(pr_raw + S::kLseOffset) + x * 2 * kPrTile;      // [buffer][128]: -lse in units of log 2
-    const unsigned long long scale2 = pf_pair(P.scale_log2e, P.scale_log2e);
+  } else if (warp == 10) {
+    // ================================================================ describes the columns, four to a lane
+    const int width = P.width, column = 4 * lane, column_head = column / width, column_q = column & (width - 1);
     int step = 0;
-    for (int n = 0; weights_item(P, n, it); ++n) {
-      const int tiles_per_head = max((it.nw + kPrTile - 1) / kPrTile - it.qt0, 1);
-      const int key = it.key0 + x * kPrTile + row, hist = it.s.nk - it.nw;     // position of the window's first query
-      // a column without a query, or of one without a key, weighs nothing: -infinity in the place of its exponent
-      auto fetch = [&](int i) {
-        const int all = it.first + i, g = all / tiles_per_head, q = (it.qt0 + all % tiles_per_head) * kPrTile + row;
-        const float l = q < it.nw ? __ldg(P.lse + (it.kvh * group + g) * P.lse_stride + it.s.q0 + it.w0 + q) : __int_as_float(0xff800000);
-        return l == __int_as_float(0xff800000) ? l : -kLog2e * l;
-      };
-      float sum = 0.f, mine = it.steps > 0 ? fetch(0) : 0.f;
-      for (int i = 0; i < it.steps; ++i, ++step) {
-        const int buffer = step & 1, q0 = (it.qt0 + (it.first + i) % tiles_per_head) * kPrTile;
-        float* const ls = lse_s + buffer * kPrTile;
-        ls[row] = mine;
-        if (i + 1 < it.steps) mine = fetch(i + 1);
-        asm volatile("bar.sync %0, 128;" ::"r"(1 + x) : "memory");
+    while (left > 0) {
+      const KeySteps k(P, at.s);
+      const int steps = min(left, at.cost - at.step), qt0 = k.first(at.tile), per_group = k.tiles - qt0, hist = at.s.nk - k.nw;
+      int g = at.step / per_group, qt = qt0 + at.step - g * per_group;
+      for (int i = 0; i < steps; ++i, ++step) {
+        const int c = step % kPwColumns, head = g * heads_per_step + column_head, q = qt * kPrTile + column_q;
+        const float* const lse = P.lse + (long long)(at.kvh * group + head) * P.lse_stride + at.s.q0 + k.w0 + q;
+        float l[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          // a column without a query, or of one without a key, weighs nothing: -infinity in the place of its exponent
+          const float x = head < group && q + j < k.nw ? __ldg(lse + j) : __int_as_float(0xff800000);
+          l[j] = x == __int_as_float(0xff800000) ? x : -kLog2e * x;
+        }
+        if (step >= kPwColumns) tc_wait(bar_cfree + 8 * c, (unsigned)(step / kPwColumns - 1) & 1u, abort_flag);
+        __syncwarp();
+        unsigned char* const to = pr_raw + S::kColumnsOffset + c * kPwColumnBytes;
+        *(float4*)(to + 4 * column) = make_float4(l[0], l[1], l[2], l[3]);
+        if (lane == 0) {
+          StepNote* const note = (StepNote*)(to + 4 * kPrTile);
+          note->lo = at.tile * kPrRows - (hist + qt * kPrTile);
+          note->hi = k.nw - qt * kPrTile;
+          note->columns = min(group - g * heads_per_step, heads_per_step) * width;
+          note->last = i + 1 == steps;
+          note->cut = steps < at.cost;
+          note->keys = note->cut ? kPrRows : at.s.nk - at.tile * kPrRows;
+          // of a cut item: the range that it begins in, and the ranges behind it
+          note->at = note->cut ? ((long long)blockIdx.x * 2 + (at.step == 0)) * kPrRows : at.kvh * P.weights_stride + at.s.k0 + at.tile * kPrRows;
+        }
+        pf_arrive(bar_c + 8 * c);
+        if (++qt == k.tiles) {
+          qt = qt0;
+          ++g;
+        }
+      }
+      left -= steps;
+      if (left > 0) next_item(P, at);
+    }
+  }
+  } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kPrSoftmaxRegs));
+    // ================================================================ one thread per key row
+    const int x = warp >> 2, row = tid & (kPrTile - 1), width = P.width;
+    const unsigned tS = tmem + ((unsigned)((warp & 3) * 32) << 16) + 256 * x;
+    const unsigned long long scale2 = pf_pair(P.scale_log2e, P.scale_log2e);
+    float sum = 0.f;
+    for (int step = 0; step < left; ++step) {
+        const int buffer = step & 1, described = step % kPwColumns;
+        const unsigned char* const about = pr_raw + S::kColumnsOffset + described * kPwColumnBytes;
+        const float* const ls = (const float*)about;
+        const StepNote* const note = (const StepNote*)(about + 4 * kPrTile);
+        tc_wait(bar_c + 8 * described, (unsigned)(step / kPwColumns) & 1u, abort_flag);
+        const int lo = note->lo + x * kPrTile + row, hi = note->hi, columns = note->columns;
+        // the last key of the tile is not seen by the first query, or a column stands for no query
+        const bool masked = note->lo + x * kPrTile + kPrTile - 1 > 0 || hi < width || columns < kPrTile;
         tc_wait(bar_s + 16 * x + 8 * buffer, (unsigned)(step >> 1) & 1u, abort_flag);
         __syncwarp();
         tc_fence_after();
-        const bool masked = hist + q0 < it.key0 + x * kPrTile + kPrTile - 1 || q0 + kPrTile > it.nw;
-        const int lo = key - (hist + q0), hi = it.nw - q0;      // columns lo .. hi - 1 are queries that see this key
-        unsigned long long sum2 = pf_pair(0.f, 0.f);
+        unsigned v[4][32];
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          unsigned v[32];
-          tc_ld32(tS + 128 * buffer + 32 * q, v);
-          tc_wait_ld32(v);
-          if (masked)
+        for (int q = 0; q < 4; ++q) tc_ld32(tS + 128 * buffer + 32 * q, v[q]);
 #pragma unroll
-            for (int c = 0; c < 32; ++c)
-              if (32 * q + c < lo || 32 * q + c >= hi) v[c] = 0xff800000u;
-#pragma unroll
-          for (int c = 0; c < 32; c += 4) {
-            const float4 l4 = *(const float4*)(ls + 32 * q + c);
-            float e0, e1, e2, e3;
-            pf_unpair(pf_fma2(pf_pair(__uint_as_float(v[c]), __uint_as_float(v[c + 1])), scale2, pf_pair(l4.x, l4.y)), e0, e1);
-            pf_unpair(pf_fma2(pf_pair(__uint_as_float(v[c + 2]), __uint_as_float(v[c + 3])), scale2, pf_pair(l4.z, l4.w)), e2, e3);
-            sum2 = pf_add2(sum2, pf_pair(pf_exp2(e0), pf_exp2(e1)));
-            sum2 = pf_add2(sum2, pf_pair(pf_exp2(e2), pf_exp2(e3)));
-          }
-        }
+        for (int q = 0; q < 4; ++q) tc_wait_ld32(v[q]);
         tc_fence_before();
         pf_arrive(bar_f + 16 * x + 8 * buffer);
+        unsigned long long sums[2] = {pf_pair(0.f, 0.f), pf_pair(0.f, 0.f)};
+        if (masked) {
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            if (32 * q >= columns || (width == kPrTile && 32 * q >= hi)) break;
+#pragma unroll
+            for (int c = 0; c < 32; c += 4) {
+              const float4 l4 = *(const float4*)(ls + 32 * q + c);
+              const float l[4] = {l4.x, l4.y, l4.z, l4.w};
+              float e[4];
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                const int i_q = (32 * q + c + i) & (width - 1);
+                e[i] = i_q < lo || i_q >= hi || 32 * q + c + i >= columns ? 0.f : pf_exp2(fmaf(__uint_as_float(v[q][c + i]), P.scale_log2e, l[i]));
+              }
+              sums[0] = pf_add2(sums[0], pf_pair(e[0], e[1]));
+              sums[1] = pf_add2(sums[1], pf_pair(e[2], e[3]));
+            }
+          }
+        } else {
+          // of four pairs of exponentials one goes to the FMA units
+#pragma unroll
+          for (int q = 0; q < 4; ++q)
+#pragma unroll
+            for (int c = 0; c < 32; c += 4) {
+              const float4 l4 = *(const float4*)(ls + 32 * q + c);
+              const unsigned long long a = pf_fma2(pf_pair(__uint_as_float(v[q][c]), __uint_as_float(v[q][c + 1])), scale2, pf_pair(l4.x, l4.y));
+              const unsigned long long b = pf_fma2(pf_pair(__uint_as_float(v[q][c + 2]), __uint_as_float(v[q][c + 3])), scale2, pf_pair(l4.z, l4.w));
+              float e0, e1, e2, e3;
+              if (c % kPwEvery == 0) {
+                pf_exp2_fma<5>(a, e0, e1);
+              } else {
+                pf_unpair(a, e0, e1);
+                e0 = pf_exp2(e0);
+                e1 = pf_exp2(e1);
+              }
+              pf_unpair(b, e2, e3);
+              sums[0] = pf_add2(sums[0], pf_pair(e0, e1));
+              sums[1] = pf_add2(sums[1], pf_pair(pf_exp2(e2), pf_exp2(e3)));
+            }
+        }
+        const unsigned long long sum2 = pf_add2(sums[0], sums[1]);
         float even, odd;
         pf_unpair(sum2, even, odd);
         sum += even + odd;
-      }
-      if (key < it.s.nk && *abort_flag == 0) {
-        // a cut item's shares lie one behind the other: [share][kv head][key row]
-        const int share = (int)(it.unit % P.splits);
-        if (P.splits == 1) P.weights[it.kvh * P.weights_stride + it.s.k0 + key] = sum;
-        else P.records[((long long)share * P.kv_heads + it.kvh) * P.k_rows + it.s.k0 + key] = sum;
-      }
+        if (note->last) {
+          if (x * kPrTile + row < note->keys && *abort_flag == 0) (note->cut ? P.records : P.weights)[note->at + x * kPrTile + row] = sum;
+          sum = 0.f;
+        }
+        __syncwarp();
+        if (lane == 0) pf_arrive(bar_cfree + 8 * described);
     }
   }
   tc_fence_before();
@@ -864,22 +1061,21 @@ __global__ void __launch_bounds__(kPrThreads, 1) prompt_weights_kernel(const Pro
   }
 }
 
-// Adds the shares of cut items, in their order.  Rows of no sequence stay as they are.
-__global__ void __launch_bounds__(256) prompt_weights_sum_kernel(const PromptParams P) {
+// Adds the parts of the items that ranges cut, in their order: block r takes the item that is cut where range r ends, if
+// it begins in range r.
+__global__ void __launch_bounds__(kPrRows) prompt_weights_sum_kernel(const PromptParams P, int ctas) {
   follow_stream();
-  const int row = blockIdx.x * 256 + threadIdx.x, h = blockIdx.y;
-  if (row >= P.k_rows) return;
-  int lo = 0, hi = P.n_seq;      // the last sequence that starts at or before the row
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    if (__ldg(P.cu_k + mid) <= row) lo = mid;
-    else hi = mid;
-  }
-  const Sequence s = load_sequence(P, lo);
-  if (row < s.k0 || row >= s.k0 + s.nk) return;
-  float sum = 0.f;
-  for (int g = 0; g < P.splits; ++g) sum += __ldcg(P.records + ((long long)g * P.kv_heads + h) * P.k_rows + row);
-  P.weights[h * P.weights_stride + row] = sum;
+  const long long total = count_steps(P);
+  const int ranges = range_count(total, ctas), r = blockIdx.x;
+  if (r + 1 >= ranges) return;
+  const long long cut = range_start(total, r + 1, ranges);
+  const StepCursor c = seek_step(P, cut);
+  if (c.step == 0 || c.cost <= kPwWhole || range_of(total, cut - c.step, ranges) != r) return;
+  const int last = range_of(total, cut - c.step + c.cost - 1, ranges);
+  float sum = __ldcg(P.records + (2LL * r + 1) * kPrRows + threadIdx.x);
+  for (int i = r + 1; i <= last; ++i) sum += __ldcg(P.records + 2LL * i * kPrRows + threadIdx.x);
+  const int key = c.tile * kPrRows + threadIdx.x;
+  if (key < c.s.nk) P.weights[c.kvh * P.weights_stride + c.s.k0 + key] = sum;
 }
 
 }  // namespace inq
@@ -948,20 +1144,21 @@ int attention_cuts(int q_heads, long long q_rows, long long k_rows, int n_seq, i
   }
   return cuts;
 }
-// Shares of an item of inq_prompt_weights: as many as make eight items per SM, each of four steps at least.
-int weights_cuts(int q_heads, int kv_heads, long long q_rows, long long k_rows, int n_seq, int window, int n_sm) {
-  const long long items = std::max<long long>(1, most_tiles(k_rows, n_seq) * kv_heads);
-  const double queries = std::min<double>((double)q_rows / n_seq, window > 0 ? window : 1e30);
-  const double steps = std::max(1.0, queries / kPrTile) * (q_heads / kv_heads);
-  return std::max(1, (int)std::min<double>(std::min<double>(kPrMaxSplits, 8.0 * n_sm / items), steps / 4.0));
+// Columns of a step per query head: windows of at most 64 queries lie side by side, as many as the group has heads for.
+int weights_width(int group, int window) {
+  int width = kPrTile;
+  while (window > 0 && width > 16 && window <= width / 2 && kPrTile / width < group) width /= 2;
+  return width;
+}
+// Whether an item of inq_prompt_weights may be cut.
+bool weights_cut(int group, long long q_rows, int window) {
+  const int width = weights_width(group, window);
+  const long long tiles = (std::min<long long>(q_rows, window > 0 ? window : q_rows) + kPrTile - 1) / kPrTile;
+  return tiles * ((group * width + kPrTile - 1) / kPrTile) > kPwWhole;
 }
 long long attention_record_bytes(int q_heads, int head_dim, long long q_rows, int n_seq, int cuts) {
   return cuts > 1 ? most_tiles(q_rows, n_seq) * q_heads * cuts * kPrRows * (head_dim + 2) * (long long)sizeof(float) : 0;
 }
-long long weights_record_bytes(int kv_heads, long long k_rows, int cuts) {
-  return cuts > 1 ? (long long)cuts * kv_heads * k_rows * (long long)sizeof(float) : 0;
-}
-
 template <typename QT, int D>
 int launch_attention(const PromptParams& P, unsigned ctas, cudaStream_t stream, const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v) {
   const int fit = prompt_registers_fit((const void*)prompt_kernel<QT, D>);
@@ -974,10 +1171,11 @@ int launch_attention(const PromptParams& P, unsigned ctas, cudaStream_t stream, 
 }
 template <typename QT, int D>
 int launch_weights(const PromptParams& P, unsigned ctas, cudaStream_t stream, const CUtensorMap& q, const CUtensorMap& k) {
+  const int fit = prompt_registers_fit((const void*)prompt_weights_kernel<QT, D>);
+  if (fit != INQ_OK) return fit;
   INQ_CUDA_CHECK(cudaFuncSetAttribute(prompt_weights_kernel<QT, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, WeightsShape<D>::kSmem));
   INQ_CUDA_CHECK(launch_following(prompt_weights_kernel<QT, D>, ctas, kPrThreads, WeightsShape<D>::kSmem, stream, P, q, k));
-  if (P.splits > 1)
-    INQ_CUDA_CHECK(launch_following(prompt_weights_sum_kernel, dim3((P.k_rows + 255) / 256, P.kv_heads), 256, 0, stream, P));
+  if (P.records) INQ_CUDA_CHECK(launch_following(prompt_weights_sum_kernel, ctas, kPrRows, 0, stream, P, (int)ctas));
   return INQ_OK;
 }
 }  // namespace
@@ -986,7 +1184,7 @@ extern "C" int64_t inq_prompt_workspace_bytes(int32_t q_heads, int32_t kv_heads,
                                               int32_t n_seq, int32_t weights, int32_t window) {
   int n_sm = 0;
   if (q_heads < 1 || kv_heads < 1 || n_seq < 1 || q_rows < 0 || k_rows < 0 || sm_count(&n_sm) != INQ_OK) return 0;
-  return weights ? weights_record_bytes(kv_heads, k_rows, weights_cuts(q_heads, kv_heads, q_rows, k_rows, n_seq, window, n_sm))
+  return weights ? weights_cut(q_heads / kv_heads, q_rows, window) ? 2LL * n_sm * kPrRows * (int64_t)sizeof(float) : 0
                  : attention_record_bytes(q_heads, head_dim, q_rows, n_seq, attention_cuts(q_heads, q_rows, k_rows, n_seq, n_sm));
 }
 
@@ -1030,15 +1228,14 @@ extern "C" int inq_prompt_weights(const inq_prompt_args_t* a, inq_stream_t strea
   int n_sm = 0;
   const int sm_rc = sm_count(&n_sm);
   if (sm_rc != INQ_OK) return sm_rc;
-  const long long items = most_tiles(a->k_rows, a->n_seq) * a->kv_heads;
-  P.splits = weights_cuts(a->q_heads, a->kv_heads, a->q_rows, a->k_rows, a->n_seq, a->window, n_sm);
-  if (!a->workspace || a->workspace_bytes < weights_record_bytes(a->kv_heads, a->k_rows, P.splits)) P.splits = 1;
-  if (items * P.splits > 0x7fffffffLL) return INQ_ERR_CAPACITY;
+  P.width = weights_width(a->q_heads / a->kv_heads, a->window);
+  if (!weights_cut(a->q_heads / a->kv_heads, a->q_rows, a->window)) P.records = nullptr;
+  else if (!a->workspace || a->workspace_bytes < 2LL * n_sm * kPrRows * (long long)sizeof(float)) return INQ_ERR_CAPACITY;
   CUtensorMap map_q, map_k;
-  if (!make_map(&map_q, a->q, a->dtype, a->head_dim, a->q_rows, a->q_heads, a->q_stride_t, a->q_stride_h, kPrTile) ||
+  if (!make_map(&map_q, a->q, a->dtype, a->head_dim, a->q_rows, a->q_heads, a->q_stride_t, a->q_stride_h, P.width) ||
       !make_map(&map_k, a->k, a->dtype, a->head_dim, a->k_rows, a->kv_heads, a->k_stride_t, a->k_stride_h, kPrTile))
     return INQ_ERR_ARGUMENT;
-  const unsigned ctas = (unsigned)std::min<long long>(items * P.splits, n_sm);
+  const unsigned ctas = (unsigned)n_sm;
   cudaStream_t stream = (cudaStream_t)stream_;
   if (a->dtype == INQ_F16)
     return a->head_dim == 64 ? launch_weights<__half, 64>(P, ctas, stream, map_q, map_k) : launch_weights<__half, 128>(P, ctas, stream, map_q, map_k);
