@@ -630,7 +630,6 @@ struct WeightsShape {
   static constexpr int kSmem = kColumnsOffset + kPwColumns * kPwColumnBytes;
 };
 constexpr int kPwWhole = 8;       // items of at most so many steps are not cut
-constexpr int kPwEvery = 8;       // a pair of columns in so many takes the FMA units
 
 // The steps of one KV head of a sequence.  Key tile t costs `groups` x (tiles - first(t)) steps, first(t) being its first
 // tile of queries with one that sees its first key: min(max(2 t - lag, 0), tiles).
@@ -969,75 +968,76 @@ __global__ void __launch_bounds__(kPrThreads, 1) prompt_weights_kernel(const Pro
     const unsigned long long scale2 = pf_pair(P.scale_log2e, P.scale_log2e);
     float sum = 0.f;
     for (int step = 0; step < left; ++step) {
-        const int buffer = step & 1, described = step % kPwColumns;
-        const unsigned char* const about = pr_raw + S::kColumnsOffset + described * kPwColumnBytes;
-        const float* const ls = (const float*)about;
-        const StepNote* const note = (const StepNote*)(about + 4 * kPrTile);
-        tc_wait(bar_c + 8 * described, (unsigned)(step / kPwColumns) & 1u, abort_flag);
-        const int lo = note->lo + x * kPrTile + row, hi = note->hi, columns = note->columns;
-        // the last key of the tile is not seen by the first query, or a column stands for no query
-        const bool masked = note->lo + x * kPrTile + kPrTile - 1 > 0 || hi < width || columns < kPrTile;
-        tc_wait(bar_s + 16 * x + 8 * buffer, (unsigned)(step >> 1) & 1u, abort_flag);
-        __syncwarp();
-        tc_fence_after();
-        unsigned v[4][32];
+      const int buffer = step & 1, described = step % kPwColumns;
+      const unsigned char* const about = pr_raw + S::kColumnsOffset + described * kPwColumnBytes;
+      const float* const exponents = (const float*)about;
+      const StepNote* const note = (const StepNote*)(about + 4 * kPrTile);
+      tc_wait(bar_c + 8 * described, (unsigned)(step / kPwColumns) & 1u, abort_flag);
+      const int lo = note->lo + x * kPrTile + row, hi = note->hi, columns = note->columns;
+      // the last key of the tile is not seen by the first query, or a column stands for no query
+      const bool masked = note->lo + x * kPrTile + kPrTile - 1 > 0 || hi < width || columns < kPrTile;
+      tc_wait(bar_s + 16 * x + 8 * buffer, (unsigned)(step >> 1) & 1u, abort_flag);
+      __syncwarp();
+      tc_fence_after();
+      unsigned v[4][32];
 #pragma unroll
-        for (int q = 0; q < 4; ++q) tc_ld32(tS + 128 * buffer + 32 * q, v[q]);
+      for (int q = 0; q < 4; ++q) tc_ld32(tS + 128 * buffer + 32 * q, v[q]);
 #pragma unroll
-        for (int q = 0; q < 4; ++q) tc_wait_ld32(v[q]);
-        tc_fence_before();
-        pf_arrive(bar_f + 16 * x + 8 * buffer);
-        unsigned long long sums[2] = {pf_pair(0.f, 0.f), pf_pair(0.f, 0.f)};
-        if (masked) {
+      for (int q = 0; q < 4; ++q) tc_wait_ld32(v[q]);
+      tc_fence_before();
+      pf_arrive(bar_f + 16 * x + 8 * buffer);
+      unsigned long long sums[2] = {pf_pair(0.f, 0.f), pf_pair(0.f, 0.f)};
+      // Columns q .. q + 31; bit c of `seen`: column q + c counts.  Of every eight pairs of exponentials three take the FMA
+      // units: MUFU and FMA units are then busy for about as long.
+      auto add = [&](int q, auto some, unsigned seen) {
 #pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            if (32 * q >= columns || (width == kPrTile && 32 * q >= hi)) break;
+        for (int c = 0; c < 32; c += 4) {
+          const float4 l4 = *(const float4*)(exponents + 32 * q + c);
 #pragma unroll
-            for (int c = 0; c < 32; c += 4) {
-              const float4 l4 = *(const float4*)(ls + 32 * q + c);
-              const float l[4] = {l4.x, l4.y, l4.z, l4.w};
-              float e[4];
-#pragma unroll
-              for (int i = 0; i < 4; ++i) {
-                const int i_q = (32 * q + c + i) & (width - 1);
-                e[i] = i_q < lo || i_q >= hi || 32 * q + c + i >= columns ? 0.f : pf_exp2(fmaf(__uint_as_float(v[q][c + i]), P.scale_log2e, l[i]));
-              }
-              sums[0] = pf_add2(sums[0], pf_pair(e[0], e[1]));
-              sums[1] = pf_add2(sums[1], pf_pair(e[2], e[3]));
+          for (int p = 0; p < 2; ++p) {
+            const int i = c + 2 * p;
+            const unsigned long long e2 = pf_fma2(pf_pair(__uint_as_float(v[q][i]), __uint_as_float(v[q][i + 1])), scale2,
+                                                  p ? pf_pair(l4.z, l4.w) : pf_pair(l4.x, l4.y));
+            float e0, e1;
+            if ((i / 2) % 8 == 0 || (i / 2) % 8 == 3 || (i / 2) % 8 == 6) {
+              pf_exp2_fma<5>(e2, e0, e1);
+            } else {
+              pf_unpair(e2, e0, e1);
+              e0 = pf_exp2(e0);
+              e1 = pf_exp2(e1);
             }
+            if (decltype(some)::value) {      // whatever a column that does not count holds
+              e0 = seen & (1u << i) ? e0 : 0.f;
+              e1 = seen & (2u << i) ? e1 : 0.f;
+            }
+            sums[p] = pf_add2(sums[p], pf_pair(e0, e1));
           }
-        } else {
-          // of four pairs of exponentials one goes to the FMA units
-#pragma unroll
-          for (int q = 0; q < 4; ++q)
-#pragma unroll
-            for (int c = 0; c < 32; c += 4) {
-              const float4 l4 = *(const float4*)(ls + 32 * q + c);
-              const unsigned long long a = pf_fma2(pf_pair(__uint_as_float(v[q][c]), __uint_as_float(v[q][c + 1])), scale2, pf_pair(l4.x, l4.y));
-              const unsigned long long b = pf_fma2(pf_pair(__uint_as_float(v[q][c + 2]), __uint_as_float(v[q][c + 3])), scale2, pf_pair(l4.z, l4.w));
-              float e0, e1, e2, e3;
-              if (c % kPwEvery == 0) {
-                pf_exp2_fma<5>(a, e0, e1);
-              } else {
-                pf_unpair(a, e0, e1);
-                e0 = pf_exp2(e0);
-                e1 = pf_exp2(e1);
-              }
-              pf_unpair(b, e2, e3);
-              sums[0] = pf_add2(sums[0], pf_pair(e0, e1));
-              sums[1] = pf_add2(sums[1], pf_pair(pf_exp2(e2), pf_exp2(e3)));
-            }
         }
-        const unsigned long long sum2 = pf_add2(sums[0], sums[1]);
-        float even, odd;
-        pf_unpair(sum2, even, odd);
-        sum += even + odd;
-        if (note->last) {
-          if (x * kPrTile + row < note->keys && *abort_flag == 0) (note->cut ? P.records : P.weights)[note->at + x * kPrTile + row] = sum;
-          sum = 0.f;
+      };
+      if (!masked) {
+#pragma unroll
+        for (int q = 0; q < 4; ++q) add(q, std::false_type{}, 0u);
+      } else {
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          if (32 * q < columns) {
+            // columns of queries lo .. hi - 1 of a window, of one head, of half a window, or of two heads
+            const int base = 32 * q & (width - 1), from = min(max(lo - base, 0), 32), to = min(max(hi - base, 0), 32);
+            unsigned seen = (unsigned)((1ull << to) - 1ull) & ~(unsigned)((1ull << from) - 1ull);
+            if (width == 16) seen = (seen & 0xffffu) | (32 * q + 16 < columns ? seen << 16 : 0u);
+            if (__any_sync(0xffffffffu, seen != 0u)) add(q, std::true_type{}, seen);
+          }
         }
-        __syncwarp();
-        if (lane == 0) pf_arrive(bar_cfree + 8 * described);
+      }
+      float even, odd;
+      pf_unpair(pf_add2(sums[0], sums[1]), even, odd);
+      sum += even + odd;
+      if (note->last) {
+        if (x * kPrTile + row < note->keys && *abort_flag == 0) (note->cut ? P.records : P.weights)[note->at + x * kPrTile + row] = sum;
+        sum = 0.f;
+      }
+      __syncwarp();
+      if (lane == 0) pf_arrive(bar_cfree + 8 * described);
     }
   }
   tc_fence_before();
