@@ -37,35 +37,6 @@ __device__ __forceinline__ unsigned long long pf_add2(unsigned long long a, unsi
   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
   return d;
 }
-// 2^x of a pair on the FMA units, beside the exponential unit that bounds kernels of many exponentials: x = n + f with
-// n the nearest integer (it falls into the low bits of x + 3 2^22) and |f| <= 1/2, 2^f by a polynomial, n added to its
-// exponent.  The polynomials are minimax fits of the relative error on that interval (Remez exchange), in fp32 off by at
-// most 7.5e-5, 2.7e-6 and 2.2e-7 for degrees 3, 4 and 5.  x is at most 126 and counts as -126 below that, so that 2^-126
-// stands for anything smaller, zero included; a NaN stays one.
-template <int DEGREE>
-__device__ __forceinline__ void pf_exp2_fma(unsigned long long x2, float& e0, float& e1) {
-  static_assert(DEGREE >= 3 && DEGREE <= 5, "a polynomial of these");
-  constexpr float kFit[3][6] = {{0.9999280571937561f, 0.6932609677314758f, 0.2426111251115799f, 0.0551716685295105f, 0.f, 0.f},
-                                {0.9999992847442627f, 0.6931217908859253f, 0.240247443318367f, 0.05591785907745361f, 0.009570102207362652f, 0.f},
-                                {1.0000001192092896f, 0.6931469440460205f, 0.24022120237350464f, 0.05550713092088699f, 0.009675540961325169f,
-                                 0.0013276472454890609f}};
-  constexpr float kShift = 12582912.f;
-  float x0, x1;
-  pf_unpair(x2, x0, x1);
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(x0) : "f"(x0), "f"(-126.f));
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(x1) : "f"(x1), "f"(-126.f));
-  x2 = pf_pair(x0, x1);
-  const unsigned long long t2 = pf_add2(x2, pf_pair(kShift, kShift)), n2 = pf_add2(t2, pf_pair(-kShift, -kShift));
-  const unsigned long long f2 = pf_fma2(n2, pf_pair(-1.f, -1.f), x2);
-  unsigned long long p2 = pf_pair(kFit[DEGREE - 3][DEGREE], kFit[DEGREE - 3][DEGREE]);
-#pragma unroll
-  for (int k = DEGREE - 1; k >= 0; --k) p2 = pf_fma2(p2, f2, pf_pair(kFit[DEGREE - 3][k], kFit[DEGREE - 3][k]));
-  float t0, t1, p0, p1;
-  pf_unpair(t2, t0, t1);
-  pf_unpair(p2, p0, p1);
-  e0 = __int_as_float(__float_as_int(p0) + (__float_as_int(t0) << 23));
-  e1 = __int_as_float(__float_as_int(p1) + (__float_as_int(t1) << 23));
-}
 template <typename QT>
 __device__ __forceinline__ unsigned pf_pack2(float lo, float hi) {
   if (std::is_same<QT, __half>::value) {
