@@ -224,3 +224,238 @@ def _evict_tokens(key_pages, value_pages, block_table, lengths, weights, positio
         args.workspace, args.workspace_bytes = scratch.data_ptr(), need
         N.check(N.library().inq_evict_tokens(ctypes.byref(args), N.stream_pointer(device)), "inq_evict_tokens")
     return out_lengths, out_weights, out_positions
+
+
+class PromptStep:
+    """The prompts (or chunks of prompts) of one step of a ``DensePagedCache``: what its layers share."""
+
+    def __init__(self, cache: "DensePagedCache", requests: list, tokens: list[int]):
+        device = cache.device
+        self.cache, self.requests, self.tokens = cache, list(requests), [int(n) for n in tokens]
+        if len(set(self.requests)) != len(self.requests) or len(self.requests) != len(self.tokens) or not self.requests:
+            raise ValueError("one positive token count per request, every request once")
+        if min(self.tokens) < 1:
+            raise ValueError("one positive token count per request, every request once")
+        self.slots = [cache.slot(r) for r in self.requests]
+        self.past = [cache._held[s] for s in self.slots]
+        for slot, past, n in zip(self.slots, self.past, self.tokens):
+            cache._reserve(slot, past + n)
+        cache._write_table()
+        starts, keys = [0], [0]
+        for past, n in zip(self.past, self.tokens):
+            starts.append(starts[-1] + n)
+            keys.append(keys[-1] + past + n)
+        self.cu_seqlens = torch.tensor(starts, dtype=torch.int32).to(device)
+        self.cu_seqlens_k = self.cu_seqlens if not any(self.past) else torch.tensor(keys, dtype=torch.int32).to(device)
+        # where every key row lies (request by request: cached tokens, then new ones), and which rows are new
+        pages, offsets, new = [], [], []
+        for slot, past, n in zip(self.slots, self.past, self.tokens):
+            t = torch.arange(past + n)
+            pages.append(torch.tensor(cache._pages[slot])[t // cache.page_tokens])
+            offsets.append(t % cache.page_tokens)
+            new.append(t >= past)
+        self.pages, self.offsets = torch.cat(pages).to(device), torch.cat(offsets).to(device)
+        is_new = torch.cat(new).to(device)
+        self.new_pages, self.new_offsets = self.pages[is_new], self.offsets[is_new]
+        self.done = False
+
+    @torch.no_grad()
+    def attend(self, layer: int, query: torch.Tensor, key: torch.Tensor, value: torch.Tensor, *, scale: float | None = None,
+               window: int | None = None) -> torch.Tensor:
+        """Attention of the step's packed rows ``query`` [T, Hq, D] over what the cache holds and over themselves; ``key`` and
+        ``value`` [T, H, D] are stored.  In a cache with weights, what every key received from the last ``window``
+        queries of its request (all of them where it is not given) is added to its weight."""
+        cache = self.cache
+        if self.done:
+            raise RuntimeError("state mismatch: this step was finished")
+        total = sum(self.tokens)
+        if key.shape != (total, cache.kv_heads, cache.head_dim) or value.shape != key.shape or key.dtype != cache.dtype or value.dtype != key.dtype:
+            raise ValueError("Expected key/value [tokens of the step, H, D] of the cache's dtype")
+        key_pages, value_pages = cache.key_pages[layer], cache.value_pages[layer]
+        key_pages[self.new_pages, :, self.new_offsets] = key
+        value_pages[self.new_pages, :, self.new_offsets] = value
+        if self.cu_seqlens_k is not self.cu_seqlens:
+            key, value = key_pages[self.pages, :, self.offsets], value_pages[self.pages, :, self.offsets]
+        out, lse = prompt_attention(query, key, value, self.cu_seqlens, self.cu_seqlens_k, scale=scale)
+        if cache.weights is not None:
+            received = prompt_weights(query, key, lse, self.cu_seqlens, self.cu_seqlens_k, scale=scale, window=window)
+            at = 0
+            for slot, past, n in zip(self.slots, self.past, self.tokens):
+                row = cache.weights[layer, slot]
+                row[:, :past] += received[:, at:at + past]
+                row[:, past:past + n] = received[:, at + past:at + past + n]
+                at += past + n
+        return out
+
+    @torch.no_grad()
+    def finish(self) -> None:
+        """Every layer has attended: the requests hold the step's tokens from now on."""
+        cache = self.cache
+        if self.done:
+            raise RuntimeError("state mismatch: this step was finished")
+        self.done = True
+        for slot, past, n in zip(self.slots, self.past, self.tokens):
+            if cache.positions is not None:
+                cache.positions[:, slot, :, past:past + n] = torch.arange(cache._seen[slot], cache._seen[slot] + n, device=cache.device, dtype=torch.int32)
+            cache._held[slot] = past + n
+            cache._seen[slot] += n
+        cache._write_lengths()
+
+
+class DensePagedCache:
+    """Uncompressed paged cache of several requests and layers, with an optional budget per KV head.
+
+    ``begin_prompt(requests, tokens)`` opens a step of packed prompts (``attend`` per layer, then ``finish``);
+    ``decode(layer, query, key, value)`` attends with one token of every slot, ``advance()`` behind the last layer takes
+    these tokens into account; ``evict(budget)`` cuts every request to its budget and gives back the pages that fell
+    empty.  Rows of a decode call are slots (``slot(request)``); slots without a request give zeros.  ``lengths``,
+    ``seen`` and ``block_table`` live on the device, so that decode calls can be captured into a CUDA graph; pages are
+    handed out by ``advance``, which is not captured.
+
+    ``gather`` returns the tokens of a request as dense rows, for instance for ``InQuantCache.update``: what is left after
+    an eviction can be coded like any other cache."""
+
+    def __init__(self, layers: int, kv_heads: int, head_dim: int, *, pages: int, max_requests: int, max_tokens: int, page_tokens: int = 64,
+                 dtype: torch.dtype = torch.bfloat16, device="cuda", weights: bool = True):
+        if min(layers, kv_heads, pages, max_requests, max_tokens, page_tokens) < 1:
+            raise ValueError("layers, heads, pages, requests and tokens must be positive")
+        if head_dim not in (64, 128) or dtype not in (torch.float16, torch.bfloat16):
+            raise NotImplementedError("the cache holds fp16 or bf16 rows of 64 or 128 channels")
+        self.layers, self.kv_heads, self.head_dim, self.page_tokens, self.max_tokens = layers, kv_heads, head_dim, page_tokens, max_tokens
+        self.dtype, self.device, self.max_requests = dtype, torch.device(device), max_requests
+        if self.device.type == "cuda" and self.device.index is None:
+            self.device = torch.device("cuda", torch.cuda.current_device())
+        columns = -(-max_tokens // page_tokens)
+        shape = (layers, pages, kv_heads, page_tokens, head_dim)
+        self.key_pages = torch.empty(shape, dtype=dtype, device=self.device)
+        self.value_pages = torch.empty(shape, dtype=dtype, device=self.device)
+        self.block_table = torch.zeros((max_requests, columns), dtype=torch.int32, device=self.device)
+        self.lengths = torch.full((max_requests,), -1, dtype=torch.int32, device=self.device)
+        self.seen = torch.zeros((max_requests,), dtype=torch.int32, device=self.device)
+        self.weights = self.positions = None
+        if weights:
+            self.weights = torch.zeros((layers, max_requests, kv_heads, columns * page_tokens), dtype=torch.float32, device=self.device)
+            self.positions = torch.zeros(self.weights.shape, dtype=torch.int32, device=self.device)
+        self._slots: dict = {}                                   # request -> slot
+        self._free_slots = list(range(max_requests))[::-1]
+        self._free_pages = list(range(pages))[::-1]
+        self._pages: list[list[int]] = [[] for _ in range(max_requests)]
+        self._held, self._seen = [0] * max_requests, [0] * max_requests
+
+    # ------------------------------------------------------------------ bookkeeping
+    def slot(self, request) -> int:
+        if request not in self._slots:
+            raise KeyError(f"unknown request {request!r}")
+        return self._slots[request]
+
+    def admit(self, request) -> int:
+        """Gives a request a slot."""
+        if request in self._slots:
+            raise ValueError(f"request {request!r} is in the cache already")
+        if not self._free_slots:
+            raise RuntimeError("no free slot: release a request first")
+        self._slots[request] = slot = self._free_slots.pop()
+        self._held[slot] = self._seen[slot] = 0
+        self._write_lengths()
+        return slot
+
+    def release(self, request) -> None:
+        slot = self.slot(request)
+        del self._slots[request]
+        self._free_pages += self._pages[slot][::-1]
+        self._pages[slot] = []
+        self._free_slots.append(slot)
+        self._write_lengths()
+
+    def tokens(self, request) -> int:
+        """Cached tokens of a request; ``seen`` counts the evicted ones too."""
+        return self._held[self.slot(request)]
+
+    @property
+    def free_pages(self) -> int:
+        return len(self._free_pages)
+
+    def _reserve(self, slot: int, tokens: int) -> None:
+        if tokens > self.max_tokens:
+            raise ValueError(f"a request of {tokens} tokens exceeds max_tokens")
+        need = -(-tokens // self.page_tokens) - len(self._pages[slot])
+        if need > len(self._free_pages):
+            raise RuntimeError("no free pages: evict tokens or release a request first")
+        for _ in range(need):
+            self._pages[slot].append(self._free_pages.pop())
+
+    def _write_table(self) -> None:
+        table = torch.zeros(self.block_table.shape, dtype=torch.int32)
+        for slot, pages in enumerate(self._pages):
+            table[slot, :len(pages)] = torch.tensor(pages, dtype=torch.int32)
+        self.block_table.copy_(table)
+
+    def _write_lengths(self) -> None:
+        used = set(self._slots.values())
+        self.lengths.copy_(torch.tensor([n if s in used else -1 for s, n in enumerate(self._held)], dtype=torch.int32))
+        self.seen.copy_(torch.tensor(self._seen, dtype=torch.int32))
+
+    # ------------------------------------------------------------------ steps
+    def begin_prompt(self, requests: list, tokens: list[int]) -> PromptStep:
+        """A step of packed prompts: ``tokens[i]`` new tokens of ``requests[i]``, behind what it holds.  Pages are reserved here."""
+        return PromptStep(self, requests, tokens)
+
+    def begin_decode(self) -> None:
+        """Reserves a place for one more token of every request."""
+        pages = [len(p) for p in self._pages]
+        for slot in self._slots.values():
+            self._reserve(slot, self._held[slot] + 1)
+        if pages != [len(p) for p in self._pages]:
+            self._write_table()
+
+    def decode(self, layer: int, query: torch.Tensor, key: torch.Tensor, value: torch.Tensor, *, scale: float | None = None,
+               out: torch.Tensor | None = None) -> torch.Tensor:
+        """Attention of one new token per slot, ``query`` [max_requests, Hq, D], over the cached ones and itself; ``key`` and
+        ``value`` [max_requests, H, D] are stored.  Places come from ``begin_decode``."""
+        weights = None if self.weights is None else self.weights[layer]
+        got = paged_attention(query, self.key_pages[layer], self.value_pages[layer], self.block_table, self.lengths, scale=scale, new_key=key,
+                              new_value=value, weights=weights, out=out)
+        return got if weights is None else got[0]
+
+    @torch.no_grad()
+    def advance(self) -> None:
+        """Every layer has decoded: the requests hold one more token each."""
+        if self.positions is not None:
+            place = self.lengths.clamp(0, self.positions.shape[3] - 1).long().view(1, -1, 1, 1).expand(self.layers, -1, self.kv_heads, 1)
+            self.positions.scatter_(3, place, self.seen.view(1, -1, 1, 1).expand(self.layers, -1, self.kv_heads, 1))
+        for slot in self._slots.values():
+            self._held[slot] += 1
+            self._seen[slot] += 1
+        self._write_lengths()
+
+    def evict(self, budget: int, *, sink: int = 4, recent: int = 128) -> None:
+        """Cuts every request to ``budget`` tokens per KV head and layer, see ``evict_tokens``."""
+        if self.weights is None:
+            raise RuntimeError("the cache was built without weights")
+        if budget < 1 or sink < 0 or recent < 0 or sink + recent > budget:
+            raise ValueError("budget must be positive and hold sink and recent tokens")
+        if all(self._held[s] <= budget for s in self._slots.values()):
+            return
+        left = torch.empty_like(self.lengths)
+        for layer in range(self.layers):
+            evict_tokens(self.key_pages[layer], self.value_pages[layer], self.block_table, self.lengths, self.weights[layer],
+                         self.positions[layer], self.seen, budget, sink=sink, recent=recent, out_weights=self.weights[layer],
+                         out_positions=self.positions[layer], out_lengths=left)
+        self.lengths.copy_(left)
+        for slot in self._slots.values():
+            self._held[slot] = min(self._held[slot], budget)
+            keep = -(-self._held[slot] // self.page_tokens)
+            self._free_pages += self._pages[slot][keep:][::-1]
+            del self._pages[slot][keep:]
+        self._write_table()
+
+    @torch.no_grad()
+    def gather(self, layer: int, request) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor | None]:
+        """Key and value rows [1, H, tokens, D] of a request as they lie in the cache, and their positions [H, tokens]."""
+        slot = self.slot(request)
+        n = self._held[slot]
+        t = torch.arange(n)
+        page = torch.tensor(self._pages[slot], dtype=torch.long)[t // self.page_tokens].to(self.device)
+        offset = (t % self.page_tokens).to(self.device)
+        rows = [p[layer][page, :, offset].transpose(0, 1).unsqueeze(0).contiguous() for p in (self.key_pages, self.value_pages)]
+        return rows[0], rows[1], None if self.positions is None else self.positions[layer, slot, :, :n].clone()

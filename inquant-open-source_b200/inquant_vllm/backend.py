@@ -20,7 +20,8 @@ class is a plain object with the attributes vLLM's ``FlashAttentionImpl.__init__
 the state is kept PER REQUEST ID, so several requests can be active at once
 (``max_requests``; the reference serves one).  ``forward`` accepts one request's metadata or an
 ``InQuantBatchMetadata`` that lists several decode requests, which are then served one after
-another on the current stream.
+another on the current stream, or an ``InQuantPromptBatchMetadata`` with the packed prompts of a step,
+which attend in one launch (``inquant.prompt.prompt_attention``).
 """
 from __future__ import annotations
 
@@ -64,6 +65,14 @@ class InQuantBatchMetadata:
     """Several single-token decode requests of one step: ``requests[i]`` describes request i, whose
     query / key / value / output rows are row i of the tensors passed to ``forward``."""
     requests: list = field(default_factory=list)
+
+
+@dataclass
+class InQuantPromptBatchMetadata:
+    """The prompts of one step: the rows of ``requests[i]`` (``context_len`` 0) are ``query_start_loc[i] ..
+    query_start_loc[i + 1]`` of the packed tensors passed to ``forward``, int32 on their device, without gaps from row 0 on."""
+    requests: list = field(default_factory=list)
+    query_start_loc: torch.Tensor | None = None
 
 
 @dataclass
@@ -150,6 +159,35 @@ class InQuantImpl:
     # ------------------------------------------------------------------ steps
     def _prefill(self, m, query, key, value, kv_cache, output) -> None:
         from inquant.prefill import prefill_attention
+        n = m.num_actual_tokens
+        # the whole prompt attends to its fresh, uncompressed K/V; no dense history is kept afterwards
+        result = prefill_attention(query[:n].transpose(0, 1).unsqueeze(0), key[:n].transpose(0, 1).unsqueeze(0),
+                                   value[:n].transpose(0, 1).unsqueeze(0), self.scale)
+        output[:n].copy_(result[0].transpose(0, 1))
+        self._keep_prompt(m, query, key, value, kv_cache)
+
+    def _prefill_batch(self, batch, query, key, value, kv_cache, output) -> None:
+        """All prompts of a step attend in one launch; each is then kept as ``_prefill`` keeps it."""
+        from inquant.prompt import prompt_attention
+        requests = batch.requests
+        if not requests or any(m.context_len != 0 or m.num_actual_tokens < 1 for m in requests):
+            raise RuntimeError("a batch of prompts lists requests without context only")
+        if len(requests) > self.max_requests or len({m.request_id for m in requests}) != len(requests):
+            raise RuntimeError("a batch of prompts lists every request once, and no more than max_requests")
+        starts = batch.query_start_loc
+        if starts is None or starts.numel() != len(requests) + 1:
+            raise ValueError("query_start_loc must hold one offset per request and the end of the last")
+        total = sum(m.num_actual_tokens for m in requests)
+        result, _ = prompt_attention(query[:total], key[:total], value[:total], starts.to(torch.int32), scale=self.scale)
+        output[:total].copy_(result)
+        at = 0
+        for m in requests:
+            rows = slice(at, at + m.num_actual_tokens)
+            self._keep_prompt(m, query[rows], key[rows], value[rows], kv_cache)
+            at = rows.stop
+
+    def _keep_prompt(self, m, query, key, value, kv_cache) -> None:
+        """A prompt's state: its first tokens in the exact sink, its full pages sealed, the rest in the exact tail."""
         n, b = m.num_actual_tokens, self.layout.block_size
         self.finish_request(m.request_id)
         while len(self.requests) >= self.max_requests:      # the oldest request makes room
@@ -158,10 +196,6 @@ class InQuantImpl:
         sink = min(4, n)
         state.dense[0, :, :sink].copy_(key[:sink].transpose(0, 1))
         state.dense[1, :, :sink].copy_(value[:sink].transpose(0, 1))
-        # the whole prompt attends to its fresh, uncompressed K/V; no dense history is kept afterwards
-        result = prefill_attention(query[:n].transpose(0, 1).unsqueeze(0), key[:n].transpose(0, 1).unsqueeze(0),
-                                   value[:n].transpose(0, 1).unsqueeze(0), self.scale)
-        output[:n].copy_(result[0].transpose(0, 1))
         if state.sealed_pages:
             full = state.sealed_pages * b
             keys = key[:full].view(state.sealed_pages, b, self.num_kv_heads, 128).transpose(1, 2)
@@ -232,6 +266,9 @@ class InQuantImpl:
             return output
         if kv_cache.dtype != torch.uint8 or kv_cache.ndim != 2 or kv_cache.shape[1] != self.layout.page_bytes:
             raise RuntimeError("InQuant cache spec was not installed; refusing dense fallback")
+        if isinstance(attn_metadata, InQuantPromptBatchMetadata):
+            self._prefill_batch(attn_metadata, query, key, value, kv_cache, output)
+            return output
         if isinstance(attn_metadata, InQuantBatchMetadata):
             for row, m in enumerate(attn_metadata.requests):
                 if m.context_len == 0 or m.num_actual_tokens != 1:
