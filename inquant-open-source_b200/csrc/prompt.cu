@@ -31,7 +31,6 @@ constexpr int kPrRows = 2 * kPrTile;         // rows per item (tiles A and B)
 constexpr int kPrSlab = kPrTile * 128;       // 128 rows x 128 bytes
 constexpr float kPrNegBig = -3.0e38f;        // stands for the maximum of nothing: below every finite logit that matters
 constexpr float kPrSlack = 8.f;              // the reference maximum may lag the true one by 2^8
-constexpr int kPrMaxSplits = 8;
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
 struct PromptParams {
@@ -41,7 +40,6 @@ struct PromptParams {
   long long o_sh, o_st, lse_stride, weights_stride;
   const int *cu_q, *cu_k;
   int n_seq, q_rows, k_rows, q_heads, kv_heads;
-  int splits;
   int window;                       // weights: queries per sequence that count, 0 = all
   int width;                        // weights: columns of a step per query head
   float* records;                   // partial results of cut items
@@ -121,21 +119,183 @@ __device__ __forceinline__ int find_item(const PromptParams& P, int rank, int ma
   return -1;
 }
 
+// How the items of a launch are dealt to its CTAs.  Ordinarily whole: in the order of falling cost, every other round through
+// the CTAs backwards, so that they end at about the same time.  Where that leaves SMs idle -- few items behind long
+// histories -- the steps (tiles of 128 keys) of all items form one list (request, head, item) that is cut into equal
+// ranges; what the ranges leave of a cut item is joined by a second launch, which is priced at six steps.
+// The estimates, in steps: whole items max(dearest, mean + dearest / rounds), ranges mean + 6.  (1500 tokens of 32 heads:
+// 15 and 15; 8192 of 28: 209 and 206, whole because a cut has to promise a tenth; 4 x 350 tokens behind 5000 of 32: 85
+// and 64, measured 121 and 87 us.)
+constexpr int kPrShortest = 12;      // steps of a range, where items have as many
+// Item i of a sequence: query rows 256 i ..; it takes ceil(keys that its last row sees / 128) steps.
+struct ItemSteps {
+  int items, lag, last;        // lag: ceil((nk - nq) / 128); last: steps of the last item
+  __device__ __forceinline__ explicit ItemSteps(const Sequence& s) {
+    items = (s.nq + kPrRows - 1) / kPrRows;
+    lag = (s.nk - s.nq + kPrTile - 1) >> 7;
+    last = (s.nk + kPrTile - 1) / kPrTile;
+  }
+  __device__ __forceinline__ int cost(int i) const { return i + 1 < items ? max(2 * (i + 1) + lag, 0) : items > 0 ? last : 0; }
+  __device__ __forceinline__ long long before(int i) const {
+    // the sum of 2 (j + 1) + lag over j = 0 .. i - 1, as far as positive, where item i exists
+    const long long first = min((long long)max(-lag >> 1, 0), (long long)i);
+    return (long long)i * (i - 1) - first * (first - 1) + (i - first) * (2 + lag);
+  }
+  __device__ __forceinline__ long long all() const { return items > 0 ? before(items - 1) + last : 0; }
+};
+__device__ __forceinline__ long long shuffle64(long long v, int lane) {
+  return (long long)__shfl_sync(0xffffffffu, (unsigned long long)v, lane);
+}
+// An item, or the part of it that a range holds.
+struct Segment {
+  int valid, q_base, nq, k_base, nk, head, q0, t_lo, n_t, part;      // part: 0 the whole item, 1 not its beginning, 2 its beginning
+};
+struct Deal {
+  long long total, items;      // steps and items of all heads
+  int dearest, ranges;         // ranges: 0 where items stay whole
+  // The whole warp takes part.
+  __device__ __forceinline__ Deal(const PromptParams& P, int ctas) {
+    total = items = 0;
+    dearest = 0;
+    for (int b = threadIdx.x & 31; b < P.n_seq; b += 32) {
+      const ItemSteps k(load_sequence(P, b));
+      total += k.all();
+      items += k.items;
+      if (k.items > 0) dearest = max(dearest, k.last);
+    }
+#pragma unroll
+    for (int d = 16; d; d >>= 1) {
+      total += (long long)__shfl_xor_sync(0xffffffffu, (unsigned long long)total, d);
+      items += (long long)__shfl_xor_sync(0xffffffffu, (unsigned long long)items, d);
+    }
+    dearest = __reduce_max_sync(0xffffffffu, dearest);
+    total *= P.q_heads;
+    items *= P.q_heads;
+    ranges = 0;
+    const int most = (int)min((long long)ctas, total / max(min(kPrShortest, dearest), 1));
+    if (most < 2 || !P.records) return;
+    // in whole numbers, so that the launches agree: times ctas x rounds, and a tenth less
+    const long long rounds = (items + ctas - 1) / ctas;
+    if (rounds > 64) return;
+    const long long whole = max(dearest * ctas * rounds, rounds > 1 ? total * rounds + (long long)dearest * ctas : 0);
+    if (10 * (total + 6LL * most) * ctas * rounds < 9 * most * whole) ranges = most;
+  }
+  __device__ __forceinline__ long long cut(int range) const { return (long long)((double)total / ranges * range); }
+  // A cut near the edge of an item moves there.
+  __device__ __forceinline__ int slack() const { return max((int)(total / ranges / 16), 1); }
+};
+// A place in the list of steps.
+struct ItemCursor {
+  int b, head, item, step, cost;      // step: inside the item
+  Sequence s;
+};
+// The place of step u, which exists; the whole warp takes part.
+__device__ __forceinline__ ItemCursor seek_item(const PromptParams& P, long long u) {
+  const int lane = threadIdx.x & 31;
+  ItemCursor c = {};
+  for (int b0 = 0; b0 < P.n_seq; b0 += 32) {
+    const Sequence s = b0 + lane < P.n_seq ? load_sequence(P, b0 + lane) : Sequence{0, 0, 0, 0};
+    const long long mine = ItemSteps(s).all() * P.q_heads;
+    long long sum = mine;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const long long other = (long long)__shfl_up_sync(0xffffffffu, (unsigned long long)sum, d);
+      if (lane >= d) sum += other;
+    }
+    const unsigned found = __ballot_sync(0xffffffffu, sum > u);
+    if (found) {
+      const int who = __ffs(found) - 1;
+      c.b = b0 + who;
+      c.s.q0 = __shfl_sync(0xffffffffu, s.q0, who);
+      c.s.nq = __shfl_sync(0xffffffffu, s.nq, who);
+      c.s.k0 = __shfl_sync(0xffffffffu, s.k0, who);
+      c.s.nk = __shfl_sync(0xffffffffu, s.nk, who);
+      u -= shuffle64(sum - mine, who);
+      break;
+    }
+    u -= shuffle64(sum, 31);
+  }
+  const ItemSteps k(c.s);
+  const long long per_head = k.all();
+  c.head = (int)(u / per_head);
+  u -= c.head * per_head;
+  int lo = 0, hi = k.items;      // before(lo) <= u, and u < before(hi) or hi is behind the last item
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (k.before(mid) <= u) lo = mid;
+    else hi = mid;
+  }
+  c.item = lo;
+  c.step = (int)(u - k.before(lo));
+  c.cost = k.cost(lo);
+  return c;
+}
+// The item behind, if there is one; items without a key, of which there is no step, are passed over.
+__device__ __forceinline__ void next_item(const PromptParams& P, ItemCursor& c) {
+  c.step = 0;
+  do {
+    if (++c.item >= ItemSteps(c.s).items) {
+      c.item = 0;
+      if (++c.head == P.q_heads) {
+        c.head = 0;
+        do {
+          if (++c.b >= P.n_seq) return;
+          c.s = load_sequence(P, c.b);
+        } while (ItemSteps(c.s).all() == 0);
+      }
+    }
+    c.cost = ItemSteps(c.s).cost(c.item);
+  } while (c.cost == 0);
+}
+// The first step of a range and its place; step `total` behind the last range.
+__device__ __forceinline__ ItemCursor range_begin(const PromptParams& P, const Deal& deal, int range, long long& step) {
+  step = deal.total;
+  if (range >= deal.ranges) return ItemCursor{};
+  step = deal.cut(range);
+  ItemCursor c = seek_item(P, step);
+  if (c.step <= deal.slack()) {
+    step -= c.step;
+    c.step = 0;
+  } else if (c.cost - c.step <= deal.slack()) {
+    step += c.cost - c.step;
+    next_item(P, c);
+  }
+  return c;
+}
+
+constexpr int kPrAhead = 4;                // segments described ahead
 template <int D>
 struct PromptShape {
   static constexpr int kSlabs = D / 64;                       // column slabs of an operand tile
   static constexpr int kTileBytes = kSlabs * kPrSlab;
   static constexpr int kStages = D == 128 ? 2 : 4;            // K and V tiles in flight
   static constexpr int kTiles = (2 + 2 * kStages) * kTileBytes;
-  static constexpr int kBars = 2 + 4 * kStages + 8;
-  // then: TMEM base, abort flag, two request counts, the item (8 words), a flag, barriers, three lists of D positions
-  static constexpr int kBarOffset = kTiles + 64, kListOffset = kBarOffset + 8 * kBars;
-  static constexpr int kSmem = kListOffset + 3 * D * 4;
+  static constexpr int kBars = 2 + 4 * kStages + 4 * kStages + 4 + 2 * kPrAhead;
+  // then: TMEM base, flags; segments; barriers; two sets of three lists of D positions
+  static constexpr int kSegmentOffset = kTiles + 64, kBarOffset = kSegmentOffset + kPrAhead * 64, kListOffset = kBarOffset + 8 * kBars;
+  static constexpr int kSmem = kListOffset + 2 * 3 * D * 4;
 };
+static_assert(sizeof(Segment) <= 64, "a segment's place");
 
 constexpr int kFar = 0x7fffffff;
 // positions of the first +infinity, -infinity and NaN of each channel among the cleaned values
 enum { kBadPlus = 0, kBadMinus = 1, kBadNan = 2 };
+
+// What the roles derive from a segment.
+struct SegmentTiles {
+  int hist, n_a, n_b, t_dark;
+  __device__ __forceinline__ explicit SegmentTiles(const Segment& g) {
+    hist = g.nk - g.nq;       // negative where the first queries have no key at all
+    // tiles that A and B walk; B may hold no query at all, and a tile no key
+    const int all_a = (max(min(g.nk, hist + g.q0 + kPrTile), 0) + kPrTile - 1) / kPrTile;
+    const int all_b = g.q0 + kPrTile < g.nq ? (max(min(g.nk, hist + g.q0 + kPrRows), 0) + kPrTile - 1) / kPrTile : 0;
+    n_a = max(0, min(all_a, g.t_lo + g.n_t) - g.t_lo);
+    n_b = max(0, min(all_b, g.t_lo + g.n_t) - g.t_lo);
+    // Tiles from t_dark on hold rows that some query of this item must not see.  Their values arrive at barriers of
+    // their own: the warp that cleans them looks at no earlier tile, and a parity alone does not tell phases apart.
+    t_dark = max(0, (max(hist + g.q0 + 1, 0) >> 7) - g.t_lo);
+  }
+};
 
 template <typename QT, int D>
 __global__ void __launch_bounds__(kPrThreads, 1) prompt_kernel(const PromptParams P, const __grid_constant__ CUtensorMap map_q,
@@ -148,227 +308,338 @@ __global__ void __launch_bounds__(kPrThreads, 1) prompt_kernel(const PromptParam
   const unsigned sQ = smem0, sKb = smem0 + 2 * kTileBytes, sVb = sKb + kStages * kTileBytes;
   unsigned* const tmem_base_p = (unsigned*)(pr_raw + S::kTiles);
   volatile int* const abort_flag = (volatile int*)(pr_raw + S::kTiles + 4);
-  volatile int* const requested = abort_flag + 1;             // K and V tiles that the TMA warp asked for in all
-  volatile int* const item_p = abort_flag + 3;                // found, index, q0, nq, k0, nk
-  volatile int* const any_bad = abort_flag + 10;
-  int* const first_bad = (int*)(pr_raw + S::kListOffset);     // [3][D]
+  int* const ended = (int*)(pr_raw + S::kTiles + 8);          // softmax warps that are done with a segment, over all segments
+  volatile int* const any_bad = (volatile int*)(pr_raw + S::kTiles + 16);      // of even and odd segments
+  int* const lists = (int*)(pr_raw + S::kListOffset);         // [2][3][D]
   const unsigned bars = smem0 + S::kBarOffset;
-  // per stage: K and V tiles, V tiles that want cleaning, such tiles cleaned
+  // Per stage: K and V tiles, V tiles that want cleaning, such tiles cleaned, S and O of tiles A and B; A and B: first half
+  // of P, P; segments.  Barriers of a stage, because a parity alone does not tell phases apart: a stage is not used
+  // again before everyone has seen its last phase.
   const unsigned bar_q = bars, bar_e = bars + 8, bar_k = bars + 16, bar_v = bar_k + 8 * kStages, bar_d = bar_v + 8 * kStages;
-  const unsigned bar_c = bar_d + 8 * kStages, bar_s = bar_c + 8 * kStages /* A, B */, bar_p = bar_s + 16 /* A, B */, bar_o = bar_p + 16, bar_h = bar_o + 16;
+  const unsigned bar_c = bar_d + 8 * kStages, bar_s = bar_c + 8 * kStages /* [x][stage] */, bar_o = bar_s + 16 * kStages /* [x][stage] */;
+  const unsigned bar_p = bar_o + 16 * kStages, bar_h = bar_p + 16;
+  const unsigned bar_g = bar_h + 16, bar_gfree = bar_g + 8 * kPrAhead;
   const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
   follow_stream();       // cu_q and cu_k may come from the launch before this one
   if (smem0 & 1023u) {
     if (tid == 0) atomicOr(P.status, INQ_STATUS_BAD_INDEX);
     return;
   }
-  const int unit = (int)(blockIdx.x / P.splits), seg = (int)(blockIdx.x % P.splits);
-  const int head = unit % P.q_heads;
   if (warp == 8) {
-    Sequence s;
-    int index = 0;
-    const int b = find_item(P, unit / P.q_heads, (P.k_rows + kPrTile - 1) / kPrTile, s, index);
-    if (lane == 0) {
-      item_p[0] = b;
-      item_p[1] = index;
-      item_p[2] = s.q0;
-      item_p[3] = s.nq;
-      item_p[4] = s.k0;
-      item_p[5] = s.nk;
-    }
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(tc_smem(tmem_base_p)), "r"(512) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   } else if (warp == 9 && lane == 0) {
-    *abort_flag = requested[0] = requested[1] = 0;
-    *any_bad = 0;
+    *abort_flag = *ended = any_bad[0] = any_bad[1] = 0;
     tc_bar_init(bar_q, 1);
     tc_bar_init(bar_e, 1);
 #pragma unroll
     for (int i = 0; i < kStages; ++i) {
+      tc_bar_init(bar_s + 8 * i, 1);
+      tc_bar_init(bar_s + 8 * (kStages + i), 1);
+      tc_bar_init(bar_o + 8 * i, 1);
+      tc_bar_init(bar_o + 8 * (kStages + i), 1);
       tc_bar_init(bar_k + 8 * i, 1);
       tc_bar_init(bar_v + 8 * i, 1);
       tc_bar_init(bar_d + 8 * i, 1);
-      tc_bar_init(bar_c + 8 * i, 2);
+      tc_bar_init(bar_c + 8 * i, 1);
     }
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      tc_bar_init(bar_s + 8 * i, 1);
       tc_bar_init(bar_p + 8 * i, kPrTile);
-      tc_bar_init(bar_o + 8 * i, 1);
       tc_bar_init(bar_h + 8 * i, kPrTile);
+    }
+#pragma unroll
+    for (int i = 0; i < kPrAhead; ++i) {
+      tc_bar_init(bar_g + 8 * i, 1);
+      tc_bar_init(bar_gfree + 8 * i, 11);       // the softmax warps, the MMA, TMA and cleaning warps
     }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  for (int i = tid; i < 3 * D; i += kPrThreads) first_bad[i] = kFar;
-  if (blockIdx.x == 0)
-    for (int b = tid; b < P.n_seq; b += kPrThreads)
-      if (bad_sequence(P, b)) atomicOr(P.status, INQ_STATUS_BAD_INDEX);
-  __syncthreads();
-  if (item_p[0] < 0) return;       // fewer items than the sizes of the tensors allow
-  if (warp == 8) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(tc_smem(tmem_base_p)), "r"(512) : "memory");
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
-  }
+  for (int i = tid; i < 2 * 3 * D; i += kPrThreads) lists[i] = kFar;
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const unsigned tmem = *tmem_base_p;      // S_A 0..127, S_B 128..255 (P over their first 64), O_A 256.., O_B 384..
   allow_next();
   auto wait = [&](unsigned mbar, unsigned parity) { tc_wait(mbar, parity, abort_flag); };   // goes on in either case
-
-  const int kvh = head / (P.q_heads / P.kv_heads);
-  const int q0 = item_p[1] * kPrRows, q_base = item_p[2], nq = item_p[3], k_base = item_p[4], nk = item_p[5];
-  const int hist = nk - nq;       // negative where the first queries have no key at all
-  // tiles that A and B walk; B may hold no query at all, and a tile no key
-  const int all_a = (max(min(nk, hist + q0 + kPrTile), 0) + kPrTile - 1) / kPrTile;
-  const int all_b = q0 + kPrTile < nq ? (max(min(nk, hist + q0 + kPrRows), 0) + kPrTile - 1) / kPrTile : 0;
-  const int all = max(all_a, all_b);
-  const int t_lo = (int)((long long)all * seg / P.splits), t_hi = (int)((long long)all * (seg + 1) / P.splits);
-  const int n_t = t_hi - t_lo;
-  const int n_a = max(0, min(all_a, t_hi) - t_lo), n_b = max(0, min(all_b, t_hi) - t_lo);
-  const int last = n_b > 0 ? 1 : 0;      // the tile that takes part in every step
-  // Tiles from t_dark on hold rows that some query of this item must not see.  Their values arrive at barriers of
-  // their own: the warps that clean them look at no earlier tile, and a parity alone does not tell phases apart.
-  const int t_dark = max(0, (max(hist + q0 + 1, 0) >> 7) - t_lo);
+  // Segment n, the same for a whole warp; an invalid one behind the last, and once a wait has given up.
+  auto segment = [&](int n) {
+    const bool there = tc_wait(bar_g + 8 * (n % kPrAhead), (unsigned)(n / kPrAhead) & 1u, abort_flag);
+    Segment g = *(const Segment*)(pr_raw + S::kSegmentOffset + 64 * (n % kPrAhead));
+    if (__any_sync(0xffffffffu, !there || *abort_flag != 0)) g.valid = 0;
+    __syncwarp();
+    if (lane == 0) pf_arrive(bar_gfree + 8 * (n % kPrAhead));
+    return g;
+  };
 
   if (warp >= 8) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kPrIssueRegs));
-    if (warp == 9) {
+    if (warp == 11) {
+      // ================================================================ deals the segments
+      int n = 0;
+      auto publish = [&](const Segment& g) {
+        if (n >= kPrAhead) wait(bar_gfree + 8 * (n % kPrAhead), (unsigned)(n / kPrAhead - 1) & 1u);
+        __syncwarp();
+        if (lane == 0) {
+          *(Segment*)(pr_raw + S::kSegmentOffset + 64 * (n % kPrAhead)) = g;
+          pf_arrive(bar_g + 8 * (n % kPrAhead));
+        }
+        ++n;
+      };
+      // the n-th whole item of this CTA; false where there are no more
+      auto whole = [&](long long round) {
+        const int ctas = gridDim.x;
+        const long long unit = round * ctas + ((round & 1) ? ctas - 1 - (int)blockIdx.x : (int)blockIdx.x), rank = unit / P.q_heads;
+        Sequence s;
+        int index = 0;
+        if (rank > 0x3fffffff || find_item(P, (int)rank, (P.k_rows + kPrTile - 1) / kPrTile, s, index) < 0) return false;
+        const int cost = ItemSteps(s).cost(index);
+        if (cost > 0) publish(Segment{1, s.q0, s.nq, s.k0, s.nk, (int)(unit - rank * P.q_heads), index * kPrRows, 0, cost, 0});
+        return true;
+      };
+      long long round = 0;
+      bool more = true, cut = false;
+      if (!P.records) {      // nothing is cut: the first item starts before anything else is looked at
+        more = whole(round++);
+      } else {
+        const Deal deal(P, gridDim.x);
+        cut = deal.ranges > 0;
+        if (cut && (int)blockIdx.x < deal.ranges) {
+          long long step, end;
+          range_begin(P, deal, blockIdx.x + 1, end);
+          ItemCursor c = range_begin(P, deal, blockIdx.x, step);
+          while (step < end && !__any_sync(0xffffffffu, *abort_flag != 0)) {
+            const int steps = (int)min(end - step, (long long)(c.cost - c.step));
+            publish(Segment{1, c.s.q0, c.s.nq, c.s.k0, c.s.nk, c.head, c.item * kPrRows, c.step, steps, steps == c.cost ? 0 : c.step ? 1 : 2});
+            step += steps;
+            if (step < end) next_item(P, c);
+          }
+        }
+      }
+      // offsets that the tensors do not hold, and queries without a key
+      for (int b = blockIdx.x; b < P.n_seq; b += gridDim.x) {
+        if (lane == 0 && bad_sequence(P, b)) atomicOr(P.status, INQ_STATUS_BAD_INDEX);
+        const Sequence s = load_sequence(P, b);
+        for (long long i = lane; i < (long long)(s.nq - s.nk) * P.q_heads; i += 32) {
+          const int row = s.q0 + (int)(i / P.q_heads), head = (int)(i % P.q_heads);
+          for (int c = 0; c < D; c += 8) *(uint4*)((QT*)P.out + head * P.o_sh + row * P.o_st + c) = make_uint4(0u, 0u, 0u, 0u);
+          if (P.lse) P.lse[head * P.lse_stride + row] = __int_as_float(0xff800000);
+        }
+      }
+      while (!cut && more && !__any_sync(0xffffffffu, *abort_flag != 0)) more = whole(round++);
+      publish(Segment{});
+    } else if (warp == 9) {
       // ================================================================ TMA warp
-      if (lane == 0 && n_t > 0) {
-        auto request = [&](int what, int t) {
-          requested[what] = t + 1;
-          const unsigned bar = (what == 0 ? bar_k : t < t_dark ? bar_v : bar_d) + 8 * (t % kStages), dst = (what ? sVb : sKb) + (t % kStages) * kTileBytes;
-          pf_expect(bar, kTileBytes);
+      // Step u of the CTA uses stage u % kStages.  Bits of a stage: the next parity of its plain and dark value barriers and of
+      // its barriers of tiles A and B, and whether the step that has it ends with tile B.
+      unsigned u = 0, v_parity = 0, d_parity = 0, a_parity = 0, b_parity = 0, ends_b = 0, queries = 0;
+      // the last contraction of kind `bar` of the step that had a stage before
+      auto stage_done = [&](unsigned bar, unsigned bit, unsigned st) {
+        const bool b = (ends_b & bit) != 0;
+        return tc_wait(bar + 8 * (b ? kStages + st : st), (b ? b_parity : a_parity) & bit ? 0u : 1u, abort_flag);
+      };
+      int n = 0;
+      for (Segment g = segment(0); g.valid; g = segment(++n)) {
+        const SegmentTiles T(g);
+        const int kvh = g.head / (P.q_heads / P.kv_heads);
+        if (lane == 0) {
+          for (int t = 0; t < g.n_t; ++t, ++u) {
+            const unsigned st = u % kStages, bit = 1u << st;
+            if (u >= kStages && !stage_done(bar_s, bit, st)) break;
+            const int y = g.k_base + (g.t_lo + t) * kPrTile;
+            pf_expect(bar_k + 8 * st, kTileBytes);
 #pragma unroll
-          for (int c = 0; c < S::kSlabs; ++c)
-            pf_tma(dst + c * kPrSlab, what ? &map_v : &map_k, 64 * c, k_base + (t_lo + t) * kPrTile, kvh, bar);
-        };
-        pf_expect(bar_q, 2 * kTileBytes);
+            for (int c = 0; c < S::kSlabs; ++c) pf_tma(sKb + st * kTileBytes + c * kPrSlab, &map_k, 64 * c, y, kvh, bar_k + 8 * st);
+            if (t == 0) {
+              // the query tiles are free once the last score contraction of the segment before is done
+              const unsigned before = (u + kStages - 1) % kStages;
+              if (u > 0 && !stage_done(bar_s, 1u << before, before)) {
+                ++u;      // its K tile is on the way
+                break;
+              }
+              ++queries;
+              pf_expect(bar_q, 2 * kTileBytes);
 #pragma unroll
-        for (int x = 0; x < 2; ++x)
+              for (int x = 0; x < 2; ++x)
 #pragma unroll
-          for (int c = 0; c < S::kSlabs; ++c)
-            pf_tma(sQ + x * kTileBytes + c * kPrSlab, &map_q, 64 * c, q_base + q0 + x * kPrTile, head, bar_q);
-        for (int t = 0; t < kStages && t < n_t; ++t) {
-          request(0, t);
-          request(1, t);
+                for (int c = 0; c < S::kSlabs; ++c)
+                  pf_tma(sQ + x * kTileBytes + c * kPrSlab, &map_q, 64 * c, g.q_base + g.q0 + x * kPrTile, g.head, bar_q);
+            }
+            if (u >= kStages && !stage_done(bar_o, bit, st)) {
+              ++u;
+              break;
+            }
+            if (t < T.n_a) a_parity ^= bit;
+            if (t < T.n_b) b_parity ^= bit;
+            ends_b = t < T.n_b ? ends_b | bit : ends_b & ~bit;
+            const unsigned bar = (t < T.t_dark ? bar_v : bar_d) + 8 * st;
+            pf_expect(bar, kTileBytes);
+#pragma unroll
+            for (int c = 0; c < S::kSlabs; ++c) pf_tma(sVb + st * kTileBytes + c * kPrSlab, &map_v, 64 * c, y, kvh, bar);
+            if (t < T.t_dark) v_parity ^= bit;
+            else d_parity ^= bit;
+          }
         }
-        for (int t = 0; t + kStages < n_t; ++t) {
-          // K(t) is free once the last score contraction of step t is done, V(t) once the last output contraction is
-          if (!tc_wait(bar_s + 8 * last, (unsigned)t & 1u, abort_flag)) break;
-          request(0, t + kStages);
-          if (!tc_wait(bar_o + 8 * last, (unsigned)t & 1u, abort_flag)) break;
-          request(1, t + kStages);
+        __syncwarp();
+      }
+      if (lane == 0 && *abort_flag) {
+        // copies in flight end before the CTA leaves: the last of each barrier that was used (a parity bit is that of the next)
+        for (unsigned i = 0; i < kStages; ++i) {
+          const unsigned bit = 1u << i, used = (u + kStages - 1 - i) / kStages;      // K tiles of this stage
+          if (used) tc_drain(bar_k + 8 * i, (used - 1) & 1u);
+          tc_drain(bar_v + 8 * i, v_parity & bit ? 0u : 1u);
+          tc_drain(bar_d + 8 * i, d_parity & bit ? 0u : 1u);
         }
+        if (queries) tc_drain(bar_q, (queries - 1) & 1u);
       }
     } else if (warp == 8) {
       // ================================================================ MMA warp
-      if (n_t > 0) {
-        constexpr bool kBf16 = !std::is_same<QT, __half>::value;
-        constexpr unsigned idesc_s = tc_idesc<kBf16, 128, 128, false>(), idesc_o = tc_idesc<kBf16, 128, D, true>();
-        auto issue_s = [&](int x, int t) {      // S_x = Q_x K(t)^T
-          const unsigned q = sQ + x * kTileBytes, k = sKb + (t % kStages) * kTileBytes;
-          if (tc_elect()) {
+      constexpr bool kBf16 = !std::is_same<QT, __half>::value;
+      constexpr unsigned idesc_s = tc_idesc<kBf16, 128, 128, false>(), idesc_o = tc_idesc<kBf16, 128, D, true>();
+      auto issue_s = [&](int x, unsigned u) {      // S_x = Q_x K^T
+        const unsigned q = sQ + x * kTileBytes, k = sKb + (u % kStages) * kTileBytes;
+        if (tc_elect()) {
 #pragma unroll
-            for (int kk = 0; kk < D / 16; ++kk) {
-              const unsigned off = (kk >> 2) * kPrSlab + (kk & 3) * 32;
-              tc_mma(tmem + x * kPrTile, tc_desc(q + off, 16, 1024), tc_desc(k + off, 16, 1024), idesc_s, kk > 0);
-            }
-            tc_commit(bar_s + 8 * x);
+          for (int kk = 0; kk < D / 16; ++kk) {
+            const unsigned off = (kk >> 2) * kPrSlab + (kk & 3) * 32;
+            tc_mma(tmem + x * kPrTile, tc_desc(q + off, 16, 1024), tc_desc(k + off, 16, 1024), idesc_s, kk > 0);
           }
-        };
-        auto issue_o = [&](int x, int t, int half) {      // O_x += P_x V(t), half a tile of tokens at a time
-          const unsigned v = sVb + (t % kStages) * kTileBytes;
-          if (tc_elect()) {
+          tc_commit(bar_s + 8 * (x * kStages + u % kStages));
+        }
+      };
+      auto issue_o = [&](int x, unsigned u, bool first, int half) {      // O_x += P_x V, half a tile of tokens at a time
+        const unsigned v = sVb + (u % kStages) * kTileBytes;
+        if (tc_elect()) {
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
-              const int kk = 4 * half + k;
-              tc_mma_ta(tmem + 2 * kPrTile + x * kPrTile, tmem + x * kPrTile + kk * 8, tc_desc(v + kk * 2048, kPrSlab, 1024), idesc_o,
-                        (t > 0 || kk > 0) ? 1u : 0u);
-            }
-            if (half) tc_commit(bar_o + 8 * x);
+          for (int k = 0; k < 4; ++k) {
+            const int kk = 4 * half + k;
+            tc_mma_ta(tmem + 2 * kPrTile + x * kPrTile, tmem + x * kPrTile + kk * 8, tc_desc(v + kk * 2048, kPrSlab, 1024), idesc_o,
+                      (!first || kk > 0) ? 1u : 0u);
           }
-        };
-        auto contract_o = [&](int x, int t) {
-          wait(bar_h + 8 * x, (unsigned)t & 1u);     // S_x(t) read, the first half of P_x(t) written
-          tc_fence_after();
-          issue_o(x, t, 0);
-          wait(bar_p + 8 * x, (unsigned)t & 1u);     // the second half
-          tc_fence_after();
-          issue_o(x, t, 1);
-        };
+          if (half) tc_commit(bar_o + 8 * (x * kStages + u % kStages));
+        }
+      };
+      unsigned count[2] = {0, 0}, v_parity = 0, d_parity = 0, u = 0;
+      auto contract_o = [&](int x, bool first) {
+        wait(bar_h + 8 * x, count[x] & 1u);     // S_x read, the first half of P_x written, the rows of the segment before stored
+        tc_fence_after();
+        issue_o(x, u, first, 0);
+        wait(bar_p + 8 * x, count[x] & 1u);     // the second half
+        tc_fence_after();
+        issue_o(x, u, first, 1);
+        ++count[x];
+      };
+      int n = 0;
+      Segment g = segment(0);
+      if (g.valid) {
+        SegmentTiles T(g), next = T;
         wait(bar_q, 0);
         wait(bar_k, 0);
         tc_fence_after();
-        if (n_a > 0) issue_s(0, 0);
-        if (n_b > 0) issue_s(1, 0);
-        for (int t = 0; t < n_t; ++t) {
-          if (t < t_dark) wait(bar_v + 8 * (t % kStages), (unsigned)(t / kStages) & 1u);
-          else wait(bar_c + 8 * (t % kStages), (unsigned)((t - t_dark) / kStages) & 1u);
-          if (t < n_a) contract_o(0, t);
-          if (t + 1 < n_t) {
-            wait(bar_k + 8 * ((t + 1) % kStages), (unsigned)((t + 1) / kStages) & 1u);
-            if (t + 1 < n_a) issue_s(0, t + 1);
+        if (T.n_a > 0) issue_s(0, 0);
+        if (T.n_b > 0) issue_s(1, 0);
+        int t = 0;
+        while (true) {
+          const unsigned st = u % kStages, bit = 1u << st;
+          if (t < T.t_dark) {
+            wait(bar_v + 8 * st, v_parity & bit ? 1u : 0u);
+            v_parity ^= bit;
+          } else {
+            wait(bar_c + 8 * st, d_parity & bit ? 1u : 0u);
+            d_parity ^= bit;
           }
-          if (t < n_b) contract_o(1, t);
-          if (t + 1 < n_b) issue_s(1, t + 1);
+          const bool b_now = t < T.n_b, b_first = t == 0;
+          if (t < T.n_a) contract_o(0, t == 0);
+          // the step behind this one, perhaps of another segment
+          bool more = true;
+          if (++t == g.n_t) {
+            t = 0;
+            g = segment(++n);
+            more = g.valid;
+          }
+          if (t == 0) next = SegmentTiles(g);
+          if (more) {
+            if (t == 0) wait(bar_q, (unsigned)n & 1u);
+            wait(bar_k + 8 * ((u + 1) % kStages), ((u + 1) / kStages) & 1u);
+            tc_fence_after();
+            if (t < next.n_a) issue_s(0, u + 1);
+          }
+          if (b_now) contract_o(1, b_first);
+          if (!more) break;
+          if (t < next.n_b) issue_s(1, u + 1);
+          if (t == 0) T = next;
+          ++u;
         }
       }
     } else {
-      // ================================================================ two warps that clean value tiles
-      // a lane owns two chunks of 16 bytes per slab and row group; chunk c of row r lies at chunk c ^ (r & 7)
-      for (int t = t_dark; t < n_t; ++t) {
-        wait(bar_d + 8 * (t % kStages), (unsigned)((t - t_dark) / kStages) & 1u);
-        unsigned char* const tile = pr_raw + (sVb - smem0) + (t % kStages) * kTileBytes;
-        const int kv0 = (t_lo + t) * kPrTile, rows = min(nk - kv0, kPrTile);     // rows of the sequence
-        const int first = (warp - 10) * 32 + lane;
-        bool touched = false;
+      // ================================================================ the warp that cleans value tiles
+      // chunk c of row r lies at chunk c ^ (r & 7) of its slab
+      unsigned u = 0, d_parity = 0, held = 0;      // held: sets of lists with something in them
+      int n = 0;
+      for (Segment g = segment(0); g.valid; g = segment(++n)) {
+        const SegmentTiles T(g);
+        int* const first_bad = lists + (n & 1) * 3 * D;
+        // The lists were those of the segment before the last: nothing changes there before all softmax warps have ended that.
+        auto others_ended = [&]() {
+          for (int it = 0; it < kTcTries && *(volatile int*)ended < 8 * (n - 1) && *abort_flag == 0; ++it) __nanosleep(64);
+        };
+        if (T.t_dark < g.n_t && (held >> (n & 1)) & 1u) {
+          others_ended();
+          __syncwarp();
+          for (int i = lane; i < 3 * D; i += 32) first_bad[i] = kFar;
+          any_bad[n & 1] = 0;
+          held &= ~(1u << (n & 1));
+          __syncwarp();
+        }
+        for (int t = T.t_dark; t < g.n_t; ++t) {
+          const unsigned st = (u + t) % kStages, bit = 1u << st;
+          wait(bar_d + 8 * st, d_parity & bit ? 1u : 0u);
+          d_parity ^= bit;
+          unsigned char* const tile = pr_raw + (sVb - smem0) + st * kTileBytes;
+          const int kv0 = (g.t_lo + t) * kPrTile, rows = min(g.nk - kv0, kPrTile);     // rows of the sequence
+          // a first look finds the largest magnitude of every batch, as whole numbers: the second is for what is not finite
+          constexpr unsigned kOnes = std::is_same<QT, __half>::value ? 0x7c00u : 0x7f80u;
+          bool touched = false;
 #pragma unroll 1
-        for (int i0 = first; i0 < kTileBytes / 16; i0 += 64 * 8) {
-          uint4 w[8];
+          for (int i0 = lane; i0 < kTileBytes / 16; i0 += 32 * 8) {
+            uint4 w[8];
 #pragma unroll
-          for (int j = 0; j < 8; ++j) w[j] = *(const uint4*)(tile + 16 * (i0 + 64 * j));
+            for (int j = 0; j < 8; ++j) w[j] = *(const uint4*)(tile + 16 * (i0 + 32 * j));
+            unsigned most = 0;
 #pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            const int i = i0 + 64 * j, row = (i >> 3) & (kPrTile - 1);
-            if (row >= rows) {
-              *(uint4*)(tile + 16 * i) = make_uint4(0u, 0u, 0u, 0u);
-              touched = true;
-              continue;
-            }
-            // all ones in the exponent of either half of a word: the mask of the type, compared half by half
-            constexpr unsigned kOnes = std::is_same<QT, __half>::value ? 0x7c007c00u : 0x7f807f80u;
-            const unsigned words[4] = {w[j].x, w[j].y, w[j].z, w[j].w};
-            bool bad = false;
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-              const unsigned e = ~words[k] & kOnes;
-              bad |= (e & 0xffffu) == 0u || (e >> 16) == 0u;
-            }
-            if (bad) {
-              const int channel = (i / (kPrTile * 8)) * 64 + (((i & 7) ^ (row & 7)) << 3);
-              unsigned clean[4];
-#pragma unroll
-              for (int k = 0; k < 4; ++k) {
-                clean[k] = words[k];
-#pragma unroll
-                for (int half = 0; half < 2; ++half) {
-                  const unsigned bits = (words[k] >> (16 * half)) & 0xffffu;
-                  if ((~bits & (kOnes & 0xffffu)) == 0u) {
-                    const int kind = (bits & ~kOnes & 0x7fffu) ? kBadNan : (bits & 0x8000u) ? kBadMinus : kBadPlus;
-                    atomicMin(first_bad + kind * D + channel + 2 * k + half, kv0 + row);
-                    clean[k] &= ~(0xffffu << (16 * half));
-                  }
-                }
+            for (int j = 0; j < 8; ++j) {
+              const int row = ((i0 + 32 * j) >> 3) & (kPrTile - 1);
+              if (row >= rows) {
+                *(uint4*)(tile + 16 * (i0 + 32 * j)) = make_uint4(0u, 0u, 0u, 0u);
+                touched = true;
+              } else {
+                most = __vmaxu2(__vmaxu2(__vmaxu2(most, w[j].x & 0x7fff7fffu), w[j].y & 0x7fff7fffu), __vmaxu2(w[j].z & 0x7fff7fffu, w[j].w & 0x7fff7fffu));
               }
-              *(uint4*)(tile + 16 * i) = make_uint4(clean[0], clean[1], clean[2], clean[3]);
-              *any_bad = 1;
-              touched = true;
+            }
+            if ((most & 0xffffu) < kOnes && (most >> 16) < kOnes) continue;
+            others_ended();
+#pragma unroll 1
+            for (int j = 0; j < 8; ++j) {
+              const int i = i0 + 32 * j, row = (i >> 3) & (kPrTile - 1), channel = (i / (kPrTile * 8)) * 64 + (((i & 7) ^ (row & 7)) << 3);
+              unsigned short* const values = (unsigned short*)(tile + 16 * i);
+#pragma unroll 1
+              for (int k = 0; k < 8 && row < rows; ++k) {
+                const unsigned bits = values[k];
+                if ((bits & 0x7fffu) < kOnes) continue;
+                const int kind = (bits & 0x7fffu) > kOnes ? kBadNan : (bits & 0x8000u) ? kBadMinus : kBadPlus;
+                atomicMin(first_bad + kind * D + channel + k, kv0 + row);
+                values[k] = 0;
+                any_bad[n & 1] = 1;
+                touched = true;
+              }
             }
           }
+          if (touched) asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+          __syncwarp();
+          if (any_bad[n & 1]) held |= 1u << (n & 1);
+          if (lane == 0) pf_arrive(bar_c + 8 * st);
         }
-        if (touched) asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-        __syncwarp();
-        if (lane == 0) pf_arrive(bar_c + 8 * (t % kStages));
+        u += g.n_t;
       }
     }
   } else {
@@ -376,149 +647,164 @@ __global__ void __launch_bounds__(kPrThreads, 1) prompt_kernel(const PromptParam
     // ================================================================ softmax warps
     const int x = warp >> 2;                       // 0: tile A, 1: tile B
     const int row = tid & (kPrTile - 1);           // query row inside the tile = TMEM lane
-    const int n_x = x ? n_b : n_a;
-    const int q_row = q0 + x * kPrTile + row;
-    const int q_pos = hist + q_row;                // keys at positions <= q_pos are visible
-    const int diag0 = hist + q0 + x * kPrTile;     // first row's diagonal: tiles reaching beyond it need masks
     const unsigned lane_field = (unsigned)((warp & 3) * 32) << 16;
     const unsigned tS = tmem + lane_field + x * kPrTile, tO = tmem + lane_field + 2 * kPrTile + x * kPrTile;
-    const unsigned my_s = bar_s + 8 * x, my_p = bar_p + 8 * x, my_o = bar_o + 8 * x;
-    float m_ref = kPrNegBig, l_sum = 0.f;
+    const unsigned my_s = bar_s + 8 * x * kStages, my_p = bar_p + 8 * x, my_o = bar_o + 8 * x * kStages;
+    unsigned u = 0, parity = 0;                    // the segment's first step; a bit per stage: the next parity of this tile's barriers
+    int n = 0;
+    for (Segment g = segment(0); g.valid; g = segment(++n)) {
+      const SegmentTiles T(g);
+      const int n_x = x ? T.n_b : T.n_a;
+      const int q_row = g.q0 + x * kPrTile + row;
+      const int q_pos = T.hist + q_row;              // keys at positions <= q_pos are visible
+      const int diag0 = T.hist + g.q0 + x * kPrTile;     // first row's diagonal: tiles reaching beyond it need masks
+      float m_ref = kPrNegBig, l_sum = 0.f;
 
-    for (int t = 0; t < n_x; ++t) {
-      const int kv0 = (t_lo + t) * kPrTile;
-      // S(t) is complete; the contractions run in issue order, so PV(t-1) is complete as well:
-      // the columns of P may be overwritten by S and O may be rescaled
-      wait(my_s, (unsigned)t & 1u);
+      for (int t = 0; t < n_x; ++t) {
+        const int kv0 = (g.t_lo + t) * kPrTile;
+        // S(t) is complete; the contractions run in issue order, so PV(t-1) is complete as well:
+        // the columns of P may be overwritten by S and O may be rescaled
+        const unsigned st = (u + t) % kStages, bit = 1u << st;
+        wait(my_s + 8 * st, parity & bit ? 1u : 0u);
+        parity ^= bit;
+        tc_fence_after();
+        unsigned v[4][32];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) tc_ld32(tS + 32 * q, v[q]);
+#pragma unroll
+        for (int q = 0; q < 4; ++q) tc_wait_ld32(v[q]);
+        if (kv0 + kPrTile - 1 > diag0) {
+#pragma unroll
+          for (int q = 0; q < 4; ++q)
+#pragma unroll
+            for (int c = 0; c < 32; ++c)
+              if (kv0 + 32 * q + c > q_pos) v[q][c] = 0xff800000u;
+        }
+        float top[4];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          top[q] = __uint_as_float(v[q][0]);
+#pragma unroll
+          for (int c = 1; c < 32; ++c) top[q] = fmaxf(top[q], __uint_as_float(v[q][c]));
+        }
+        const float smax = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+        const bool raise = smax * P.scale_log2e > m_ref + kPrSlack;
+        if (__any_sync(0xffffffffu, raise)) {
+          // rare after the first tile: bring the running sum and the output accumulator to the new reference maximum
+          const float m_new = raise ? smax * P.scale_log2e : m_ref;
+          const float factor = pf_exp2(m_ref - m_new);
+          l_sum *= factor;
+          m_ref = m_new;
+          if (t > 0) {
+#pragma unroll 1
+            for (int c0 = 0; c0 < D; c0 += 16) {
+              unsigned o[16];
+              tc_ld16(tO + c0, o);
+              tc_wait_ld16(o);
+#pragma unroll
+              for (int c = 0; c < 16; ++c) o[c] = __float_as_uint(__uint_as_float(o[c]) * factor);
+              tc_st16(tO + c0, o);
+            }
+          }
+        }
+        const unsigned long long scale2 = pf_pair(P.scale_log2e, P.scale_log2e), minus_ref2 = pf_pair(-m_ref, -m_ref);
+        unsigned long long sum2 = pf_pair(0.f, 0.f);
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          unsigned packed[16];
+#pragma unroll
+          for (int c = 0; c < 32; c += 2) {
+            float e0, e1;
+            pf_unpair(pf_fma2(pf_pair(__uint_as_float(v[q][c]), __uint_as_float(v[q][c + 1])), scale2, minus_ref2), e0, e1);
+            e0 = pf_exp2(e0);
+            e1 = pf_exp2(e1);
+            sum2 = pf_add2(sum2, pf_pair(e0, e1));
+            packed[c >> 1] = pf_pack2<QT>(e0, e1);
+          }
+          tc_st16(tS + 16 * q, packed);
+          if (q == 1) {   // S has been read, the first half of P is in tensor memory: the contraction with V starts
+            tc_wait_st();
+            tc_fence_before();
+            pf_arrive(bar_h + 8 * x);
+          }
+        }
+        float sum_even, sum_odd;
+        pf_unpair(sum2, sum_even, sum_odd);
+        l_sum += sum_even + sum_odd;
+        tc_wait_st();
+        tc_fence_before();
+        pf_arrive(my_p);
+      }
+      if (n_x > 0) {
+        const unsigned st = (u + n_x - 1) % kStages;
+        wait(my_o + 8 * st, (parity >> st) & 1u ? 0u : 1u);
+      }
+      u += g.n_t;
       tc_fence_after();
-      unsigned v[4][32];
-#pragma unroll
-      for (int q = 0; q < 4; ++q) tc_ld32(tS + 32 * q, v[q]);
-#pragma unroll
-      for (int q = 0; q < 4; ++q) tc_wait_ld32(v[q]);
-      if (kv0 + kPrTile - 1 > diag0) {
-#pragma unroll
-        for (int q = 0; q < 4; ++q)
-#pragma unroll
-          for (int c = 0; c < 32; ++c)
-            if (kv0 + 32 * q + c > q_pos) v[q][c] = 0xff800000u;
-      }
-      float top[4];
-#pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        top[q] = __uint_as_float(v[q][0]);
-#pragma unroll
-        for (int c = 1; c < 32; ++c) top[q] = fmaxf(top[q], __uint_as_float(v[q][c]));
-      }
-      const float smax = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
-      const bool raise = smax * P.scale_log2e > m_ref + kPrSlack;
-      if (__any_sync(0xffffffffu, raise)) {
-        // rare after the first tile: bring the running sum and the output accumulator to the new reference maximum
-        const float m_new = raise ? smax * P.scale_log2e : m_ref;
-        const float factor = pf_exp2(m_ref - m_new);
-        l_sum *= factor;
-        m_ref = m_new;
-        if (t > 0) {
-#pragma unroll 1
-          for (int c0 = 0; c0 < D; c0 += 16) {
-            unsigned o[16];
-            tc_ld16(tO + c0, o);
-            tc_wait_ld16(o);
-#pragma unroll
-            for (int c = 0; c < 16; ++c) o[c] = __float_as_uint(__uint_as_float(o[c]) * factor);
-            tc_st16(tO + c0, o);
-          }
-        }
-      }
-      const unsigned long long scale2 = pf_pair(P.scale_log2e, P.scale_log2e), minus_ref2 = pf_pair(-m_ref, -m_ref);
-      unsigned long long sum2 = pf_pair(0.f, 0.f);
-#pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        unsigned packed[16];
-#pragma unroll
-        for (int c = 0; c < 32; c += 2) {
-          float e0, e1;
-          pf_unpair(pf_fma2(pf_pair(__uint_as_float(v[q][c]), __uint_as_float(v[q][c + 1])), scale2, minus_ref2), e0, e1);
-          e0 = pf_exp2(e0);
-          e1 = pf_exp2(e1);
-          sum2 = pf_add2(sum2, pf_pair(e0, e1));
-          packed[c >> 1] = pf_pack2<QT>(e0, e1);
-        }
-        tc_st16(tS + 16 * q, packed);
-        if (q == 1) {   // S has been read, the first half of P is in tensor memory: the contraction with V starts
-          tc_wait_st();
-          tc_fence_before();
-          pf_arrive(bar_h + 8 * x);
-        }
-      }
-      float sum_even, sum_odd;
-      pf_unpair(sum2, sum_even, sum_odd);
-      l_sum += sum_even + sum_odd;
-      tc_wait_st();
-      tc_fence_before();
-      pf_arrive(my_p);
-    }
-    if (n_x > 0) wait(my_o, (unsigned)(n_x - 1) & 1u);
-    tc_fence_after();
-    const bool ok = *abort_flag == 0;
-    const bool live = ok && q_row < nq;
-    const bool bad = *any_bad != 0;     // complete: the last contraction came after the last cleaned tile
-    // What cleaning took out, for the rows that see it: the sum of a NaN or of infinities of both signs is NaN.
-    auto put_back = [&](float o, int channel) {
-      const bool plus = first_bad[kBadPlus * D + channel] <= q_pos, minus = first_bad[kBadMinus * D + channel] <= q_pos;
-      if (first_bad[kBadNan * D + channel] <= q_pos || (plus && minus)) return __int_as_float(0x7fc00000);
-      return plus ? o + __int_as_float(0x7f800000) : minus ? o + __int_as_float(0xff800000) : o;
-    };
+      const bool live = *abort_flag == 0 && q_row < g.nq;
+      // complete: the last contraction came after the last cleaned tile
+      const int* const first_bad = lists + (n & 1) * 3 * D;
+      const bool bad = T.t_dark < g.n_t && any_bad[n & 1] != 0;
+      // What cleaning took out, for the rows that see it: the sum of a NaN or of infinities of both signs is NaN.
+      auto put_back = [&](float o, int channel) {
+        const bool plus = first_bad[kBadPlus * D + channel] <= q_pos, minus = first_bad[kBadMinus * D + channel] <= q_pos;
+        if (first_bad[kBadNan * D + channel] <= q_pos || (plus && minus)) return __int_as_float(0x7fc00000);
+        return plus ? o + __int_as_float(0x7f800000) : minus ? o + __int_as_float(0xff800000) : o;
+      };
 
-    if (P.splits == 1) {
-      // a row without keys gives zeros; one whose logits are all -infinity divides zero by zero, as its formula does
-      const float inv = q_pos < 0 ? 0.f : 1.f / l_sum;
-      if (live && P.lse) P.lse[head * P.lse_stride + q_base + q_row] = q_pos < 0 ? __int_as_float(0xff800000) : (m_ref + log2f(l_sum)) * kLn2;
-      QT* orow = (QT*)P.out + (long long)head * P.o_sh + (long long)(q_base + q_row) * P.o_st;
+      if (g.part == 0) {
+        // a row without keys gives zeros; one whose logits are all -infinity divides zero by zero, as its formula does
+        const float inv = q_pos < 0 ? 0.f : 1.f / l_sum;
+        if (live && P.lse) P.lse[g.head * P.lse_stride + g.q_base + q_row] = q_pos < 0 ? __int_as_float(0xff800000) : (m_ref + log2f(l_sum)) * kLn2;
+        QT* orow = (QT*)P.out + (long long)g.head * P.o_sh + (long long)(g.q_base + q_row) * P.o_st;
 #pragma unroll 1
-      for (int c0 = 0; c0 < D; c0 += 32) {
-        unsigned v[32];
+        for (int c0 = 0; c0 < D; c0 += 32) {
+          unsigned v[32];
 #pragma unroll
-        for (int c = 0; c < 32; ++c) v[c] = 0u;
-        if (n_x > 0) {
-          tc_ld32(tO + c0, v);
-          tc_wait_ld32(v);
-        }
-        if (bad)
+          for (int c = 0; c < 32; ++c) v[c] = 0u;
+          if (n_x > 0) {
+            tc_ld32(tO + c0, v);
+            tc_wait_ld32(v);
+          }
+          if (bad)
 #pragma unroll
-          for (int c = 0; c < 32; ++c) v[c] = __float_as_uint(put_back(__uint_as_float(v[c]), c0 + c));
-        if (live) {
+            for (int c = 0; c < 32; ++c) v[c] = __float_as_uint(put_back(__uint_as_float(v[c]), c0 + c));
+          if (live) {
 #pragma unroll
-          for (int q4 = 0; q4 < 4; ++q4) {
-            uint4 w;
-            w.x = pf_pack2<QT>(__uint_as_float(v[8 * q4 + 0]) * inv, __uint_as_float(v[8 * q4 + 1]) * inv);
-            w.y = pf_pack2<QT>(__uint_as_float(v[8 * q4 + 2]) * inv, __uint_as_float(v[8 * q4 + 3]) * inv);
-            w.z = pf_pack2<QT>(__uint_as_float(v[8 * q4 + 4]) * inv, __uint_as_float(v[8 * q4 + 5]) * inv);
-            w.w = pf_pack2<QT>(__uint_as_float(v[8 * q4 + 6]) * inv, __uint_as_float(v[8 * q4 + 7]) * inv);
-            *(uint4*)(orow + c0 + 8 * q4) = w;
+            for (int q4 = 0; q4 < 4; ++q4) {
+              uint4 w;
+              w.x = pf_pack2<QT>(__uint_as_float(v[8 * q4 + 0]) * inv, __uint_as_float(v[8 * q4 + 1]) * inv);
+              w.y = pf_pack2<QT>(__uint_as_float(v[8 * q4 + 2]) * inv, __uint_as_float(v[8 * q4 + 3]) * inv);
+              w.z = pf_pack2<QT>(__uint_as_float(v[8 * q4 + 4]) * inv, __uint_as_float(v[8 * q4 + 5]) * inv);
+              w.w = pf_pack2<QT>(__uint_as_float(v[8 * q4 + 6]) * inv, __uint_as_float(v[8 * q4 + 7]) * inv);
+              *(uint4*)(orow + c0 + 8 * q4) = w;
+            }
           }
         }
-      }
-    } else {
-      // partial record of this row: unnormalised output, reference maximum, sum
-      float* rec = P.records + (((long long)unit * P.splits + seg) * kPrRows + x * kPrTile + row) * (D + 2);
+      } else {
+        // partial record of this row: unnormalised output, reference maximum, sum
+        float* rec = P.records + (((long long)blockIdx.x * 2 + (g.part == 2)) * kPrRows + x * kPrTile + row) * (D + 2);
 #pragma unroll 1
-      for (int c0 = 0; c0 < D; c0 += 32) {
-        unsigned v[32];
+        for (int c0 = 0; c0 < D; c0 += 32) {
+          unsigned v[32];
 #pragma unroll
-        for (int c = 0; c < 32; ++c) v[c] = 0u;
-        if (n_x > 0) {
-          tc_ld32(tO + c0, v);
-          tc_wait_ld32(v);
+          for (int c = 0; c < 32; ++c) v[c] = 0u;
+          if (n_x > 0) {
+            tc_ld32(tO + c0, v);
+            tc_wait_ld32(v);
+          }
+          if (bad)
+#pragma unroll
+            for (int c = 0; c < 32; ++c) v[c] = __float_as_uint(put_back(__uint_as_float(v[c]), c0 + c));
+          if (live)
+#pragma unroll
+            for (int c = 0; c < 32; c += 2) *(float2*)(rec + c0 + c) = make_float2(__uint_as_float(v[c]), __uint_as_float(v[c + 1]));
         }
-        if (bad)
-#pragma unroll
-          for (int c = 0; c < 32; ++c) v[c] = __float_as_uint(put_back(__uint_as_float(v[c]), c0 + c));
-        if (live)
-#pragma unroll
-          for (int c = 0; c < 32; c += 2) *(float2*)(rec + c0 + c) = make_float2(__uint_as_float(v[c]), __uint_as_float(v[c + 1]));
+        if (live) *(float2*)(rec + D) = make_float2(m_ref, l_sum);
       }
-      if (live) *(float2*)(rec + D) = make_float2(m_ref, l_sum);
+      tc_fence_before();      // O has been read: the arrivals of the next segment let it be overwritten
+      __syncwarp();
+      if (lane == 0) atomicAdd(ended, 1);
     }
   }
   tc_fence_before();
@@ -527,74 +813,58 @@ __global__ void __launch_bounds__(kPrThreads, 1) prompt_kernel(const PromptParam
   if (warp == 8) {
     __syncwarp();
     if (__any_sync(0xffffffffu, *abort_flag != 0)) {
-      // contractions and copies may be in flight: they end before tensor memory is freed and the CTA leaves
+      // contractions may be in flight: they end before tensor memory is freed and the CTA leaves
       if (tc_elect()) tc_commit(bar_e);
       tc_drain(bar_e, 0);
-      if (requested[1] > 0) tc_drain(bar_q, 0);
-#pragma unroll 1
-      for (int back = kStages; back > 0; --back) {
-        const int k = requested[0] - back, v = requested[1] - back;
-        if (k >= 0) tc_drain(bar_k + 8 * (k % kStages), (unsigned)(k / kStages) & 1u);
-        if (v >= t_dark) tc_drain(bar_d + 8 * (v % kStages), (unsigned)((v - t_dark) / kStages) & 1u);
-        else if (v >= 0) tc_drain(bar_v + 8 * (v % kStages), (unsigned)(v / kStages) & 1u);
-      }
       __syncwarp();
     }
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
   }
 }
 
-// Joins the KV segments of every item: out = sum_s O_s 2^(m_s - m) / sum_s l_s 2^(m_s - m).  A block takes 64 rows of
-// an item, a warp eight of them in turn, a lane D / 32 neighbouring channels; the loads of all segments of a row are
-// issued before the first is used.
-constexpr int kPrMergeRows = 64;
+// Joins the parts of the items that ranges cut: out = sum_c O_c 2^(m_c - m) / sum_c l_c 2^(m_c - m) over the parts in their
+// order.  Block (r, y) takes rows 32 y .. of the item that is cut where range r ends, if it begins in range r; a warp four of
+// them in turn, a lane D / 32 channels.
+constexpr int kPrMergeRows = 32;
 template <typename QT, int D>
-__global__ void __launch_bounds__(256) prompt_merge_kernel(const PromptParams P) {
+__global__ void __launch_bounds__(256) prompt_merge_kernel(const PromptParams P, int ctas) {
   follow_stream();
-  const int unit = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, head = unit % P.q_heads;
-  Sequence s;
-  int index = 0;
-  if (find_item(P, unit / P.q_heads, (P.k_rows + kPrTile - 1) / kPrTile, s, index) < 0) return;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = blockIdx.x;
+  const Deal deal(P, ctas);
+  if (r + 1 >= deal.ranges) return;
+  long long cut, begin;
+  const ItemCursor c = range_begin(P, deal, r + 1, cut);
+  if (c.step == 0) return;                                          // nothing is cut here
+  range_begin(P, deal, r, begin);
+  const long long item = cut - c.step;
+  if (begin > item) return;                                         // an earlier range's
+  int last = r + 1;                                                 // the range that holds the item's end
+  while (last + 1 < deal.ranges && deal.cut(last + 1) < item + c.cost - deal.slack()) ++last;
+  const Sequence& s = c.s;
 #pragma unroll 1
-  for (int r = warp; r < kPrMergeRows; r += 8) {
-    const int row = blockIdx.y * kPrMergeRows + r, q_row = index * kPrRows + row;
+  for (int i = warp; i < kPrMergeRows; i += 8) {
+    const int row = blockIdx.y * kPrMergeRows + i, q_row = c.item * kPrRows + row;
     if (q_row >= s.nq) return;
-    const float* base = P.records + ((long long)unit * P.splits * kPrRows + row) * (D + 2);
-    float2 ml[kPrMaxSplits], va[kPrMaxSplits][D / 64];
-#pragma unroll
-    for (int g = 0; g < kPrMaxSplits; ++g) {
-      if (g < P.splits) {
-        const float2* rec = (const float2*)(base + (long long)g * kPrRows * (D + 2));
-        ml[g] = __ldcg(rec + D / 2);
-#pragma unroll
-        for (int c = 0; c < D / 64; ++c) va[g][c] = __ldcg(rec + 32 * c + lane);
-      }
-    }
-    float top = kPrNegBig;
-#pragma unroll
-    for (int g = 0; g < kPrMaxSplits; ++g)
-      if (g < P.splits) top = fmaxf(top, ml[g].x);
-    float l = 0.f;
+    float top = kPrNegBig, l = 0.f;
     float2 o[D / 64] = {};
+    for (int part = r; part <= last; ++part) {
+      const float2* const rec = (const float2*)(P.records + ((2LL * part + (part == r)) * kPrRows + row) * (D + 2));
+      const float2 ml = __ldcg(rec + D / 2);
+      float2 x[D / 64];
 #pragma unroll
-    for (int g = 0; g < kPrMaxSplits; ++g) {
-      if (g < P.splits) {
-        const float w = pf_exp2(ml[g].x - top);
-        l = fmaf(ml[g].y, w, l);
+      for (int k = 0; k < D / 64; ++k) x[k] = __ldcg(rec + 32 * k + lane);
+      const float next = fmaxf(top, ml.x), before = pf_exp2(top - next), w = pf_exp2(ml.x - next);
+      top = next;
+      l = fmaf(ml.y, w, l * before);
 #pragma unroll
-        for (int c = 0; c < D / 64; ++c) {
-          o[c].x = fmaf(va[g][c].x, w, o[c].x);
-          o[c].y = fmaf(va[g][c].y, w, o[c].y);
-        }
-      }
+      for (int k = 0; k < D / 64; ++k) o[k] = make_float2(fmaf(x[k].x, w, o[k].x * before), fmaf(x[k].y, w, o[k].y * before));
     }
     const bool empty = s.nk - s.nq + q_row < 0;
     const float inv = empty ? 0.f : 1.f / l;
-    QT* out = (QT*)P.out + (long long)head * P.o_sh + (long long)(s.q0 + q_row) * P.o_st;
+    QT* out = (QT*)P.out + (long long)c.head * P.o_sh + (long long)(s.q0 + q_row) * P.o_st;
 #pragma unroll
-    for (int c = 0; c < D / 64; ++c) *(unsigned*)(out + 64 * c + 2 * lane) = pf_pack2<QT>(o[c].x * inv, o[c].y * inv);
-    if (lane == 0 && P.lse)
-      P.lse[head * P.lse_stride + s.q0 + q_row] = empty ? __int_as_float(0xff800000) : (top + log2f(l)) * kLn2;
+    for (int k = 0; k < D / 64; ++k) *(unsigned*)(out + 64 * k + 2 * lane) = pf_pack2<QT>(o[k].x * inv, o[k].y * inv);
+    if (lane == 0 && P.lse) P.lse[c.head * P.lse_stride + s.q0 + q_row] = empty ? __int_as_float(0xff800000) : (top + log2f(l)) * kLn2;
   }
 }
 
@@ -652,9 +922,6 @@ struct KeySteps {
     return groups * ((long long)t * tiles - sum);
   }
 };
-__device__ __forceinline__ long long shuffle64(long long v, int lane) {
-  return (long long)__shfl_sync(0xffffffffu, (unsigned long long)v, lane);
-}
 // Steps of all items; the whole warp takes part.
 __device__ __forceinline__ long long count_steps(const PromptParams& P) {
   long long n = 0;
@@ -1103,7 +1370,6 @@ PromptParams base_params(const inq_prompt_args_t* a) {
   P.cu_q = a->cu_q; P.cu_k = a->cu_k;
   P.n_seq = a->n_seq; P.q_rows = (int)a->q_rows; P.k_rows = (int)a->k_rows;
   P.q_heads = a->q_heads; P.kv_heads = a->kv_heads;
-  P.splits = 1;
   P.scale_log2e = a->scale * kLog2e;
   P.status = a->status;
   P.records = (float*)a->workspace;
@@ -1118,27 +1384,11 @@ int sm_count(int* n) {
 // Items that `rows` rows of `n_seq` sequences make at most.
 long long most_tiles(long long rows, int n_seq) { return rows / kPrRows + std::min<long long>(rows, n_seq); }
 
-// KV segments per item of inq_prompt_attention.  Cuts only pay while the items are few compared with the SMs: at most 2048
-// segments in all.  The lengths are not known here, a mean sequence stands for all: rounds of CTAs over the SMs, each
-// as long as a mean segment, six tile times per cut (the model of inq_prefill_attention, with its figures).
-int attention_cuts(int q_heads, long long q_rows, long long k_rows, int n_seq, int n_sm) {
-  const long long items = most_tiles(q_rows, n_seq) * q_heads;
-  const int most = (int)std::max<long long>(1, std::min<long long>(kPrMaxSplits, 2048 / std::max<long long>(items, 1)));
-  const double keys = (double)k_rows / n_seq, queries = (double)q_rows / n_seq;
-  const double tiles = std::max(1.0, (keys - 0.5 * std::min(queries, keys)) / kPrTile);
-  const long long likely = std::max<long long>(1, (q_rows / kPrRows + (n_seq + 1) / 2) * q_heads);
-  double best = 1e30;
-  int cuts = 1;
-  for (int sp = 1; sp <= most; ++sp) {
-    if (sp > 1 && tiles / sp < 2) break;
-    const double rounds = (double)((likely * sp + n_sm - 1) / n_sm);
-    const double cost = rounds * (tiles / sp + (sp > 1 ? 6.0 : 0.0));
-    if (cost < best - 1e-9) {
-      best = cost;
-      cuts = sp;
-    }
-  }
-  return cuts;
+// Whether the kernel may find that cutting items pays (see Deal): not where even the dearest item that the tensors allow costs
+// no more than a cut, nor where the items are many rounds of whole ones.
+bool attention_may_cut(int q_heads, long long q_rows, long long k_rows, int n_seq, int n_sm) {
+  const long long least = std::max<long long>(1, q_rows / kPrRows) * q_heads;
+  return k_rows > 8 * kPrTile && least < 3LL * n_sm;
 }
 // Columns of a step per query head: windows of at most 64 queries lie side by side, as many as the group has heads for.
 int weights_width(int group, int window) {
@@ -1152,17 +1402,15 @@ bool weights_cut(int group, long long q_rows, int window) {
   const long long tiles = (std::min<long long>(q_rows, window > 0 ? window : q_rows) + kPrTile - 1) / kPrTile;
   return tiles * ((group * width + kPrTile - 1) / kPrTile) > kPwWhole;
 }
-long long attention_record_bytes(int q_heads, int head_dim, long long q_rows, int n_seq, int cuts) {
-  return cuts > 1 ? most_tiles(q_rows, n_seq) * q_heads * cuts * kPrRows * (head_dim + 2) * (long long)sizeof(float) : 0;
-}
+long long attention_record_bytes(int head_dim, int n_sm) { return 2LL * n_sm * kPrRows * (head_dim + 2) * (long long)sizeof(float); }
+
 template <typename QT, int D>
 int launch_attention(const PromptParams& P, unsigned ctas, cudaStream_t stream, const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v) {
   const int fit = prompt_registers_fit((const void*)prompt_kernel<QT, D>);
   if (fit != INQ_OK) return fit;
   INQ_CUDA_CHECK(cudaFuncSetAttribute(prompt_kernel<QT, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, PromptShape<D>::kSmem));
   INQ_CUDA_CHECK(launch_following(prompt_kernel<QT, D>, ctas, kPrThreads, PromptShape<D>::kSmem, stream, P, q, k, v));
-  if (P.splits > 1)
-    INQ_CUDA_CHECK(launch_following(prompt_merge_kernel<QT, D>, dim3(ctas / P.splits, kPrRows / kPrMergeRows), 256, 0, stream, P));
+  if (P.records) INQ_CUDA_CHECK(launch_following(prompt_merge_kernel<QT, D>, dim3(ctas, kPrRows / kPrMergeRows), 256, 0, stream, P, (int)ctas));
   return INQ_OK;
 }
 template <typename QT, int D>
@@ -1181,7 +1429,7 @@ extern "C" int64_t inq_prompt_workspace_bytes(int32_t q_heads, int32_t kv_heads,
   int n_sm = 0;
   if (q_heads < 1 || kv_heads < 1 || n_seq < 1 || q_rows < 0 || k_rows < 0 || sm_count(&n_sm) != INQ_OK) return 0;
   return weights ? weights_cut(q_heads / kv_heads, q_rows, window) ? 2LL * n_sm * kPrRows * (int64_t)sizeof(float) : 0
-                 : attention_record_bytes(q_heads, head_dim, q_rows, n_seq, attention_cuts(q_heads, q_rows, k_rows, n_seq, n_sm));
+                 : attention_may_cut(q_heads, q_rows, k_rows, n_seq, n_sm) ? attention_record_bytes(head_dim, n_sm) : 0;
 }
 
 extern "C" int inq_prompt_attention(const inq_prompt_args_t* a, inq_stream_t stream_) {
@@ -1195,16 +1443,15 @@ extern "C" int inq_prompt_attention(const inq_prompt_args_t* a, inq_stream_t str
   int n_sm = 0;
   const int sm_rc = sm_count(&n_sm);
   if (sm_rc != INQ_OK) return sm_rc;
-  const long long items = most_tiles(a->q_rows, a->n_seq) * a->q_heads;
-  P.splits = attention_cuts(a->q_heads, a->q_rows, a->k_rows, a->n_seq, n_sm);
-  if (!a->workspace || a->workspace_bytes < attention_record_bytes(a->q_heads, a->head_dim, a->q_rows, a->n_seq, P.splits)) P.splits = 1;
-  if (items * P.splits > 0x7fffffffLL) return INQ_ERR_CAPACITY;
+  if (!attention_may_cut(a->q_heads, a->q_rows, a->k_rows, a->n_seq, n_sm) || !a->workspace ||
+      a->workspace_bytes < attention_record_bytes(a->head_dim, n_sm))
+    P.records = nullptr;
   CUtensorMap map_q, map_k, map_v;
   if (!make_map(&map_q, a->q, a->dtype, a->head_dim, a->q_rows, a->q_heads, a->q_stride_t, a->q_stride_h, kPrTile) ||
       !make_map(&map_k, a->k, a->dtype, a->head_dim, a->k_rows, a->kv_heads, a->k_stride_t, a->k_stride_h, kPrTile) ||
       !make_map(&map_v, a->v, a->dtype, a->head_dim, a->k_rows, a->kv_heads, a->v_stride_t, a->v_stride_h, kPrTile))
     return INQ_ERR_ARGUMENT;
-  const unsigned ctas = (unsigned)(items * P.splits);
+  const unsigned ctas = (unsigned)std::min<long long>(n_sm, most_tiles(a->q_rows, a->n_seq) * a->q_heads);
   cudaStream_t stream = (cudaStream_t)stream_;
   if (a->dtype == INQ_F16)
     return a->head_dim == 64 ? launch_attention<__half, 64>(P, ctas, stream, map_q, map_k, map_v)
