@@ -33,6 +33,7 @@ constexpr float kPrNegBig = -3.0e38f;        // stands for the maximum of nothin
 constexpr float kPrSlack = 8.f;              // the reference maximum may lag the true one by 2^8
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
+struct CutItem;
 struct PromptParams {
   void* out;
   float* lse;                       // attention: written, weights: read; [q_heads][lse_stride]
@@ -43,6 +44,7 @@ struct PromptParams {
   int window;                       // weights: queries per sequence that count, 0 = all
   int width;                        // weights: columns of a step per query head
   float* records;                   // partial results of cut items
+  CutItem* cuts;                    // of attention, per CTA
   float scale_log2e;
   int* status;
 };
@@ -120,12 +122,11 @@ __device__ __forceinline__ int find_item(const PromptParams& P, int rank, int ma
 }
 
 // How the items of a launch are dealt to its CTAs.  Ordinarily whole: in the order of falling cost, every other round through
-// the CTAs backwards, so that they end at about the same time.  Where that leaves SMs idle -- few items behind long
+// the CTAs backwards, so that they end at about the same time.  Where that leaves most SMs idle -- few items behind long
 // histories -- the steps (tiles of 128 keys) of all items form one list (request, head, item) that is cut into equal
-// ranges; what the ranges leave of a cut item is joined by a second launch, which is priced at six steps.
-// The estimates, in steps: whole items max(dearest, mean + dearest / rounds), ranges mean + 6.  (1500 tokens of 32 heads:
-// 15 and 15; 8192 of 28: 209 and 206, whole because a cut has to promise a tenth; 4 x 350 tokens behind 5000 of 32: 85
-// and 64, measured 121 and 87 us.)
+// ranges; what the ranges leave of a cut item is joined by a second launch.  The estimates, in steps: whole items
+// max(dearest, mean + dearest / rounds), ranges mean + 6 (parts written, read and joined), and a tenth less.
+constexpr int kPrCut = 6;
 constexpr int kPrShortest = 12;      // steps of a range, where items have as many
 // Item i of a sequence: query rows 256 i ..; it takes ceil(keys that its last row sees / 128) steps.
 struct ItemSteps {
@@ -149,6 +150,10 @@ __device__ __forceinline__ long long shuffle64(long long v, int lane) {
 // An item, or the part of it that a range holds.
 struct Segment {
   int valid, q_base, nq, k_base, nk, head, q0, t_lo, n_t, part;      // part: 0 the whole item, 1 not its beginning, 2 its beginning
+};
+// What the joining launch has to know of a range: the item that is cut where it ends, if the item begins in it.
+struct CutItem {
+  int valid, q_base, nq, hist, head, q0, last, reserved;      // last: the range that holds the item's end
 };
 struct Deal {
   long long total, items;      // steps and items of all heads
@@ -178,7 +183,7 @@ struct Deal {
     const long long rounds = (items + ctas - 1) / ctas;
     if (rounds > 64) return;
     const long long whole = max(dearest * ctas * rounds, rounds > 1 ? total * rounds + (long long)dearest * ctas : 0);
-    if (10 * (total + 6LL * most) * ctas * rounds < 9 * most * whole) ranges = most;
+    if (10 * (total + (long long)kPrCut * most) * ctas * rounds < 9 * most * whole) ranges = most;
   }
   __device__ __forceinline__ long long cut(int range) const { return (long long)((double)total / ranges * range); }
   // A cut near the edge of an item moves there.
@@ -403,6 +408,7 @@ __global__ void __launch_bounds__(kPrThreads, 1) prompt_kernel(const PromptParam
         more = whole(round++);
       } else {
         const Deal deal(P, gridDim.x);
+        CutItem mark = {};
         cut = deal.ranges > 0;
         if (cut && (int)blockIdx.x < deal.ranges) {
           long long step, end;
@@ -412,9 +418,17 @@ __global__ void __launch_bounds__(kPrThreads, 1) prompt_kernel(const PromptParam
             const int steps = (int)min(end - step, (long long)(c.cost - c.step));
             publish(Segment{1, c.s.q0, c.s.nq, c.s.k0, c.s.nk, c.head, c.item * kPrRows, c.step, steps, steps == c.cost ? 0 : c.step ? 1 : 2});
             step += steps;
+            if (step == end && c.step + steps < c.cost && c.step == 0) {
+              // the item goes on behind this range, and begins in it
+              const long long item = step - steps;
+              int last = blockIdx.x + 1;
+              while (last + 1 < deal.ranges && deal.cut(last + 1) < item + c.cost - deal.slack()) ++last;
+              mark = CutItem{1, c.s.q0, c.s.nq, c.s.nk - c.s.nq, c.head, c.item * kPrRows, last, 0};
+            }
             if (step < end) next_item(P, c);
           }
         }
+        if (lane == 0) P.cuts[blockIdx.x] = mark;
       }
       // offsets that the tensors do not hold, and queries without a key
       for (int b = blockIdx.x; b < P.n_seq; b += gridDim.x) {
@@ -823,48 +837,49 @@ __global__ void __launch_bounds__(kPrThreads, 1) prompt_kernel(const PromptParam
 }
 
 // Joins the parts of the items that ranges cut: out = sum_c O_c 2^(m_c - m) / sum_c l_c 2^(m_c - m) over the parts in their
-// order.  Block (r, y) takes rows 32 y .. of the item that is cut where range r ends, if it begins in range r; a warp four of
-// them in turn, a lane D / 32 channels.
-constexpr int kPrMergeRows = 32;
+// order.  Block (r, y) takes rows 32 y .. of the item that is cut where range r ends, if it begins in range r; a warp four
+// rows at once, a lane D / 32 channels, and the next part is asked for while one is added.
+constexpr int kPrMergeRows = 32, kPrMergeEach = 4;
 template <typename QT, int D>
-__global__ void __launch_bounds__(256) prompt_merge_kernel(const PromptParams P, int ctas) {
+__global__ void __launch_bounds__(256) prompt_merge_kernel(const PromptParams P) {
   follow_stream();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = blockIdx.x;
-  const Deal deal(P, ctas);
-  if (r + 1 >= deal.ranges) return;
-  long long cut, begin;
-  const ItemCursor c = range_begin(P, deal, r + 1, cut);
-  if (c.step == 0) return;                                          // nothing is cut here
-  range_begin(P, deal, r, begin);
-  const long long item = cut - c.step;
-  if (begin > item) return;                                         // an earlier range's
-  int last = r + 1;                                                 // the range that holds the item's end
-  while (last + 1 < deal.ranges && deal.cut(last + 1) < item + c.cost - deal.slack()) ++last;
-  const Sequence& s = c.s;
-#pragma unroll 1
-  for (int i = warp; i < kPrMergeRows; i += 8) {
-    const int row = blockIdx.y * kPrMergeRows + i, q_row = c.item * kPrRows + row;
-    if (q_row >= s.nq) return;
-    float top = kPrNegBig, l = 0.f;
-    float2 o[D / 64] = {};
-    for (int part = r; part <= last; ++part) {
-      const float2* const rec = (const float2*)(P.records + ((2LL * part + (part == r)) * kPrRows + row) * (D + 2));
-      const float2 ml = __ldcg(rec + D / 2);
-      float2 x[D / 64];
+  const CutItem c = P.cuts[r];
+  const int row0 = blockIdx.y * kPrMergeRows + warp * kPrMergeEach;
+  if (!c.valid || c.q0 + row0 >= c.nq) return;
+  float top[kPrMergeEach], l[kPrMergeEach] = {};
+  float2 o[kPrMergeEach][D / 64] = {};
 #pragma unroll
-      for (int k = 0; k < D / 64; ++k) x[k] = __ldcg(rec + 32 * k + lane);
-      const float next = fmaxf(top, ml.x), before = pf_exp2(top - next), w = pf_exp2(ml.x - next);
-      top = next;
-      l = fmaf(ml.y, w, l * before);
+  for (int i = 0; i < kPrMergeEach; ++i) top[i] = kPrNegBig;
+#pragma unroll 2
+  for (int part = r; part <= c.last; ++part) {
+    float2 ml[kPrMergeEach], x[kPrMergeEach][D / 64];
 #pragma unroll
-      for (int k = 0; k < D / 64; ++k) o[k] = make_float2(fmaf(x[k].x, w, o[k].x * before), fmaf(x[k].y, w, o[k].y * before));
+    for (int i = 0; i < kPrMergeEach; ++i) {      // rows that the item does not have hold whatever memory does, and are not stored
+      const float2* const rec = (const float2*)(P.records + ((2LL * part + (part == r)) * kPrRows + row0 + i) * (D + 2));
+      ml[i] = __ldcg(rec + D / 2);
+#pragma unroll
+      for (int k = 0; k < D / 64; ++k) x[i][k] = __ldcg(rec + 32 * k + lane);
     }
-    const bool empty = s.nk - s.nq + q_row < 0;
-    const float inv = empty ? 0.f : 1.f / l;
-    QT* out = (QT*)P.out + (long long)c.head * P.o_sh + (long long)(s.q0 + q_row) * P.o_st;
 #pragma unroll
-    for (int k = 0; k < D / 64; ++k) *(unsigned*)(out + 64 * k + 2 * lane) = pf_pack2<QT>(o[k].x * inv, o[k].y * inv);
-    if (lane == 0 && P.lse) P.lse[c.head * P.lse_stride + s.q0 + q_row] = empty ? __int_as_float(0xff800000) : (top + log2f(l)) * kLn2;
+    for (int i = 0; i < kPrMergeEach; ++i) {
+      const float next = fmaxf(top[i], ml[i].x), before = pf_exp2(top[i] - next), w = pf_exp2(ml[i].x - next);
+      top[i] = next;
+      l[i] = fmaf(ml[i].y, w, l[i] * before);
+#pragma unroll
+      for (int k = 0; k < D / 64; ++k) o[i][k] = make_float2(fmaf(x[i][k].x, w, o[i][k].x * before), fmaf(x[i][k].y, w, o[i][k].y * before));
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < kPrMergeEach; ++i) {
+    const int q_row = c.q0 + row0 + i;
+    if (q_row >= c.nq) return;
+    const bool empty = c.hist + q_row < 0;
+    const float inv = empty ? 0.f : 1.f / l[i];
+    QT* out = (QT*)P.out + (long long)c.head * P.o_sh + (long long)(c.q_base + q_row) * P.o_st;
+#pragma unroll
+    for (int k = 0; k < D / 64; ++k) *(unsigned*)(out + 64 * k + 2 * lane) = pf_pack2<QT>(o[i][k].x * inv, o[i][k].y * inv);
+    if (lane == 0 && P.lse) P.lse[c.head * P.lse_stride + c.q_base + q_row] = empty ? __int_as_float(0xff800000) : (top[i] + log2f(l[i])) * kLn2;
   }
 }
 
@@ -1184,6 +1199,11 @@ __global__ void __launch_bounds__(kPrThreads, 1) prompt_weights_kernel(const Pro
       left -= steps;
       if (left > 0) next_item(P, at);
     }
+    // the CTA does not leave before the last commits have arrived
+    if (step > 0) {
+      tc_wait(bar_qfree + 8 * ((step - 1) % kStages), (unsigned)((step - 1) / kStages) & 1u, abort_flag);
+      tc_wait(bar_kfree + 8 * ((pairs - 1) & 1), (unsigned)((pairs - 1) >> 1) & 1u, abort_flag);
+    }
   } else if (warp == 10) {
     // ================================================================ describes the columns, four to a lane
     const int width = P.width, column = 4 * lane, column_head = column / width, column_q = column & (width - 1);
@@ -1402,7 +1422,9 @@ bool weights_cut(int group, long long q_rows, int window) {
   const long long tiles = (std::min<long long>(q_rows, window > 0 ? window : q_rows) + kPrTile - 1) / kPrTile;
   return tiles * ((group * width + kPrTile - 1) / kPrTile) > kPwWhole;
 }
-long long attention_record_bytes(int head_dim, int n_sm) { return 2LL * n_sm * kPrRows * (head_dim + 2) * (long long)sizeof(float); }
+long long attention_record_bytes(int head_dim, int n_sm) {
+  return n_sm * (2LL * kPrRows * (head_dim + 2) * (long long)sizeof(float) + (long long)sizeof(CutItem));
+}
 
 template <typename QT, int D>
 int launch_attention(const PromptParams& P, unsigned ctas, cudaStream_t stream, const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v) {
@@ -1410,7 +1432,7 @@ int launch_attention(const PromptParams& P, unsigned ctas, cudaStream_t stream, 
   if (fit != INQ_OK) return fit;
   INQ_CUDA_CHECK(cudaFuncSetAttribute(prompt_kernel<QT, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, PromptShape<D>::kSmem));
   INQ_CUDA_CHECK(launch_following(prompt_kernel<QT, D>, ctas, kPrThreads, PromptShape<D>::kSmem, stream, P, q, k, v));
-  if (P.records) INQ_CUDA_CHECK(launch_following(prompt_merge_kernel<QT, D>, dim3(ctas, kPrRows / kPrMergeRows), 256, 0, stream, P, (int)ctas));
+  if (P.records) INQ_CUDA_CHECK(launch_following(prompt_merge_kernel<QT, D>, dim3(ctas, kPrRows / kPrMergeRows), 256, 0, stream, P));
   return INQ_OK;
 }
 template <typename QT, int D>
@@ -1446,12 +1468,13 @@ extern "C" int inq_prompt_attention(const inq_prompt_args_t* a, inq_stream_t str
   if (!attention_may_cut(a->q_heads, a->q_rows, a->k_rows, a->n_seq, n_sm) || !a->workspace ||
       a->workspace_bytes < attention_record_bytes(a->head_dim, n_sm))
     P.records = nullptr;
+  P.cuts = P.records ? (CutItem*)(P.records + 2LL * n_sm * kPrRows * (a->head_dim + 2)) : nullptr;
   CUtensorMap map_q, map_k, map_v;
   if (!make_map(&map_q, a->q, a->dtype, a->head_dim, a->q_rows, a->q_heads, a->q_stride_t, a->q_stride_h, kPrTile) ||
       !make_map(&map_k, a->k, a->dtype, a->head_dim, a->k_rows, a->kv_heads, a->k_stride_t, a->k_stride_h, kPrTile) ||
       !make_map(&map_v, a->v, a->dtype, a->head_dim, a->k_rows, a->kv_heads, a->v_stride_t, a->v_stride_h, kPrTile))
     return INQ_ERR_ARGUMENT;
-  const unsigned ctas = (unsigned)std::min<long long>(n_sm, most_tiles(a->q_rows, a->n_seq) * a->q_heads);
+  const unsigned ctas = (unsigned)(P.records ? n_sm : std::min<long long>(n_sm, most_tiles(a->q_rows, a->n_seq) * a->q_heads));
   cudaStream_t stream = (cudaStream_t)stream_;
   if (a->dtype == INQ_F16)
     return a->head_dim == 64 ? launch_attention<__half, 64>(P, ctas, stream, map_q, map_k, map_v)

@@ -68,11 +68,13 @@ def formula(q, k, v, lengths, keys, scale, window=0):
 
 
 def check(q, k, v, lengths, keys, scale=None, window=0, cu_offset=0):
+    from inquant import _native as N
     from inquant.prompt import prompt_attention, prompt_weights
     scale = q.shape[2] ** -0.5 if scale is None else scale
     cu, cu_k = ints(starts(lengths)), ints(starts(keys))
     out, lse = prompt_attention(q, k, v, cu, cu_k, scale=scale)
     w = prompt_weights(q, k, lse, cu, cu_k, scale=scale, window=window or None)
+    assert N.take_status(q.device) == 0      # no wait gave up
     want, share, delta, want_lse, lse_bound, want_w, w_bound = formula(q, k, v, lengths, keys, scale, window)
     n, m, u = sum(lengths), sum(keys), unit(q.dtype)
     off = (out[:n].double() - want[:n]).abs()
@@ -126,6 +128,15 @@ def test_long_histories_are_cut_and_joined(dim, dtype, lengths, keys):
 def test_long_prompt_of_many_steps_per_item():
     q, k, v = states([2900], [2900], 7, 1, 128, torch.bfloat16, seed=4)
     check(q, k, v, [2900], [2900], window=1000)
+
+
+@pytest.mark.parametrize("dim,dtype", [(128, torch.bfloat16), (64, torch.float16)])
+@pytest.mark.parametrize("lengths,past", [([17, 900, 256, 1, 1300, 640, 90, 128, 1100, 333, 512, 700], [0] * 12), ([130, 0, 300, 60, 500], [1900, 700, 40, 2500, 1000])])
+def test_many_items_per_sm(lengths, past, dim, dtype):
+    """Items with and without a second tile, of one step to many, one behind the other in a CTA."""
+    keys = [n + p for n, p in zip(lengths, past)]
+    q, k, v = states(lengths, keys, 32, 8, dim, dtype, seed=11)
+    check(q, k, v, lengths, keys)
 
 
 def test_large_logits_raise_the_reference_maximum():
