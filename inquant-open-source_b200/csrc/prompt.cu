@@ -884,7 +884,8 @@ __global__ void __launch_bounds__(256) prompt_merge_kernel(const PromptParams P)
 }
 
 // ---------------------------------------------------------------------------------------- attention weights of keys
-// An item is 256 keys (tiles A and B, one softmax warpgroup each) of one KV head; a step of it is 128 columns of queries:
+// An item is 256 keys (tiles A and B, two softmax warpgroups each, which share out the columns) of one KV head; a step of it
+// is 128 columns of queries:
 // a tile of 128 queries of one query head of the group or, with a window of at most 64, the windows of 128 / width heads
 // side by side.  The steps of all items form one list (request, KV head, keys rising, then query heads and queries), cut
 // into equal ranges, one per CTA: what an item costs, 256 keys near the end of a sequence a fraction of the first ones,
@@ -912,8 +913,12 @@ struct WeightsShape {
   static constexpr int kBars = 4 + 2 * kStages + 8 + 2 * kPwColumns + 1;
   // after the tiles: TMEM base, abort flag, request counts; the range; barriers; what the columns of the next steps are
   static constexpr int kRangeOffset = kTiles + 16, kBarOffset = kTiles + 128, kColumnsOffset = kBarOffset + 8 * kBars + 8;
-  static constexpr int kSmem = kColumnsOffset + kPwColumns * kPwColumnBytes;
+  static constexpr int kSumOffset = kColumnsOffset + kPwColumns * kPwColumnBytes;      // sums of the second halves of the columns
+  static constexpr int kSmem = kSumOffset + kPrRows * 4;
 };
+constexpr int kPwThreads = 640;      // 16 softmax warps, then the MMA warp, the TMA warp, one that describes columns, an idle one
+constexpr int kPwSoftmaxWarps = 16;
+constexpr int kPwLaunchRegs = 96, kPwIssueRegs = 64, kPwSoftmaxRegs = (5 * kPwLaunchRegs - kPwIssueRegs) / 4;
 constexpr int kPwWhole = 8;       // items of at most so many steps are not cut
 
 // The steps of one KV head of a sequence.  Key tile t costs `groups` x (tiles - first(t)) steps, first(t) being its first
@@ -1030,7 +1035,7 @@ __device__ __forceinline__ StepCursor range_cursor(const PromptParams& P, long l
 }
 
 template <typename QT, int D>
-__global__ void __launch_bounds__(kPrThreads, 1) prompt_weights_kernel(const PromptParams P, const __grid_constant__ CUtensorMap map_q,
+__global__ void __launch_bounds__(kPwThreads, 1) prompt_weights_kernel(const PromptParams P, const __grid_constant__ CUtensorMap map_q,
                                                                        const __grid_constant__ CUtensorMap map_k) {
   using S = WeightsShape<D>;
   constexpr int kStages = S::kStages, kTileBytes = S::kTileBytes;
@@ -1089,27 +1094,28 @@ __global__ void __launch_bounds__(kPrThreads, 1) prompt_weights_kernel(const Pro
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         tc_bar_init(bar_s + 8 * i, 1);
-        tc_bar_init(bar_f + 8 * i, kPrTile);
+        tc_bar_init(bar_f + 8 * i, 2 * kPrTile);
       }
 #pragma unroll
       for (int i = 0; i < kPwColumns; ++i) {
         tc_bar_init(bar_c + 8 * i, 32);
-        tc_bar_init(bar_cfree + 8 * i, 8);
+        tc_bar_init(bar_cfree + 8 * i, kPwSoftmaxWarps);
       }
       tc_bar_init(bar_e, 1);
       asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-  } else if (warp < 8) {
+  } else if (warp < kPwSoftmaxWarps) {
     // offsets that the tensors do not hold, and keys of a sequence without queries
+    constexpr int kThreads = 32 * (kPwSoftmaxWarps - 3);
     const int t = tid - 96;
     for (int b = blockIdx.x; b < P.n_seq; b += gridDim.x) {
       if (t == 0 && bad_sequence(P, b)) atomicOr(P.status, INQ_STATUS_BAD_INDEX);
       const Sequence s = load_sequence(P, b);
       if (s.nq == 0)
         for (int h = 0; h < P.kv_heads; ++h)
-          for (int i = t; i < s.nk; i += 160) P.weights[h * P.weights_stride + s.k0 + i] = 0.f;
+          for (int i = t; i < s.nk; i += kThreads) P.weights[h * P.weights_stride + s.k0 + i] = 0.f;
     }
-  } else if (warp == 8) {
+  } else if (warp == kPwSoftmaxWarps) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(tc_smem(tmem_base_p)), "r"(512) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
@@ -1121,10 +1127,10 @@ __global__ void __launch_bounds__(kPrThreads, 1) prompt_weights_kernel(const Pro
   const int group = P.q_heads / P.kv_heads, heads_per_step = kPrTile / P.width;
   int left = (int)(range->end - range->first);           // steps of this range
 
-  if (warp >= 8) {
-  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kPrIssueRegs));
+  if (warp >= kPwSoftmaxWarps) {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kPwIssueRegs));
   StepCursor at = range->at;
-  if (warp == 9) {
+  if (warp == kPwSoftmaxWarps + 1) {
     // ================================================================ TMA warp
     int pairs = 0, tiles = 0;      // key pairs and query tiles requested so far
     bool go = true;
@@ -1164,7 +1170,7 @@ __global__ void __launch_bounds__(kPrThreads, 1) prompt_weights_kernel(const Pro
       left -= steps;
       if (left > 0) next_item(P, at);
     }
-  } else if (warp == 8) {
+  } else if (warp == kPwSoftmaxWarps) {
     // ================================================================ MMA warp
     constexpr bool kBf16 = !std::is_same<QT, __half>::value;
     constexpr unsigned idesc = tc_idesc<kBf16, 128, 128, false>();
@@ -1204,7 +1210,7 @@ __global__ void __launch_bounds__(kPrThreads, 1) prompt_weights_kernel(const Pro
       tc_wait(bar_qfree + 8 * ((step - 1) % kStages), (unsigned)((step - 1) / kStages) & 1u, abort_flag);
       tc_wait(bar_kfree + 8 * ((pairs - 1) & 1), (unsigned)((pairs - 1) >> 1) & 1u, abort_flag);
     }
-  } else if (warp == 10) {
+  } else if (warp == kPwSoftmaxWarps + 2) {
     // ================================================================ describes the columns, four to a lane
     const int width = P.width, column = 4 * lane, column_head = column / width, column_q = column & (width - 1);
     int step = 0;
@@ -1248,9 +1254,10 @@ __global__ void __launch_bounds__(kPrThreads, 1) prompt_weights_kernel(const Pro
     }
   }
   } else {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kPrSoftmaxRegs));
-    // ================================================================ one thread per key row
-    const int x = warp >> 2, row = tid & (kPrTile - 1), width = P.width;
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kPwSoftmaxRegs));
+    // ================================================================ two threads per key row, 64 columns each
+    const int x = (warp >> 2) & 1, half = warp >> 3, row = tid & (kPrTile - 1), width = P.width;
+    float* const second = (float*)(pr_raw + S::kSumOffset) + x * kPrTile + row;
     const unsigned tS = tmem + ((unsigned)((warp & 3) * 32) << 16) + 256 * x;
     const unsigned long long scale2 = pf_pair(P.scale_log2e, P.scale_log2e);
     float sum = 0.f;
@@ -1266,20 +1273,21 @@ __global__ void __launch_bounds__(kPrThreads, 1) prompt_weights_kernel(const Pro
       tc_wait(bar_s + 16 * x + 8 * buffer, (unsigned)(step >> 1) & 1u, abort_flag);
       __syncwarp();
       tc_fence_after();
-      unsigned v[4][32];
-#pragma unroll
-      for (int q = 0; q < 4; ++q) tc_ld32(tS + 128 * buffer + 32 * q, v[q]);
-#pragma unroll
-      for (int q = 0; q < 4; ++q) tc_wait_ld32(v[q]);
+      unsigned v[2][32];
+      tc_ld32(tS + 128 * buffer + 64 * half, v[0]);
+      tc_ld32(tS + 128 * buffer + 64 * half + 32, v[1]);
+      tc_wait_ld32(v[0]);
+      tc_wait_ld32(v[1]);
       tc_fence_before();
       pf_arrive(bar_f + 16 * x + 8 * buffer);
       unsigned long long sums[2] = {pf_pair(0.f, 0.f), pf_pair(0.f, 0.f)};
-      // Columns 32 q .. 32 q + 31; bit c of `seen`: column 32 q + c counts.  (A polynomial on the FMA units in the place of a
-      // quarter or three eighths of the exponentials changed nothing: 87 to 90 us for 4096 tokens either way.)
+      // Columns 32 q .. 32 q + 31 of this half; bit c of `seen`: column 32 q + c counts.  (A polynomial on the FMA units in the
+      // place of a quarter or three eighths of the exponentials changed nothing, with eight softmax warps: 87 to 90 us for
+      // 4096 tokens either way.)
       auto add = [&](int q, auto some, unsigned seen) {
 #pragma unroll
         for (int c = 0; c < 32; c += 4) {
-          const float4 l4 = *(const float4*)(exponents + 32 * q + c);
+          const float4 l4 = *(const float4*)(exponents + 64 * half + 32 * q + c);
 #pragma unroll
           for (int p = 0; p < 2; ++p) {
             const int i = c + 2 * p;
@@ -1299,15 +1307,16 @@ __global__ void __launch_bounds__(kPrThreads, 1) prompt_weights_kernel(const Pro
       };
       if (!masked) {
 #pragma unroll
-        for (int q = 0; q < 4; ++q) add(q, std::false_type{}, 0u);
+        for (int q = 0; q < 2; ++q) add(q, std::false_type{}, 0u);
       } else {
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          if (32 * q < columns) {
+        for (int q = 0; q < 2; ++q) {
+          const int column = 64 * half + 32 * q;
+          if (column < columns) {
             // columns of queries lo .. hi - 1 of a window, of one head, of half a window, or of two heads
-            const int base = 32 * q & (width - 1), from = min(max(lo - base, 0), 32), to = min(max(hi - base, 0), 32);
+            const int base = column & (width - 1), from = min(max(lo - base, 0), 32), to = min(max(hi - base, 0), 32);
             unsigned seen = (unsigned)((1ull << to) - 1ull) & ~(unsigned)((1ull << from) - 1ull);
-            if (width == 16) seen = (seen & 0xffffu) | (32 * q + 16 < columns ? seen << 16 : 0u);
+            if (width == 16) seen = (seen & 0xffffu) | (column + 16 < columns ? seen << 16 : 0u);
             if (__any_sync(0xffffffffu, seen != 0u)) add(q, std::true_type{}, seen);
           }
         }
@@ -1316,7 +1325,12 @@ __global__ void __launch_bounds__(kPrThreads, 1) prompt_weights_kernel(const Pro
       pf_unpair(pf_add2(sums[0], sums[1]), even, odd);
       sum += even + odd;
       if (note->last) {
-        if (x * kPrTile + row < note->keys && *abort_flag == 0) (note->cut ? P.records : P.weights)[note->at + x * kPrTile + row] = sum;
+        // the halves' sums, always in this order; the second barrier frees the place
+        if (half) *second = sum;
+        asm volatile("bar.sync %0, 256;" ::"r"(1 + x) : "memory");
+        if (!half && x * kPrTile + row < note->keys && *abort_flag == 0)
+          (note->cut ? P.records : P.weights)[note->at + x * kPrTile + row] = sum + *second;
+        asm volatile("bar.sync %0, 256;" ::"r"(1 + x) : "memory");
         sum = 0.f;
       }
       __syncwarp();
@@ -1326,7 +1340,7 @@ __global__ void __launch_bounds__(kPrThreads, 1) prompt_weights_kernel(const Pro
   tc_fence_before();
   __syncthreads();
   if (tid == 0 && *abort_flag) atomicOr(P.status, INQ_STATUS_WAIT_TIMEOUT);
-  if (warp == 8) {
+  if (warp == kPwSoftmaxWarps) {
     __syncwarp();
     if (__any_sync(0xffffffffu, *abort_flag != 0)) {
       if (tc_elect()) tc_commit(bar_e);
@@ -1367,10 +1381,10 @@ using namespace inq;
 
 namespace {
 // The shares that setmaxnreg hands out must not exceed what the kernel is launched with (as in csrc/prefill.cu).
-int prompt_registers_fit(const void* kernel) {
+int prompt_registers_fit(const void* kernel, int launched) {
   cudaFuncAttributes attributes;
   INQ_CUDA_CHECK(cudaFuncGetAttributes(&attributes, kernel));
-  return attributes.numRegs < kPrLaunchRegs ? INQ_ERR_UNSUPPORTED : INQ_OK;
+  return attributes.numRegs < launched ? INQ_ERR_UNSUPPORTED : INQ_OK;
 }
 int check_args(const inq_prompt_args_t* a) {
   if (!a || !a->q || !a->k || !a->cu_q || !a->cu_k || !a->status) return INQ_ERR_ARGUMENT;
@@ -1428,7 +1442,7 @@ long long attention_record_bytes(int head_dim, int n_sm) {
 
 template <typename QT, int D>
 int launch_attention(const PromptParams& P, unsigned ctas, cudaStream_t stream, const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v) {
-  const int fit = prompt_registers_fit((const void*)prompt_kernel<QT, D>);
+  const int fit = prompt_registers_fit((const void*)prompt_kernel<QT, D>, kPrLaunchRegs);
   if (fit != INQ_OK) return fit;
   INQ_CUDA_CHECK(cudaFuncSetAttribute(prompt_kernel<QT, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, PromptShape<D>::kSmem));
   INQ_CUDA_CHECK(launch_following(prompt_kernel<QT, D>, ctas, kPrThreads, PromptShape<D>::kSmem, stream, P, q, k, v));
@@ -1437,10 +1451,10 @@ int launch_attention(const PromptParams& P, unsigned ctas, cudaStream_t stream, 
 }
 template <typename QT, int D>
 int launch_weights(const PromptParams& P, unsigned ctas, cudaStream_t stream, const CUtensorMap& q, const CUtensorMap& k) {
-  const int fit = prompt_registers_fit((const void*)prompt_weights_kernel<QT, D>);
+  const int fit = prompt_registers_fit((const void*)prompt_weights_kernel<QT, D>, kPwLaunchRegs);
   if (fit != INQ_OK) return fit;
   INQ_CUDA_CHECK(cudaFuncSetAttribute(prompt_weights_kernel<QT, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, WeightsShape<D>::kSmem));
-  INQ_CUDA_CHECK(launch_following(prompt_weights_kernel<QT, D>, ctas, kPrThreads, WeightsShape<D>::kSmem, stream, P, q, k));
+  INQ_CUDA_CHECK(launch_following(prompt_weights_kernel<QT, D>, ctas, kPwThreads, WeightsShape<D>::kSmem, stream, P, q, k));
   if (P.records) INQ_CUDA_CHECK(launch_following(prompt_weights_sum_kernel, ctas, kPrRows, 0, stream, P, (int)ctas));
   return INQ_OK;
 }
