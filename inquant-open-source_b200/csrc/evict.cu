@@ -69,7 +69,7 @@ __global__ void __launch_bounds__(kEvThreads, KEYS <= 5 ? 2 : 1) evict_select_ke
   const int row = blockIdx.x / ctas, b = row / P.kv_heads, h = row % P.kv_heads, tid = threadIdx.x;
   __shared__ int histograms[kEvPasses][kEvBins];      // one per pass: none is cleared while others read it
   __shared__ int shared_counts[2];                    // this CTA's free places and moving tokens
-  __shared__ int scratch[kEvThreads / 32], chosen[kEvPasses][2];
+  __shared__ int scratch[kEvThreads / 32], chosen[kEvPasses][3];
   const int warp = tid >> 5, lane = tid & 31;
   follow_stream();
   allow_next();
@@ -152,10 +152,17 @@ __global__ void __launch_bounds__(kEvThreads, KEYS <= 5 ? 2 : 1) evict_select_ke
     if (before < want && before + mine >= want) {
       chosen[pass][0] = kEvBins - 1 - tid;
       chosen[pass][1] = want - before;
+      chosen[pass][2] = mine == want - before;
     }
     __syncthreads();
     prefix = prefix << 8 | (unsigned)chosen[pass][0];
     want = chosen[pass][1];
+    if (chosen[pass][2]) {
+      // all tokens that begin like this stay, as they mostly do after three digits: no order among them is needed
+      prefix <<= shift;
+      want = 0x7fffffff;
+      break;
+    }
   }
   // tokens above the threshold stay, and the first `want` of those at it
   int ties_before = 0;
