@@ -496,8 +496,8 @@ typedef struct {
   int32_t requests, q_heads, kv_heads, head_dim, page_tokens, table_columns, dtype;
   float scale;
   int32_t* status;
-  int32_t* counters;              /* [requests * kv_heads * ceil(q_heads / kv_heads / 16) + 1], zero: every call leaves them zero,
-                                   * and calls that may run at the same time need counters of their own */
+  int32_t* counters;              /* [requests * kv_heads * ceil(q_heads / kv_heads / 16)], zero: every call leaves them zero, and
+                                   * calls that may run at the same time need counters of their own */
   void* workspace;                /* scratch of one call at a time */
   int64_t workspace_bytes;
 } inq_paged_attention_args_t;

@@ -3,16 +3,19 @@
 //
 // out = sum_j p_j v_j / sum_j p_j with p_j = 2^(s_j - m): one pass over the cache, bound by its bytes (2 D elements
 // a token and KV head).  What counts is that loads never pause, so the shape is built around them:
-//   * a unit is 128 tokens of one pair (request, KV head, up to 16 of its query heads); the units of all pairs form
-//     one list, cut into equal ranges, one per CTA and one CTA per SM.  The lengths are read on the device, so that a
-//     captured step serves every later length; a pair that no range cuts is finished by its CTA.
+//   * a unit is 64 tokens of one pair (request, KV head, up to 16 of its query heads); the units of all pairs form
+//     one list, cut into ranges, one per CTA and two CTAs per SM (one streams while the other starts or joins).  The lengths
+//     are read on the device, so that a captured step serves every later length; a pair that no range cuts is finished
+//     by its CTA.
 //   * a warp owns 16 tokens of every unit and everything about them: its own ring of asynchronous copies, both
 //     contractions (mma.sync m16n8k16), its own running maximum, sum and output.  Warps meet only where their CTA's
 //     range of a pair ends; until then no barrier keeps a load waiting.
 // mma.sync suffices: per 512 bytes of a token it computes 8192 operations, a tenth of what the SM could do meanwhile.
-// The parts of a pair that ranges cut are joined, in their order, by the CTA that hands in the last one.
+// The parts of a pair that ranges cut are joined, in their order, by the CTA that hands in the last one, or by a launch.
+// 131072 tokens of one request, 4 KV heads: 51 us, of them 45 of streaming (5.9 TB/s); 64 requests of up to 8192 tokens, 8 KV
+// heads, 159 us (6.0 TB/s); 700 tokens 10.5 us, launch and four dependent trips to memory.
 //
-// Where weights are asked for, a second launch turns the logits that the first one left into them:
+// Where weights are asked for, a further launch turns the logits that the first one left into them:
 // out_w_j = w_j + sum_g 2^(s_gj - lse_g).
 #include <algorithm>
 #include <atomic>
@@ -88,46 +91,39 @@ __device__ __forceinline__ unsigned count_units(const DensePagedParams& P, int u
 
 // How the list of units is cut into ranges, one CTA each.  CTAs do not stream alike (64 requests in equal ranges: half of
 // them had finished after 135 us, the last after 160), so the first CTAs get three quarters of an even share and those that
-// take their places ever smaller ranges of the rest.  Few units are cut evenly: what joins the parts costs more.
-constexpr unsigned kDpLeast = 4;         // units of a range, where there are many
+// take their places an eighth each.  Few units are cut evenly: what joins the parts costs more (16 requests, an even share
+// of 29 units: 70 us, 81 with smaller ranges behind).
 constexpr unsigned kDpEven = 48;         // an even share of fewer units than this is not cut further
-constexpr int kDpMostRanges = 5;         // ranges per CTA of an even cut, at most
+constexpr int kDpMostRanges = 3;         // ranges per CTA of an even cut, at most
 struct Ranges {
   unsigned total, ctas, size0, extra;    // the first `ctas` ranges: size0 units, the first `extra` of them one more
-  unsigned size1, count1, size2, count;  // then count1 ranges of size1, then ranges of size2; count: all
+  unsigned size1, count;                 // then ranges of size1; count: all
   __host__ __device__ __forceinline__ Ranges(unsigned units, unsigned most) : total(units) {
     ctas = units < most ? units : most;
     count = ctas;
-    size0 = size1 = size2 = extra = count1 = 0;
+    size0 = size1 = extra = 0;
     if (ctas == 0) return;
     const unsigned even = units / ctas;
+    size0 = even < kDpEven ? even : even - even / 4;
+    const unsigned rest = units - size0 * ctas;
     if (even < kDpEven) {
-      size0 = even;
-      extra = units - even * ctas;
-      return;
+      extra = rest;
+    } else {
+      size1 = (rest + 2 * ctas - 1) / (2 * ctas);
+      count = ctas + (rest + size1 - 1) / size1;
     }
-    size0 = even - even / 4;
-    unsigned rest = units - size0 * ctas;
-    size1 = rest / (2 * ctas) > kDpLeast ? rest / (2 * ctas) : kDpLeast;
-    count1 = (rest + size1 - 1) / size1 < ctas ? (rest + size1 - 1) / size1 : ctas;
-    rest -= rest < count1 * size1 ? rest : count1 * size1;
-    size2 = size1 / 2 > kDpLeast ? size1 / 2 : kDpLeast;
-    count = ctas + count1 + (rest + size2 - 1) / size2;
   }
   __device__ __forceinline__ unsigned start(unsigned range) const {
-    if (range < ctas) return range * size0 + min(range, extra);
-    const unsigned behind = ctas * size0 + extra, r = range - ctas;
-    return min(r < count1 ? behind + r * size1 : behind + count1 * size1 + (r - count1) * size2, total);
+    return range < ctas ? range * size0 + min(range, extra) : min(ctas * size0 + extra + (range - ctas) * size1, total);
   }
   // The range that holds a unit
   __device__ __forceinline__ unsigned of(unsigned unit) const {
     const unsigned longer = extra * (size0 + 1), behind = ctas * size0 + extra;
     if (unit < longer) return unit / (size0 + 1);
-    if (unit < behind) return extra + (unit - longer) / size0;
-    const unsigned r = unit - behind;
-    return r < count1 * size1 ? ctas + r / size1 : ctas + count1 + (r - count1 * size1) / size2;
+    return unit < behind ? extra + (unit - longer) / size0 : ctas + (unit - behind) / size1;
   }
 };
+
 // A place in the list of units: request, pair inside the request, unit inside the pair.
 struct Cursor {
   int b, pair, unit;

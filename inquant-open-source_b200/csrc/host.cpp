@@ -521,7 +521,7 @@ PyObject* paged_attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
     a.q_heads = (int32_t)q->size(1);
     a.dtype = q->scalar_type() == at::kHalf ? INQ_F16 : INQ_BF16;
     a.status = reinterpret_cast<int32_t*>(v[0]);
-    if (counters->device() != q->device() || counters->numel() <= (int64_t)a.requests * a.kv_heads * ((a.q_heads / a.kv_heads + 15) / 16)) return none();
+    if (counters->device() != q->device() || counters->numel() < (int64_t)a.requests * a.kv_heads * ((a.q_heads / a.kv_heads + 15) / 16)) return none();
     a.counters = static_cast<int32_t*>(counters->data_ptr());
     a.workspace_bytes = g_dense.paged_bytes(&a);
     const at::Tensor scratch = bytes_on(*k, a.workspace_bytes);

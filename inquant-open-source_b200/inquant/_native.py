@@ -459,10 +459,10 @@ def decode_counters(device: torch.device, count: int, handle: int | None = None)
 
 
 def launch_counters(device: torch.device, count: int) -> torch.Tensor:
-    """``count`` and one more ``decode_counters`` of the current stream; a call that is being captured gets zeroed ones of its own, because two
+    """``decode_counters`` of the current stream; a call that is being captured gets zeroed ones of its own, because two
     graphs that were captured on one stream may be replayed at the same time."""
     if torch.cuda.is_current_stream_capturing():
-        return torch.zeros(count + 1, dtype=torch.int32, device=device)
+        return torch.zeros(count, dtype=torch.int32, device=device)
     return decode_counters(device, count)
 
 

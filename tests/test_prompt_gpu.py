@@ -99,7 +99,8 @@ def test_one_prompt_of_any_length(q_heads, heads, dim, dtype, lengths):
 
 @pytest.mark.parametrize("q_heads,heads,dim,dtype", SHAPES)
 @pytest.mark.parametrize("lengths,past", [([3, 0, 300, 1, 257, 64], [0] * 6), ([5, 130, 1, 40], [700, 3, 129, 0]),
-                                          ([1] * 70, list(range(70))), ([17] * 33 + [400], [0] * 34), ([0, 0, 9], [0, 50, 0])])
+                                          ([1] * 70, list(range(70))), ([17] * 33 + [400], [0] * 34), ([0, 0, 9], [0, 50, 0]),
+                                          ([3] * 150 + [0, 300] + [1] * 150, [0] * 100 + [20] * 202)])
 @pytest.mark.parametrize("window", [0, 1, 33])
 def test_packed_prompts_behind_histories(q_heads, heads, dim, dtype, lengths, past, window):
     keys = [n + p for n, p in zip(lengths, past)]
