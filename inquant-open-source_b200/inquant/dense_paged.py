@@ -73,7 +73,8 @@ def paged_attention(query: torch.Tensor, key_pages: torch.Tensor, value_pages: t
     A negative length marks an unused row (zeros, nothing stored); a request without tokens gives zeros.  A page id
     outside the pool is never used as an address: its tokens are left out, and ``STATUS_BAD_INDEX`` is set in the
     device's status word, as it is for a length beyond the table.  Two requests may share pages as long as neither
-    stores into them.  Returns the output [B, Hq, D], and with weights ``(output, out_weights)``."""
+    stores into them.  With weights the call takes scratch of 4 bytes per query head and token that the table can
+    hold.  Returns the output [B, Hq, D], and with weights ``(output, out_weights)``."""
     host = N.native_call(query)      # the ordinary call in native code, the rest takes the checks and copies below
     if host is not None:
         device = query.device
@@ -259,6 +260,12 @@ class PromptStep:
         self.new_pages, self.new_offsets = self.pages[is_new], self.offsets[is_new]
         self.done = False
 
+    def _check(self) -> None:
+        if self.done:
+            raise RuntimeError("state mismatch: this step was finished")
+        if [self.cache._slots.get(r) for r in self.requests] != self.slots or [self.cache._held[s] for s in self.slots] != self.past:
+            raise RuntimeError("state mismatch: the cache has changed since this step began")
+
     @torch.no_grad()
     def attend(self, layer: int, query: torch.Tensor, key: torch.Tensor, value: torch.Tensor, *, scale: float | None = None,
                window: int | None = None) -> torch.Tensor:
@@ -266,8 +273,7 @@ class PromptStep:
         ``value`` [T, H, D] are stored.  In a cache with weights, what every key received from the last ``window``
         queries of its request (all of them where it is not given) is added to its weight."""
         cache = self.cache
-        if self.done:
-            raise RuntimeError("state mismatch: this step was finished")
+        self._check()
         total = sum(self.tokens)
         if key.shape != (total, cache.kv_heads, cache.head_dim) or value.shape != key.shape or key.dtype != cache.dtype or value.dtype != key.dtype:
             raise ValueError("Expected key/value [tokens of the step, H, D] of the cache's dtype")
@@ -291,8 +297,7 @@ class PromptStep:
     def finish(self) -> None:
         """Every layer has attended: the requests hold the step's tokens from now on."""
         cache = self.cache
-        if self.done:
-            raise RuntimeError("state mismatch: this step was finished")
+        self._check()
         self.done = True
         for slot, past, n in zip(self.slots, self.past, self.tokens):
             if cache.positions is not None:
@@ -329,7 +334,7 @@ class DensePagedCache:
         shape = (layers, pages, kv_heads, page_tokens, head_dim)
         self.key_pages = torch.empty(shape, dtype=dtype, device=self.device)
         self.value_pages = torch.empty(shape, dtype=dtype, device=self.device)
-        self.block_table = torch.zeros((max_requests, columns), dtype=torch.int32, device=self.device)
+        self.block_table = torch.full((max_requests, columns), -1, dtype=torch.int32, device=self.device)
         self.lengths = torch.full((max_requests,), -1, dtype=torch.int32, device=self.device)
         self.seen = torch.zeros((max_requests,), dtype=torch.int32, device=self.device)
         self.weights = self.positions = None
@@ -385,7 +390,7 @@ class DensePagedCache:
             self._pages[slot].append(self._free_pages.pop())
 
     def _write_table(self) -> None:
-        table = torch.zeros(self.block_table.shape, dtype=torch.int32)
+        table = torch.full(self.block_table.shape, -1, dtype=torch.int32)      # a place that nobody reserved is nobody's page
         for slot, pages in enumerate(self._pages):
             table[slot, :len(pages)] = torch.tensor(pages, dtype=torch.int32)
         self.block_table.copy_(table)
@@ -420,6 +425,8 @@ class DensePagedCache:
     @torch.no_grad()
     def advance(self) -> None:
         """Every layer has decoded: the requests hold one more token each."""
+        if any(self._held[s] + 1 > len(self._pages[s]) * self.page_tokens for s in self._slots.values()):
+            raise RuntimeError("state mismatch: begin_decode reserves the places of a step's tokens")
         if self.positions is not None:
             place = self.lengths.clamp(0, self.positions.shape[3] - 1).long().view(1, -1, 1, 1).expand(self.layers, -1, self.kv_heads, 1)
             self.positions.scatter_(3, place, self.seen.view(1, -1, 1, 1).expand(self.layers, -1, self.kv_heads, 1))

@@ -259,6 +259,18 @@ def test_the_cache_refuses():
     step = c.begin_prompt(["a"], [3])
     with pytest.raises(ValueError):
         step.attend(0, torch.zeros(3, 4, 64, dtype=BF16), torch.zeros(2, 2, 64, dtype=BF16), torch.zeros(2, 2, 64, dtype=BF16))
+    c.release("a")
+    with pytest.raises(RuntimeError, match="changed"):
+        step.finish()
+    c.admit("a")
+    step = c.begin_prompt(["a"], [16])
+    other = c.begin_prompt(["a"], [2])
+    step.finish()
+    with pytest.raises(RuntimeError, match="changed"):
+        other.finish()
+    assert c.block_table[c.slot("a"), 1:].tolist() == [-1] * 4
+    with pytest.raises(RuntimeError, match="begin_decode"):
+        c.advance()
     with pytest.raises(ValueError):
         c.evict(4, sink=4, recent=1)
     with pytest.raises(RuntimeError, match="without weights"):
