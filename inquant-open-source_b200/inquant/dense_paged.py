@@ -239,9 +239,8 @@ class PromptStep:
             raise ValueError("one positive token count per request, every request once")
         self.slots = [cache.slot(r) for r in self.requests]
         self.past = [cache._held[s] for s in self.slots]
-        for slot, past, n in zip(self.slots, self.past, self.tokens):
-            cache._reserve(slot, past + n)
-        cache._write_table()
+        cache._reserve([(slot, past + n) for slot, past, n in zip(self.slots, self.past, self.tokens)])
+        self.reserved = [list(cache._pages[s]) for s in self.slots]
         starts, keys = [0], [0]
         for past, n in zip(self.past, self.tokens):
             starts.append(starts[-1] + n)
@@ -263,7 +262,9 @@ class PromptStep:
     def _check(self) -> None:
         if self.done:
             raise RuntimeError("state mismatch: this step was finished")
-        if [self.cache._slots.get(r) for r in self.requests] != self.slots or [self.cache._held[s] for s in self.slots] != self.past:
+        cache, n = self.cache, [len(p) for p in self.reserved]
+        if [cache._slots.get(r) for r in self.requests] != self.slots or [cache._held[s] for s in self.slots] != self.past \
+                or [cache._pages[s][:k] for s, k in zip(self.slots, n)] != self.reserved:
             raise RuntimeError("state mismatch: the cache has changed since this step began")
 
     @torch.no_grad()
@@ -275,6 +276,8 @@ class PromptStep:
         cache = self.cache
         self._check()
         total = sum(self.tokens)
+        if query.ndim != 3 or query.shape[0] != total:
+            raise ValueError("Expected query [tokens of the step, Hq, D]")
         if key.shape != (total, cache.kv_heads, cache.head_dim) or value.shape != key.shape or key.dtype != cache.dtype or value.dtype != key.dtype:
             raise ValueError("Expected key/value [tokens of the step, H, D] of the cache's dtype")
         key_pages, value_pages = cache.key_pages[layer], cache.value_pages[layer]
@@ -371,6 +374,7 @@ class DensePagedCache:
         self._pages[slot] = []
         self._free_slots.append(slot)
         self._write_lengths()
+        self._write_table()
 
     def tokens(self, request) -> int:
         """Cached tokens of a request; ``seen`` counts the evicted ones too."""
@@ -380,14 +384,18 @@ class DensePagedCache:
     def free_pages(self) -> int:
         return len(self._free_pages)
 
-    def _reserve(self, slot: int, tokens: int) -> None:
-        if tokens > self.max_tokens:
-            raise ValueError(f"a request of {tokens} tokens exceeds max_tokens")
-        need = -(-tokens // self.page_tokens) - len(self._pages[slot])
-        if need > len(self._free_pages):
+    def _reserve(self, wanted: list[tuple[int, int]]) -> None:
+        """Pages for (slot, tokens) pairs: all of them, or none and an error."""
+        for _, tokens in wanted:
+            if tokens > self.max_tokens:
+                raise ValueError(f"a request of {tokens} tokens exceeds max_tokens")
+        need = [max(-(-tokens // self.page_tokens) - len(self._pages[slot]), 0) for slot, tokens in wanted]
+        if sum(need) > len(self._free_pages):
             raise RuntimeError("no free pages: evict tokens or release a request first")
-        for _ in range(need):
-            self._pages[slot].append(self._free_pages.pop())
+        for (slot, _), n in zip(wanted, need):
+            self._pages[slot] += [self._free_pages.pop() for _ in range(n)]
+        if any(need):
+            self._write_table()
 
     def _write_table(self) -> None:
         table = torch.full(self.block_table.shape, -1, dtype=torch.int32)      # a place that nobody reserved is nobody's page
@@ -407,11 +415,7 @@ class DensePagedCache:
 
     def begin_decode(self) -> None:
         """Reserves a place for one more token of every request."""
-        pages = [len(p) for p in self._pages]
-        for slot in self._slots.values():
-            self._reserve(slot, self._held[slot] + 1)
-        if pages != [len(p) for p in self._pages]:
-            self._write_table()
+        self._reserve([(slot, self._held[slot] + 1) for slot in self._slots.values()])
 
     def decode(self, layer: int, query: torch.Tensor, key: torch.Tensor, value: torch.Tensor, *, scale: float | None = None,
                out: torch.Tensor | None = None) -> torch.Tensor:

@@ -279,3 +279,50 @@ def test_the_cache_refuses():
     assert c.free_pages == 5
 
 
+
+
+def test_pages_that_cannot_all_be_had_are_not_reserved_at_all():
+    c = cache(pages=3)
+    a, b = c.admit("a"), c.admit("b")
+    with pytest.raises(RuntimeError, match="no free pages"):
+        c.begin_prompt(["a", "b"], [16, 48])
+    with pytest.raises(ValueError, match="max_tokens"):
+        c.begin_prompt(["a", "b"], [16, 71])
+    assert c.free_pages == 3 and (c.block_table == -1).all()
+    c.begin_prompt(["a", "b"], [16, 32]).finish()
+    with pytest.raises(RuntimeError, match="no free pages"):
+        c.begin_decode()
+    c.release("b")
+    assert (c.block_table[b] == -1).all() and c.block_table[a, 0] >= 0
+    c.begin_decode()
+    assert c.block_table[a, :2].tolist() == c._pages[a] and c.free_pages == 1
+
+
+def test_a_step_does_not_outlive_its_pages(monkeypatch):
+    c = cache()
+    c.admit("a")
+    step = c.begin_prompt(["a"], [16])
+    c.release("a")
+    assert c.admit("a") == step.slots[0]        # the same slot, as empty as it was, and without the step's page
+    rows = torch.zeros(16, 2, 64, dtype=BF16)
+    for call in (step.finish, lambda: step.attend(0, rows, rows, rows)):
+        with pytest.raises(RuntimeError, match="changed"):
+            call()
+    c.admit("b")
+    c.begin_prompt(["b"], [40]).finish()
+    step = c.begin_prompt(["a"], [16])
+    monkeypatch.setattr("inquant.dense_paged.evict_tokens", lambda *_, out_lengths, **__: out_lengths.copy_(c.lengths.clamp(max=32)))
+    c.evict(32, sink=0, recent=0)               # gives back what lies behind every request's tokens
+    with pytest.raises(RuntimeError, match="changed"):
+        step.finish()
+
+
+def test_rows_of_another_length_are_refused_before_they_are_stored():
+    c = cache()
+    c.admit("a")
+    step = c.begin_prompt(["a"], [3])
+    c.key_pages.fill_(7)
+    rows = torch.zeros(3, 2, 64, dtype=BF16)
+    with pytest.raises(ValueError, match="query"):
+        step.attend(0, torch.zeros(2, 4, 64, dtype=BF16), rows, rows)
+    assert (c.key_pages == 7).all()
