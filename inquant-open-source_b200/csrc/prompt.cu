@@ -283,7 +283,13 @@ struct PromptShape {
   static constexpr int kTileBytes = kSlabs * kPrSlab;
   static constexpr int kStages = D == 128 ? 2 : 4;            // K and V tiles in flight
   static constexpr int kTiles = (2 + 2 * kStages) * kTileBytes;
-  static constexpr int kBars = 2 + 4 * kStages + 4 * kStages + 4 + 2 * kPrAhead;
+  static constexpr int kBars = 2 + 4 * kStages + 4 * kStages + 6 + 2 * kPrAhead;
+  // Columns of tensor memory: S_A, S_B, O_A, O_B.  Two outputs of 64 channels leave room for P beside S, so that the next S
+  // is contracted while the softmax of this one runs (four chunks of up to
+  // 700 queries behind 2500 to 7000 keys, 32 heads: 105 us against 119); with
+  // 128 channels P lies over the first half of S.
+  static constexpr bool kApart = D == 64;
+  static constexpr int kOutput = 2 * kPrTile, kP = kApart ? kOutput + 2 * D : 0, kPEach = kApart ? kPrTile / 2 : kPrTile;
   // then: TMEM base, flags; segments; barriers; two sets of three lists of D positions
   static constexpr int kSegmentOffset = kTiles + 64, kBarOffset = kSegmentOffset + kPrAhead * 64, kListOffset = kBarOffset + 8 * kBars;
   static constexpr int kSmem = kListOffset + 2 * 3 * D * 4;
@@ -325,13 +331,14 @@ __global__ void __launch_bounds__(kPrThreads, 1) prompt_kernel(const PromptParam
   volatile int* const any_bad = (volatile int*)(pr_raw + S::kTiles + 16);      // of even and odd segments
   int* const lists = (int*)(pr_raw + S::kListOffset);         // [2][3][D]
   const unsigned bars = smem0 + S::kBarOffset;
-  // Per stage: K and V tiles, V tiles that want cleaning, such tiles cleaned, S and O of tiles A and B; A and B: first half
-  // of P, P; segments.  Barriers of a stage, because a parity alone does not tell phases apart: a stage is not used
+  // Per stage: K and V tiles, V tiles that want cleaning, such tiles cleaned, S and O of tiles A and B; A and B: P,
+  // first half of P, S read (where P lies apart); segments.  Barriers of a stage, because a parity alone does not tell phases apart: a stage is not used
   // again before everyone has seen its last phase.
   const unsigned bar_q = bars, bar_e = bars + 8, bar_k = bars + 16, bar_v = bar_k + 8 * kStages, bar_d = bar_v + 8 * kStages;
   const unsigned bar_c = bar_d + 8 * kStages, bar_s = bar_c + 8 * kStages /* [x][stage] */, bar_o = bar_s + 16 * kStages /* [x][stage] */;
   const unsigned bar_p = bar_o + 16 * kStages, bar_h = bar_p + 16;
-  const unsigned bar_g = bar_h + 16, bar_gfree = bar_g + 8 * kPrAhead;
+  const unsigned bar_r = bar_h + 16;
+  const unsigned bar_g = bar_r + 16, bar_gfree = bar_g + 8 * kPrAhead;
   const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
   follow_stream();       // cu_q and cu_k may come from the launch before this one
   if (smem0 & 1023u) {
@@ -360,6 +367,7 @@ __global__ void __launch_bounds__(kPrThreads, 1) prompt_kernel(const PromptParam
     for (int i = 0; i < 2; ++i) {
       tc_bar_init(bar_p + 8 * i, kPrTile);
       tc_bar_init(bar_h + 8 * i, kPrTile);
+      tc_bar_init(bar_r + 8 * i, kPrTile);
     }
 #pragma unroll
     for (int i = 0; i < kPrAhead; ++i) {
@@ -372,7 +380,7 @@ __global__ void __launch_bounds__(kPrThreads, 1) prompt_kernel(const PromptParam
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const unsigned tmem = *tmem_base_p;      // S_A 0..127, S_B 128..255 (P over their first 64), O_A 256.., O_B 384..
+  const unsigned tmem = *tmem_base_p;
   allow_next();
   auto wait = [&](unsigned mbar, unsigned parity) { tc_wait(mbar, parity, abort_flag); };   // goes on in either case
   // Segment n, the same for a whole warp; an invalid one behind the last, and once a wait has given up.
@@ -535,7 +543,7 @@ __global__ void __launch_bounds__(kPrThreads, 1) prompt_kernel(const PromptParam
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
             const int kk = 4 * half + k;
-            tc_mma_ta(tmem + 2 * kPrTile + x * kPrTile, tmem + x * kPrTile + kk * 8, tc_desc(v + kk * 2048, kPrSlab, 1024), idesc_o,
+            tc_mma_ta(tmem + S::kOutput + x * D, tmem + S::kP + x * S::kPEach + kk * 8, tc_desc(v + kk * 2048, kPrSlab, 1024), idesc_o,
                       (!first || kk > 0) ? 1u : 0u);
           }
           if (half) tc_commit(bar_o + 8 * (x * kStages + u % kStages));
@@ -543,7 +551,7 @@ __global__ void __launch_bounds__(kPrThreads, 1) prompt_kernel(const PromptParam
       };
       unsigned count[2] = {0, 0}, v_parity = 0, d_parity = 0, u = 0;
       auto contract_o = [&](int x, bool first) {
-        wait(bar_h + 8 * x, count[x] & 1u);     // S_x read, the first half of P_x written, the rows of the segment before stored
+        wait(bar_h + 8 * x, count[x] & 1u);     // S_x read where P_x lies over it, the first half of P_x written, the rows of the segment before stored
         tc_fence_after();
         issue_o(x, u, first, 0);
         wait(bar_p + 8 * x, count[x] & 1u);     // the second half
@@ -563,15 +571,20 @@ __global__ void __launch_bounds__(kPrThreads, 1) prompt_kernel(const PromptParam
         int t = 0;
         while (true) {
           const unsigned st = u % kStages, bit = 1u << st;
-          if (t < T.t_dark) {
-            wait(bar_v + 8 * st, v_parity & bit ? 1u : 0u);
-            v_parity ^= bit;
-          } else {
-            wait(bar_c + 8 * st, d_parity & bit ? 1u : 0u);
-            d_parity ^= bit;
+          const bool dark = t >= T.t_dark, a_now = t < T.n_a, b_now = t < T.n_b, first = t == 0;
+          auto wait_v = [&]() {
+            if (!dark) {
+              wait(bar_v + 8 * st, v_parity & bit ? 1u : 0u);
+              v_parity ^= bit;
+            } else {
+              wait(bar_c + 8 * st, d_parity & bit ? 1u : 0u);
+              d_parity ^= bit;
+            }
+          };
+          if constexpr (!S::kApart) {
+            wait_v();
+            if (a_now) contract_o(0, first);
           }
-          const bool b_now = t < T.n_b, b_first = t == 0;
-          if (t < T.n_a) contract_o(0, t == 0);
           // the step behind this one, perhaps of another segment
           bool more = true;
           if (++t == g.n_t) {
@@ -583,12 +596,23 @@ __global__ void __launch_bounds__(kPrThreads, 1) prompt_kernel(const PromptParam
           if (more) {
             if (t == 0) wait(bar_q, (unsigned)n & 1u);
             wait(bar_k + 8 * ((u + 1) % kStages), ((u + 1) / kStages) & 1u);
+            if constexpr (S::kApart)
+              if (a_now) wait(bar_r, count[0] & 1u);
             tc_fence_after();
             if (t < next.n_a) issue_s(0, u + 1);
           }
-          if (b_now) contract_o(1, b_first);
+          if constexpr (S::kApart) {
+            wait_v();
+            if (a_now) contract_o(0, first);
+            if (more && b_now) {
+              wait(bar_r + 8, count[1] & 1u);
+              tc_fence_after();
+            }
+            if (more && t < next.n_b) issue_s(1, u + 1);
+          }
+          if (b_now) contract_o(1, first);
           if (!more) break;
-          if (t < next.n_b) issue_s(1, u + 1);
+          if (!S::kApart && t < next.n_b) issue_s(1, u + 1);
           if (t == 0) T = next;
           ++u;
         }
@@ -670,7 +694,7 @@ __global__ void __launch_bounds__(kPrThreads, 1) prompt_kernel(const PromptParam
     const int x = warp >> 2;                       // 0: tile A, 1: tile B
     const int row = tid & (kPrTile - 1);           // query row inside the tile = TMEM lane
     const unsigned lane_field = (unsigned)((warp & 3) * 32) << 16;
-    const unsigned tS = tmem + lane_field + x * kPrTile, tO = tmem + lane_field + 2 * kPrTile + x * kPrTile;
+    const unsigned tS = tmem + lane_field + x * kPrTile, tO = tmem + lane_field + S::kOutput + x * D, tP = tmem + lane_field + S::kP + x * S::kPEach;
     const unsigned my_s = bar_s + 8 * x * kStages, my_p = bar_p + 8 * x, my_o = bar_o + 8 * x * kStages;
     unsigned u = 0, parity = 0;                    // the segment's first step; a bit per stage: the next parity of this tile's barriers
     int n = 0;
@@ -684,8 +708,8 @@ __global__ void __launch_bounds__(kPrThreads, 1) prompt_kernel(const PromptParam
 
       for (int t = 0; t < n_x; ++t) {
         const int kv0 = (g.t_lo + t) * kPrTile;
-        // S(t) is complete; the contractions run in issue order, so PV(t-1) is complete as well:
-        // the columns of P may be overwritten by S and O may be rescaled
+        // S(t) is complete; the contractions run in issue order, so that PV(t-1) is complete as well, if it was issued first:
+        // P may be overwritten and O may be rescaled
         const unsigned st = (u + t) % kStages, bit = 1u << st;
         wait(my_s + 8 * st, parity & bit ? 1u : 0u);
         parity ^= bit;
@@ -695,6 +719,10 @@ __global__ void __launch_bounds__(kPrThreads, 1) prompt_kernel(const PromptParam
         for (int q = 0; q < 4; ++q) tc_ld32(tS + 32 * q, v[q]);
 #pragma unroll
         for (int q = 0; q < 4; ++q) tc_wait_ld32(v[q]);
+        if constexpr (S::kApart) {
+          tc_fence_before();
+          pf_arrive(bar_r + 8 * x);
+        }
         if (kv0 + kPrTile - 1 > diag0) {
 #pragma unroll
           for (int q = 0; q < 4; ++q)
@@ -710,6 +738,11 @@ __global__ void __launch_bounds__(kPrThreads, 1) prompt_kernel(const PromptParam
           for (int c = 1; c < 32; ++c) top[q] = fmaxf(top[q], __uint_as_float(v[q][c]));
         }
         const float smax = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+        if (S::kApart && t > 0) {      // S(t) was issued before PV(t-1)
+          const unsigned last = (u + t - 1) % kStages;
+          wait(my_o + 8 * last, (parity >> last) & 1u ? 0u : 1u);
+          tc_fence_after();
+        }
         const bool raise = smax * P.scale_log2e > m_ref + kPrSlack;
         if (__any_sync(0xffffffffu, raise)) {
           // rare after the first tile: bring the running sum and the output accumulator to the new reference maximum
@@ -743,7 +776,7 @@ __global__ void __launch_bounds__(kPrThreads, 1) prompt_kernel(const PromptParam
             sum2 = pf_add2(sum2, pf_pair(e0, e1));
             packed[c >> 1] = pf_pack2<QT>(e0, e1);
           }
-          tc_st16(tS + 16 * q, packed);
+          tc_st16(tP + 16 * q, packed);
           if (q == 1) {   // S has been read, the first half of P is in tensor memory: the contraction with V starts
             tc_wait_st();
             tc_fence_before();
