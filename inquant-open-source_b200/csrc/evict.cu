@@ -11,6 +11,7 @@
 // histograms added over distributed shared memory.  It writes the lists of free places and of tokens that move.
 // Its passes depend on one another, which is what bounds it: 15 us for 256 rows of 2304 tokens, 24 for 16 of 32768.
 // evict_move_kernel moves the rows of K and V: 4 D elements read and written per token, which is what bounds it (67 MB 10 us).
+// Where many short rows are selected, the selecting CTAs move them instead, and one row's moves overlap the next's passes.
 #include <cooperative_groups.h>
 
 #include <algorithm>
@@ -34,6 +35,7 @@ struct EvictParams {
   long long pages, capacity;
   int requests, kv_heads, page_tokens, page_shift, budget, sink, recent, row_bytes;
   long long list_columns;
+  int moves_here;
   int* lists;          // per row: count, then up to list_columns free places, then as many tokens that move
   int* status;
 };
@@ -62,6 +64,43 @@ __device__ __forceinline__ int warps_before(int mine, int& all, int* scratch /* 
   return before;
 }
 
+// Moves tokens i0 .. of a row's lists, eight at once, by a warp that asks for all of them before it writes the first: half of
+// its lanes the key rows, the others the value rows, 16 bytes each.
+constexpr int kEvMoveEach = 8;
+__device__ __forceinline__ void move_tokens(const EvictParams& P, int b, int h, const int* list, int i0, int count) {
+  const int lane = threadIdx.x & 31;
+  // lane 2 i (+ 1) finds the page and offset of where token i goes (comes from), and moves its weight and position
+  const int i = i0 + (lane >> 1);
+  const bool some = lane < 2 * kEvMoveEach && i < count;
+  const int j = some ? __ldcg(list + 1 + (lane & 1 ? P.list_columns : 0) + i) : 0;
+  const int column = P.page_shift >= 0 ? j >> P.page_shift : j / P.page_tokens, o = j - column * P.page_tokens;
+  int page = some ? __ldg(P.table + b * P.table_stride + column) : -1;
+  if (some && (page < 0 || page >= P.pages)) {
+    atomicOr(P.status, INQ_STATUS_BAD_INDEX);
+    page = -1;
+  }
+  const int place = __shfl_xor_sync(0xffffffffu, j, 1);
+  if (some && (lane & 1)) {
+    P.out_weights[b * P.ow_sb + h * P.ow_sh + place] = P.weights[b * P.w_sb + h * P.w_sh + j];
+    P.out_positions[b * P.op_sb + h * P.op_sh + place] = P.positions[b * P.p_sb + h * P.p_sh + j];
+  }
+  const bool key = lane < 16;
+  const long long sp = key ? P.k_sp : P.v_sp, st = key ? P.k_st : P.v_st;
+  char* const base = (char*)(key ? P.k : P.v) + 2 * h * (key ? P.k_sh : P.v_sh) + (lane & 15) * 16;
+  const bool mine = (lane & 15) * 16 < P.row_bytes;
+  uint4 rows[kEvMoveEach];
+#pragma unroll
+  for (int n = 0; n < kEvMoveEach; ++n) {
+    const int to = __shfl_sync(0xffffffffu, page, 2 * n), from = __shfl_sync(0xffffffffu, page, 2 * n + 1), from_o = __shfl_sync(0xffffffffu, o, 2 * n + 1);
+    if (to >= 0 && from >= 0 && mine) rows[n] = __ldcs((const uint4*)(base + 2 * (from * sp + from_o * st)));
+  }
+#pragma unroll
+  for (int n = 0; n < kEvMoveEach; ++n) {
+    const int to = __shfl_sync(0xffffffffu, page, 2 * n), from = __shfl_sync(0xffffffffu, page, 2 * n + 1), to_o = __shfl_sync(0xffffffffu, o, 2 * n);
+    if (to >= 0 && from >= 0 && mine) *(uint4*)(base + 2 * (to * sp + to_o * st)) = rows[n];
+  }
+}
+
 // KEYS: tokens per thread whose keys stay in registers over all passes; a slice of more is read anew for each.
 template <int KEYS>
 __global__ void __launch_bounds__(kEvThreads, KEYS <= 5 ? 2 : 1) evict_select_kernel(const EvictParams P) {
@@ -78,6 +117,7 @@ __global__ void __launch_bounds__(kEvThreads, KEYS <= 5 ? 2 : 1) evict_select_ke
   const int length = (int)min(max(asked, 0LL), P.capacity), budget = P.budget;
   if (asked > P.capacity && row % P.kv_heads == 0 && me == 0 && tid == 0) atomicOr(P.status, INQ_STATUS_BAD_INDEX);
   const int left = min(length, budget);
+  if (P.moves_here && h == 0 && me == 0 && tid == 0) P.out_lengths[b] = (int)min(min(asked, (long long)budget), P.capacity);
   const float* const w = P.weights + b * P.w_sb + h * P.w_sh;
   const int* const pos = P.positions + b * P.p_sb + h * P.p_sh;
   float* const out_w = P.out_weights + b * P.ow_sb + h * P.ow_sh;
@@ -249,49 +289,21 @@ __global__ void __launch_bounds__(kEvThreads, KEYS <= 5 ? 2 : 1) evict_select_ke
     moves += group_moves;
   }
   if (me == ctas - 1 && tid == 0) list[0] = moves;
-  cluster.sync();       // the counts of a CTA are read until here
+  cluster.sync();       // the counts of a CTA are read until here, and the lists of the cluster are complete
+  if (!P.moves_here) return;
+  const int count = __ldcg(list);
+  for (int i0 = (me * (kEvThreads / 32) + warp) * kEvMoveEach; i0 < count; i0 += ctas * (kEvThreads / 32) * kEvMoveEach)
+    move_tokens(P, b, h, list, i0, count);
 }
 
-// A warp moves eight tokens at once, and asks for all of them before it writes the first: half of its lanes the key rows, the
-// others the value rows, 16 bytes each.
-constexpr int kEvMoveThreads = 256, kEvMoveEach = 8, kEvMoveTokens = kEvMoveThreads / 32 * kEvMoveEach;      // tokens of a block
+constexpr int kEvMoveThreads = 256, kEvMoveTokens = kEvMoveThreads / 32 * kEvMoveEach;      // tokens of a block
 __global__ void __launch_bounds__(kEvMoveThreads) evict_move_kernel(const EvictParams P) {
   follow_stream();
-  const int row = blockIdx.x, b = row / P.kv_heads, h = row % P.kv_heads, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int row = blockIdx.x, b = row / P.kv_heads, h = row % P.kv_heads, warp = threadIdx.x >> 5;
   const int* const list = P.lists + row * (2 * P.list_columns + 1);
   if (blockIdx.y == 0 && h == 0 && threadIdx.x == 0) P.out_lengths[b] = (int)min((long long)min(P.lengths[b], P.budget), P.capacity);
   const int count = __ldcg(list), i0 = blockIdx.y * kEvMoveTokens + warp * kEvMoveEach;
-  if (i0 >= count) return;
-  // lane 2 i (+ 1) finds the page and offset of where token i goes (comes from), and moves its weight and position
-  const int i = i0 + (lane >> 1);
-  const bool some = lane < 2 * kEvMoveEach && i < count;
-  const int j = some ? __ldcg(list + 1 + (lane & 1 ? P.list_columns : 0) + i) : 0;
-  const int column = P.page_shift >= 0 ? j >> P.page_shift : j / P.page_tokens, o = j - column * P.page_tokens;
-  int page = some ? __ldg(P.table + b * P.table_stride + column) : -1;
-  if (some && (page < 0 || page >= P.pages)) {
-    atomicOr(P.status, INQ_STATUS_BAD_INDEX);
-    page = -1;
-  }
-  const int place = __shfl_xor_sync(0xffffffffu, j, 1);
-  if (some && (lane & 1)) {
-    P.out_weights[b * P.ow_sb + h * P.ow_sh + place] = P.weights[b * P.w_sb + h * P.w_sh + j];
-    P.out_positions[b * P.op_sb + h * P.op_sh + place] = P.positions[b * P.p_sb + h * P.p_sh + j];
-  }
-  const bool key = lane < 16;
-  const long long sp = key ? P.k_sp : P.v_sp, st = key ? P.k_st : P.v_st;
-  char* const base = (char*)(key ? P.k : P.v) + 2 * h * (key ? P.k_sh : P.v_sh) + (lane & 15) * 16;
-  const bool mine = (lane & 15) * 16 < P.row_bytes;
-  uint4 rows[kEvMoveEach];
-#pragma unroll
-  for (int n = 0; n < kEvMoveEach; ++n) {
-    const int to = __shfl_sync(0xffffffffu, page, 2 * n), from = __shfl_sync(0xffffffffu, page, 2 * n + 1), from_o = __shfl_sync(0xffffffffu, o, 2 * n + 1);
-    if (to >= 0 && from >= 0 && mine) rows[n] = __ldcs((const uint4*)(base + 2 * (from * sp + from_o * st)));
-  }
-#pragma unroll
-  for (int n = 0; n < kEvMoveEach; ++n) {
-    const int to = __shfl_sync(0xffffffffu, page, 2 * n), from = __shfl_sync(0xffffffffu, page, 2 * n + 1), to_o = __shfl_sync(0xffffffffu, o, 2 * n);
-    if (to >= 0 && from >= 0 && mine) *(uint4*)(base + 2 * (to * sp + to_o * st)) = rows[n];
-  }
+  if (i0 < count) move_tokens(P, b, h, list, i0, count);
 }
 
 }  // namespace inq
@@ -337,6 +349,14 @@ extern "C" int inq_evict_tokens(const inq_evict_args_t* a, inq_stream_t stream_)
   // slices of a row: while they fill the SMs and hold 2048 tokens at least
   int ctas = 1;
   while (ctas < kEvMaxCluster && rows * ctas * 2 <= 2 * n_sm && P.capacity / (2 * ctas) >= 2048) ctas *= 2;
+  const long long slice = (P.capacity + ctas - 1) / ctas;
+  // As many tokens move as places fall free, at most, and as there are behind the budget.  Where the rows fill the SMs and two
+  // CTAs fit on one, few moves are done at once, beside the selection of other rows (256 rows of 2304 tokens, 256 of them
+  // evicted: 24.7 us against 26.8; 512 rows of 1024, a half evicted: 48.6 against 50.9).  Else they take a launch of their own,
+  // over all SMs (256 rows of 4096, one CTA per SM: 46 us against 49.5; 16 of 32768 to 8192: 42.6 against 54).  Other
+  // heads may still read a length when one writes it, so that it is not written in place.
+  const long long most = std::min<long long>(P.budget, std::max<long long>(P.capacity - P.budget, 1));
+  P.moves_here = slice <= 5 * kEvThreads && rows * ctas > n_sm && most <= 4LL * ctas * (kEvThreads / 32) * kEvMoveEach && P.out_lengths != P.lengths;
   cudaStream_t stream = (cudaStream_t)stream_;
   {
     cudaLaunchAttribute attrs[2];
@@ -352,14 +372,11 @@ extern "C" int inq_evict_tokens(const inq_evict_args_t* a, inq_stream_t stream_)
     config.attrs = attrs;
     config.numAttrs = 2;
     // the keys of a slice in registers where 16 per thread do, in fewer where a power of two and some slack fit
-    const long long slice = (P.capacity + ctas - 1) / ctas;
     INQ_CUDA_CHECK(slice <= 5 * kEvThreads ? cudaLaunchKernelEx(&config, evict_select_kernel<5>, P)
                                            : slice <= 9 * kEvThreads ? cudaLaunchKernelEx(&config, evict_select_kernel<9>, P)
                                                                      : cudaLaunchKernelEx(&config, evict_select_kernel<16>, P));
   }
-  // as many tokens move as places fall free, at most, and as there are behind the budget
-  const long long most = std::min<long long>(P.budget, std::max<long long>(P.capacity - P.budget, 1));
-  const unsigned blocks = (unsigned)((most + kEvMoveTokens - 1) / kEvMoveTokens);
-  INQ_CUDA_CHECK(launch_following(evict_move_kernel, dim3((unsigned)rows, blocks), kEvMoveThreads, 0, stream, P));
+  if (!P.moves_here) INQ_CUDA_CHECK(launch_following(evict_move_kernel, dim3((unsigned)rows, (unsigned)((most + kEvMoveTokens - 1) / kEvMoveTokens)),
+                                                     kEvMoveThreads, 0, stream, P));
   return INQ_OK;
 }

@@ -274,6 +274,8 @@ def check_evict(pool, heads, lengths, seen, weights, positions, budget, sink, re
             for b, n in enumerate(lengths)]
     w0, p0, n0 = weights.clone(), positions.clone(), ints(lengths)
     into = dict(out_weights=weights, out_positions=positions, out_lengths=n0) if in_place else {}
+    if in_place == "state":
+        del into["out_lengths"]
     n, w, p = evict_tokens(pool.keys, pool.values, pool.table, n0, weights, positions, ints(seen), budget, sink=sink, recent=recent, **into)
     assert n.tolist() == [min(x, budget) for x in lengths]
     for b in range(len(lengths)):
@@ -322,6 +324,15 @@ def test_eviction_of_other_shapes(heads, dim, dtype):
     pool = Pool(lengths, heads, dim, 32, dtype, seed=13)
     weights, positions, seen = eviction_state(lengths, heads, pool.columns * 32, 14)
     check_evict(pool, heads, lengths, seen, weights, positions, 512, 4, 64)
+
+
+@pytest.mark.parametrize("budget", [1, 96, 500, 600])
+@pytest.mark.parametrize("page,in_place", [(16, False), (24, "state"), (64, True)])
+def test_eviction_of_many_short_rows(budget, page, in_place):
+    lengths = [[1200, 0, 97, 513, -1, budget, budget + 1, 1100 + i][i % 8] for i in range(40)]
+    pool = Pool(lengths, 8, 64, page, torch.float16, seed=23)
+    weights, positions, seen = eviction_state(lengths, 8, pool.columns * page, 24)
+    check_evict(pool, 8, lengths, seen, weights, positions, budget, 0, 1, in_place)
 
 
 @pytest.mark.parametrize("value", [0.0, 1.5, -2.0, float("nan"), float("inf"), 1e-42])
