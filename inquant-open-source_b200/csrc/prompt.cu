@@ -285,9 +285,8 @@ struct PromptShape {
   static constexpr int kTiles = (2 + 2 * kStages) * kTileBytes;
   static constexpr int kBars = 2 + 4 * kStages + 4 * kStages + 6 + 2 * kPrAhead;
   // Columns of tensor memory: S_A, S_B, O_A, O_B.  Two outputs of 64 channels leave room for P beside S, so that the next S
-  // is contracted while the softmax of this one runs (four chunks of up to
-  // 700 queries behind 2500 to 7000 keys, 32 heads: 105 us against 119); with
-  // 128 channels P lies over the first half of S.
+  // is contracted while the softmax of this one runs (four chunks of up to 700 queries behind 2500 to 7000 keys, 32 heads:
+  // 105 us against 119); with 128 channels P lies over the first half of S.
   static constexpr bool kApart = D == 64;
   static constexpr int kOutput = 2 * kPrTile, kP = kApart ? kOutput + 2 * D : 0, kPEach = kApart ? kPrTile / 2 : kPrTile;
   // then: TMEM base, flags; segments; barriers; two sets of three lists of D positions
@@ -332,8 +331,8 @@ __global__ void __launch_bounds__(kPrThreads, 1) prompt_kernel(const PromptParam
   int* const lists = (int*)(pr_raw + S::kListOffset);         // [2][3][D]
   const unsigned bars = smem0 + S::kBarOffset;
   // Per stage: K and V tiles, V tiles that want cleaning, such tiles cleaned, S and O of tiles A and B; A and B: P,
-  // first half of P, S read (where P lies apart); segments.  Barriers of a stage, because a parity alone does not tell phases apart: a stage is not used
-  // again before everyone has seen its last phase.
+  // first half of P, S read (where P lies apart); segments.  Barriers of a stage, because a parity alone does not tell
+  // phases apart: a stage is not used again before everyone has seen its last phase.
   const unsigned bar_q = bars, bar_e = bars + 8, bar_k = bars + 16, bar_v = bar_k + 8 * kStages, bar_d = bar_v + 8 * kStages;
   const unsigned bar_c = bar_d + 8 * kStages, bar_s = bar_c + 8 * kStages /* [x][stage] */, bar_o = bar_s + 16 * kStages /* [x][stage] */;
   const unsigned bar_p = bar_o + 16 * kStages, bar_h = bar_p + 16;
