@@ -30,6 +30,7 @@
 namespace inq {
 
 constexpr int kPrThreads = 384;              // 8 softmax warps, the MMA warp, the TMA warp, one that cleans value tiles, one that deals
+constexpr int kPrSoftmaxWarps = 8;
 constexpr int kPrLaunchRegs = 168, kPrIssueRegs = 72, kPrSoftmaxRegs = (3 * kPrLaunchRegs - kPrIssueRegs) / 2;
 constexpr int kPrTile = 128;                 // rows per tile
 constexpr int kPrRows = 2 * kPrTile;         // rows per item (tiles A and B)
@@ -289,7 +290,7 @@ struct PromptShape {
   // 105 us against 119); with 128 channels P lies over the first half of S.
   static constexpr bool kApart = D == 64;
   static constexpr int kOutput = 2 * kPrTile, kP = kApart ? kOutput + 2 * D : 0, kPEach = kApart ? kPrTile / 2 : kPrTile;
-  // then: TMEM base, flags; segments; barriers; two sets of three lists of D positions
+  // then: TMEM base, flags, the softmax warps' progress; segments; barriers; two sets of three lists of D positions
   static constexpr int kSegmentOffset = kTiles + 64, kBarOffset = kSegmentOffset + kPrAhead * 64, kListOffset = kBarOffset + 8 * kBars;
   static constexpr int kSmem = kListOffset + 2 * 3 * D * 4;
 };
@@ -326,8 +327,8 @@ __global__ void __launch_bounds__(kPrThreads, 1) prompt_kernel(const PromptParam
   const unsigned sQ = smem0, sKb = smem0 + 2 * kTileBytes, sVb = sKb + kStages * kTileBytes;
   unsigned* const tmem_base_p = (unsigned*)(pr_raw + S::kTiles);
   volatile int* const abort_flag = (volatile int*)(pr_raw + S::kTiles + 4);
-  int* const ended = (int*)(pr_raw + S::kTiles + 8);          // softmax warps that are done with a segment, over all segments
   volatile int* const any_bad = (volatile int*)(pr_raw + S::kTiles + 16);      // of even and odd segments
+  volatile int* const ended = (volatile int*)(pr_raw + S::kTiles + 32);        // per softmax warp: segments that it is done with
   int* const lists = (int*)(pr_raw + S::kListOffset);         // [2][3][D]
   const unsigned bars = smem0 + S::kBarOffset;
   // Per stage: K and V tiles, V tiles that want cleaning, such tiles cleaned, S and O of tiles A and B; A and B: P,
@@ -348,7 +349,9 @@ __global__ void __launch_bounds__(kPrThreads, 1) prompt_kernel(const PromptParam
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(tc_smem(tmem_base_p)), "r"(512) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   } else if (warp == 9 && lane == 0) {
-    *abort_flag = *ended = any_bad[0] = any_bad[1] = 0;
+    *abort_flag = any_bad[0] = any_bad[1] = 0;
+#pragma unroll
+    for (int i = 0; i < kPrSoftmaxWarps; ++i) ended[i] = 0;
     tc_bar_init(bar_q, 1);
     tc_bar_init(bar_e, 1);
 #pragma unroll
@@ -371,7 +374,7 @@ __global__ void __launch_bounds__(kPrThreads, 1) prompt_kernel(const PromptParam
 #pragma unroll
     for (int i = 0; i < kPrAhead; ++i) {
       tc_bar_init(bar_g + 8 * i, 1);
-      tc_bar_init(bar_gfree + 8 * i, 11);       // the softmax warps, the MMA, TMA and cleaning warps
+      tc_bar_init(bar_gfree + 8 * i, kPrSoftmaxWarps + 3);       // the softmax warps, the MMA, TMA and cleaning warps
     }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -624,9 +627,19 @@ __global__ void __launch_bounds__(kPrThreads, 1) prompt_kernel(const PromptParam
       for (Segment g = segment(0); g.valid; g = segment(++n)) {
         const SegmentTiles T(g);
         int* const first_bad = lists + (n & 1) * 3 * D;
-        // The lists were those of the segment before the last: nothing changes there before all softmax warps have ended that.
+        // The lists were those of the segment before the last: nothing changes there before every softmax warp has ended that.
+        // A word per warp, because a sum over them does not tell: where tile A (or a tile B without rows) is a segment
+        // ahead, its warps would make up for those that still read.  Half a second at most.
         auto others_ended = [&]() {
-          for (int it = 0; it < kTcTries && *(volatile int*)ended < 8 * (n - 1) && *abort_flag == 0; ++it) __nanosleep(64);
+          for (int it = 0; *abort_flag == 0; ++it) {
+            int least = ended[0];
+#pragma unroll
+            for (int i = 1; i < kPrSoftmaxWarps; ++i) least = min(least, ended[i]);
+            if (least >= n - 1) break;
+            if (it == kTcTries) *abort_flag = 1;
+            __nanosleep(it < 64 ? 64 : 2048);
+          }
+          __threadfence_block();
         };
         if (T.t_dark < g.n_t && (held >> (n & 1)) & 1u) {
           others_ended();
@@ -858,7 +871,10 @@ __global__ void __launch_bounds__(kPrThreads, 1) prompt_kernel(const PromptParam
       }
       tc_fence_before();      // O has been read: the arrivals of the next segment let it be overwritten
       __syncwarp();
-      if (lane == 0) atomicAdd(ended, 1);
+      if (lane == 0) {
+        __threadfence_block();      // the lists have been read
+        ended[warp] = n + 1;
+      }
     }
   }
   tc_fence_before();

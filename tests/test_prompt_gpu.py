@@ -278,3 +278,45 @@ def test_agrees_with_the_attention_of_one_sequence():
     single = prefill_attention(*(t.transpose(0, 1).unsqueeze(0) for t in (q, k, v)))[0].transpose(0, 1)
     out, _ = prompt_attention(q, k, v, ints([0, 700]), ints([0, 1500]))
     assert (out.float() - single.float()).abs().max() <= 2 * unit(q.dtype) * v.abs().max().float()
+
+
+@pytest.mark.parametrize("dim,dtype", [(128, torch.bfloat16), (64, torch.float16)])
+@pytest.mark.parametrize("lengths", [[100, 300, 128, 260, 17, 290, 129, 200] * 7, [60, 1100, 90, 500, 256, 30] * 5])
+def test_values_that_are_not_finite_stay_with_the_rows_that_see_them(dim, dtype, lengths):
+    """Many items behind one another in a CTA, with and without a second tile, some with values that are not finite: what one
+    item found is neither lost to its own rows nor handed to those of another."""
+    from inquant.prompt import prompt_attention
+    heads, q_heads = 8, 32
+    q, k, v = states(lengths, lengths, q_heads, heads, dim, dtype, seed=21)
+    clean, clean_lse, _ = check(q, k, v, lengths, lengths)
+    first = starts(lengths)
+    cu = ints(first)
+    specials = torch.tensor([math.inf, -math.inf, math.nan])
+    where = torch.zeros(sum(lengths), dtype=torch.long, device=DEV)       # first row of the row's sequence
+    for b, n in enumerate(lengths):
+        where[first[b]:first[b] + n] = first[b]
+    row = torch.arange(sum(lengths), device=DEV)
+    g = torch.Generator().manual_seed(22)
+    for turn in range(6):
+        values = v.clone()
+        kinds = [torch.zeros(v.shape, dtype=torch.bool, device=DEV) for _ in specials]
+        for b, n in enumerate(lengths):
+            if (b + turn) % 3 == 0:
+                continue        # nothing to find between two that have something
+            for _ in range(4):
+                at, h, c, kind = (int(torch.randint(m, (1,), generator=g)) for m in (n, heads, dim, 3))
+                values[first[b] + at, h, c] = specials[kind]
+                for i in range(3):
+                    kinds[i][first[b] + at, h, c] = i == kind
+        seen = []
+        for kind in kinds:      # whether a row's sequence has one at or before the row
+            total = torch.cat([torch.zeros_like(kind[:1], dtype=torch.int32), kind.to(torch.int32).cumsum(0, dtype=torch.int32)])
+            seen.append((total[row + 1] > total[where]).repeat_interleave(q_heads // heads, 1))
+        plus, minus, nan = seen
+        want = torch.where(plus, math.inf, clean.float())
+        want = torch.where(minus, -math.inf, want)
+        want = torch.where(nan | (plus & minus), math.nan, want)
+        # a channel's result depends on that channel's values alone: where a row sees nothing of the kind it is bit by bit what it was
+        out, lse = prompt_attention(q, k, values, cu)
+        assert torch.equal(out.float().nan_to_num(1e30), want.nan_to_num(1e30)), turn
+        assert torch.equal(torch.isnan(out), torch.isnan(want)) and torch.equal(lse, clean_lse)
