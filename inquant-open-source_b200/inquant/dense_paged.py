@@ -307,6 +307,7 @@ class PromptStep:
                 cache.positions[:, slot, :, past:past + n] = torch.arange(cache._seen[slot], cache._seen[slot] + n, device=cache.device, dtype=torch.int32)
             cache._held[slot] = past + n
             cache._seen[slot] += n
+            cache._changes[slot] += 1
         cache._write_lengths()
 
 
@@ -314,11 +315,12 @@ class DensePagedCache:
     """Uncompressed paged cache of several requests and layers, with an optional budget per KV head.
 
     ``begin_prompt(requests, tokens)`` opens a step of packed prompts (``attend`` per layer, then ``finish``);
-    ``decode(layer, query, key, value)`` attends with one token of every slot, ``advance()`` behind the last layer takes
-    these tokens into account; ``evict(budget)`` cuts every request to its budget and gives back the pages that fell
+    ``begin_decode()`` opens a step of one token per request, ``decode(layer, query, key, value)`` attends with them, and
+    ``advance()`` behind the last layer takes them into account, unless the cache has changed in between;
+    ``evict(budget)``, between steps, cuts every request to its budget and gives back the pages that fell
     empty.  Rows of a decode call are slots (``slot(request)``); slots without a request give zeros.  ``lengths``,
     ``seen`` and ``block_table`` live on the device, so that decode calls can be captured into a CUDA graph; pages are
-    handed out by ``advance``, which is not captured.
+    handed out by ``begin_decode``, which is not captured, and neither is ``advance``.
 
     ``gather`` returns the tokens of a request as dense rows, for instance for ``InQuantCache.update``: what is left after
     an eviction can be coded like any other cache."""
@@ -349,6 +351,8 @@ class DensePagedCache:
         self._free_pages = list(range(pages))[::-1]
         self._pages: list[list[int]] = [[] for _ in range(max_requests)]
         self._held, self._seen = [0] * max_requests, [0] * max_requests
+        self._changes = [0] * max_requests                       # of a slot: all that a decode step must not meet on its way
+        self._step: dict[int, int] | None = None                 # slots of the open decode step, as many changes as they had had
 
     # ------------------------------------------------------------------ bookkeeping
     def slot(self, request) -> int:
@@ -364,6 +368,7 @@ class DensePagedCache:
             raise RuntimeError("no free slot: release a request first")
         self._slots[request] = slot = self._free_slots.pop()
         self._held[slot] = self._seen[slot] = 0
+        self._changes[slot] += 1
         self._write_lengths()
         return slot
 
@@ -414,8 +419,12 @@ class DensePagedCache:
         return PromptStep(self, requests, tokens)
 
     def begin_decode(self) -> None:
-        """Reserves a place for one more token of every request."""
+        """Opens a step: reserves a place for one more token of every request."""
         self._reserve([(slot, self._held[slot] + 1) for slot in self._slots.values()])
+        self._open_step()
+
+    def _open_step(self) -> None:
+        self._step = {slot: self._changes[slot] for slot in self._slots.values()}
 
     def decode(self, layer: int, query: torch.Tensor, key: torch.Tensor, value: torch.Tensor, *, scale: float | None = None,
                out: torch.Tensor | None = None) -> torch.Tensor:
@@ -424,13 +433,19 @@ class DensePagedCache:
         weights = None if self.weights is None else self.weights[layer]
         got = paged_attention(query, self.key_pages[layer], self.value_pages[layer], self.block_table, self.lengths, scale=scale, new_key=key,
                               new_value=value, weights=weights, out=out)
+        if self._step is None:       # without begin_decode: a step whose tokens have room in the pages that there are
+            self._open_step()
         return got if weights is None else got[0]
 
     @torch.no_grad()
     def advance(self) -> None:
-        """Every layer has decoded: the requests hold one more token each."""
-        if any(self._held[s] + 1 > len(self._pages[s]) * self.page_tokens for s in self._slots.values()):
-            raise RuntimeError("state mismatch: begin_decode reserves the places of a step's tokens")
+        """Every layer has decoded: the requests hold one more token each.  Refused where requests came in, got a chunk of
+        their prompt or lost tokens or pages since the step was opened: the step's tokens are not all there, and it is
+        begun again.  A request may have been released."""
+        step = self._step or {}
+        if any(step.get(s) != self._changes[s] or self._held[s] + 1 > len(self._pages[s]) * self.page_tokens for s in self._slots.values()):
+            raise RuntimeError("state mismatch: begin_decode reserves the places of a step's tokens, and the cache has changed since")
+        self._step = None
         if self.positions is not None:
             place = self.lengths.clamp(0, self.positions.shape[3] - 1).long().view(1, -1, 1, 1).expand(self.layers, -1, self.kv_heads, 1)
             self.positions.scatter_(3, place, self.seen.view(1, -1, 1, 1).expand(self.layers, -1, self.kv_heads, 1))
@@ -454,8 +469,10 @@ class DensePagedCache:
                          out_positions=self.positions[layer], out_lengths=left)
         self.lengths.copy_(left)
         for slot in self._slots.values():
+            keep = -(-min(self._held[slot], budget) // self.page_tokens)
+            if self._held[slot] > budget or keep < len(self._pages[slot]):
+                self._changes[slot] += 1
             self._held[slot] = min(self._held[slot], budget)
-            keep = -(-self._held[slot] // self.page_tokens)
             self._free_pages += self._pages[slot][keep:][::-1]
             del self._pages[slot][keep:]
         self._write_table()

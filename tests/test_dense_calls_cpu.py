@@ -326,3 +326,103 @@ def test_rows_of_another_length_are_refused_before_they_are_stored():
     with pytest.raises(ValueError, match="query"):
         step.attend(0, torch.zeros(2, 4, 64, dtype=BF16), rows, rows)
     assert (c.key_pages == 7).all()
+
+
+def cut(c, budget, monkeypatch):
+    monkeypatch.setattr("inquant.dense_paged.evict_tokens", lambda *_, out_lengths, **__: out_lengths.copy_(c.lengths.clamp(max=budget)))
+    c.evict(budget, sink=0, recent=0)
+
+
+def refused_and_repeated(c):
+    """``advance`` refuses and changes nothing; the step begun again is taken into account."""
+    held, seen, lengths, positions = list(c._held), list(c._seen), c.lengths.clone(), c.positions.clone()
+    with pytest.raises(RuntimeError, match="begin_decode"):
+        c.advance()
+    assert (c._held, c._seen) == (held, seen) and torch.equal(c.lengths, lengths) and torch.equal(c.positions, positions)
+    c.begin_decode()
+    c.advance()
+    assert all(c._held[s] == held[s] + 1 for s in c._slots.values())
+
+
+def test_a_step_whose_token_was_evicted_is_not_counted(monkeypatch):
+    c = cache()
+    c.admit("a")
+    c.begin_prompt(["a"], [40]).finish()
+    c.begin_decode()
+    cut(c, 35, monkeypatch)                      # does not end a page: there is room behind it, for a token that is not there
+    refused_and_repeated(c)
+
+
+def test_a_step_whose_place_was_given_back_is_not_counted(monkeypatch):
+    c = cache()
+    c.admit("a"), c.admit("b")
+    c.begin_prompt(["a", "b"], [16, 40]).finish()
+    c.begin_decode()
+    cut(c, 33, monkeypatch)                      # of "a" nothing leaves but the page of its next token
+    refused_and_repeated(c)
+
+
+def test_a_request_that_came_in_during_a_step_is_not_counted():
+    c = cache()
+    c.admit("a")
+    c.begin_prompt(["a"], [5]).finish()
+    c.begin_decode()
+    c.admit("b")
+    c.begin_prompt(["b"], [7]).finish()
+    refused_and_repeated(c)
+    assert (c.tokens("a"), c.tokens("b")) == (6, 8)
+
+
+def test_a_chunk_that_came_in_during_a_step_ends_it():
+    c = cache()
+    c.admit("a")
+    c.begin_prompt(["a"], [5]).finish()
+    c.begin_decode()
+    c.begin_prompt(["a"], [4]).finish()
+    refused_and_repeated(c)
+
+
+def test_a_slot_that_changed_hands_during_a_step_is_not_counted():
+    c = cache()
+    c.admit("a"), c.admit("b")
+    c.begin_prompt(["a", "b"], [5, 5]).finish()
+    c.begin_decode()
+    c.release("b")
+    assert c.admit("b") >= 0
+    c.begin_prompt(["b"], [5]).finish()          # as many tokens as before, others
+    refused_and_repeated(c)
+
+
+def test_a_step_is_counted_once():
+    c = cache()
+    c.admit("a")
+    c.begin_prompt(["a"], [5]).finish()
+    c.begin_decode()
+    c.advance()
+    refused_and_repeated(c)
+
+
+def test_what_does_not_touch_a_step_does_not_end_it(monkeypatch):
+    c = cache(pages=9, max_requests=3)
+    for r in "abc":
+        c.admit(r)
+    c.begin_prompt(["a", "b", "c"], [5, 16, 20]).finish()
+    c.begin_decode()
+    c.evict(64, sink=4, recent=32)               # nobody holds so many
+    c.begin_prompt(["a"], [30])                  # pages are reserved behind the step's, nothing else has happened
+    c.release("c")                               # a request that has ended
+    with pytest.raises(KeyError):
+        c.begin_prompt(["z"], [1])
+    c.advance()
+    assert (c.tokens("a"), c.tokens("b")) == (6, 17)
+    # without begin_decode, where the last page has room: the step begins with its first layer
+    monkeypatch.setattr("inquant.dense_paged.paged_attention", lambda q, *_, **__: (q, None))
+    q, k = torch.zeros(3, 4, 64, dtype=BF16), torch.zeros(3, 2, 64, dtype=BF16)
+    for layer in range(2):
+        c.decode(layer, q, k, k)
+    c.advance()
+    assert (c.tokens("a"), c.tokens("b")) == (7, 18)
+    c.decode(0, q, k, k)
+    c.admit("d")
+    with pytest.raises(RuntimeError, match="begin_decode"):
+        c.advance()
