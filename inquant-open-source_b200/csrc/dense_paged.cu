@@ -318,7 +318,7 @@ __global__ void __launch_bounds__(kDpThreads, kDpPerSm) paged_kernel(const Dense
       // any row may lie in a page of its own, or be the new token's
       const int t = t0 + (lane & 15);
       const bool is_new = t == c.r.fresh;
-      valid = __ballot_sync(0xffffffffu, page >= 0 || (is_new && t < c.r.tokens)) & 0xffffu;
+      valid = __ballot_sync(0xffffffffu, page >= 0) & 0xffffu;      // a new token without a page is not stored, and not attended to
       const long long p = max(page, 0);
       const int o = P.page_shift >= 0 ? t & (P.page_tokens - 1) : t % P.page_tokens;
       const QT* const kr = is_new ? (const QT*)P.new_k + c.b * P.n_sb + kvh * P.n_sh : (const QT*)P.k + p * P.k_sp + kvh * P.k_sh + o * P.k_st;

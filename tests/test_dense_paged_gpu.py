@@ -381,3 +381,37 @@ def test_eviction_out_of_range():
     assert torch.equal(kept[other].view(torch.int16), pool.keys[other].view(torch.int16))
     n, _, _ = evict_tokens(pool.keys, pool.values, pool.table, ints([2 ** 31 - 1, 300]), weights, positions, ints(seen), 256)
     assert N.take_status(pool.keys.device) == N.STATUS_BAD_INDEX and n.tolist() == [256, 256]
+
+
+@pytest.mark.parametrize("heads,q_heads,dim", [(2, 4, 128), (1, 20, 64)])
+@pytest.mark.parametrize("page", [16, 24])
+def test_a_new_token_whose_page_is_not_there_is_left_out(heads, q_heads, dim, page):
+    """It is not stored, so that nothing attends to it and no weight is kept up for it."""
+    from inquant import _native as N
+    from inquant.dense_paged import paged_attention
+    lengths = [12 * page, 12 * page + 5, 40, 0]
+    pool = Pool(lengths, heads, dim, page, torch.bfloat16, seed=31)
+    q, new_k, new_v = (query(4, h, dim, torch.bfloat16, s) for h, s in ((q_heads, 7), (heads, 8), (heads, 9)))
+    old = torch.rand((4, heads, pool.columns * page), device=DEV)
+    assert N.take_status(q.device) == 0
+    for bad in (-1, pool.keys.shape[0], 2 ** 31 - 1):
+        table = pool.table.clone()
+        table[0, 12] = table[1, 12] = table[3, 0] = bad         # tokens 12 page ..: the new one alone, five and the new one, the new one alone
+        kept = pool.keys.clone(), pool.values.clone()
+        into = torch.full_like(old, 5.0)
+        out, w = paged_attention(q, pool.keys, pool.values, table, pool.n, new_key=new_k, new_value=new_v, weights=old, out_weights=into)
+        assert N.take_status(q.device) == N.STATUS_BAD_INDEX
+        check_token(pool, q, out, tokens=[12 * page, 12 * page, 41, 0])
+        for b, n in ((0, 12 * page), (1, 12 * page)):
+            alone = paged_attention(q, pool.keys, pool.values, pool.table, ints([n if i == b else 0 for i in range(4)]),
+                                    weights=old, out_weights=torch.zeros_like(old))[1]
+            assert ((w[b, :, :n] - alone[b, :, :n]).abs() <= 2.0 ** -18 * w[b, :, :n]).all()
+            assert (w[b, :, lengths[b]] == 0).all() and (w[b, :, lengths[b] + 1:] == 5).all()
+        assert torch.equal(w[1, :, 12 * page:12 * page + 5], old[1, :, 12 * page:12 * page + 5])
+        assert (w[3, :, 0] == 0).all()
+        # request 2 has its page: its token was stored, and nothing else
+        p, o = pool.places(2, torch.tensor([40], device=DEV))
+        for now, before, new in zip((pool.keys, pool.values), kept, (new_k, new_v)):
+            assert torch.equal(now[p, :, o][0], new[2])
+            before[p, :, o] = new[2]
+            assert torch.equal(now.view(torch.int16), before.view(torch.int16))
