@@ -473,7 +473,7 @@ int64_t inq_prompt_workspace_bytes(int32_t q_heads, int32_t kv_heads, int32_t he
  * lies in page table[b][t / page_tokens], at offset t % page_tokens; the pages' strides are free (rows of unit
  * channel stride that start on 16 bytes).  lengths[b] tokens are cached; with new_k / new_v the request's new row is stored
  * behind them (lengths is not changed: the layers of a model share it) and attended to.  A negative length marks an
- * unused row: zeros, nothing stored; zeros also where nothing is cached.  A page id outside the pool is never used as an
+ * unused row: zeros, nothing stored; zeros also where nothing is cached (logits that are all -infinity give NaN).  A page id outside the pool is never used as an
  * address: its tokens are left out and INQ_STATUS_BAD_INDEX is set, as it is for a length that the table cannot hold.
  * With out_weights, fp32 [requests, kv_heads, >= table_columns * page_tokens]:
  *   out_weights[b][h][t] = weights[b][h][t] (0 for the new token and where weights is NULL)

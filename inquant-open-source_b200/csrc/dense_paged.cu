@@ -27,7 +27,8 @@ namespace inq {
 constexpr int kDpWarps = 4, kDpThreads = 32 * kDpWarps, kDpPerSm = 2;
 constexpr int kDpSlice = 16;                       // tokens of a unit per warp
 constexpr int kDpUnit = kDpWarps * kDpSlice;
-constexpr float kDpNegBig = -3.0e38f;              // the maximum of nothing
+constexpr float kDpNothing = -3.3e38f;             // the maximum of no token at all
+constexpr float kDpNegBig = -3.0e38f;              // where there are tokens, the maximum is this at least: their logits may all be -infinity
 constexpr float kDpSlack = 8.f;                    // the reference maximum may lag the true one by 2^8
 
 struct DensePagedParams {
@@ -211,19 +212,21 @@ struct DensePagedShape {
   static constexpr int kSmem = kRing + kExchange + kDpWarps * 16 * 2 * 4;
 };
 
-// Log-sum-exp of a row to base 2; a row without weight, for what divides by it.
-__device__ __forceinline__ float join_lse(float top, float sum) { return sum == 0.f ? __int_as_float(0x7f800000) : top + log2f(sum); }
+// Log-sum-exp of a row to base 2 (+infinity without a token, for what divides by it), and the reciprocal of its sum (zero without
+// a token).  A row whose logits are all -infinity divides zero by zero, as its formula does.
+__device__ __forceinline__ float join_lse(float top, float sum) { return top < kDpNegBig ? __int_as_float(0x7f800000) : top + log2f(sum); }
+__device__ __forceinline__ float join_inverse(float top, float sum) { return top < kDpNegBig ? 0.f : 1.f / sum; }
 // Parts c0 .. c1 - 1 of a row in their order: reference maximum, sum and, D / 32 channels a lane, unnormalised output.  A warp;
 // all it reads of 16 parts is asked for at once, since a trip to memory is what this costs.
 template <int D>
 struct Joined {
   static constexpr int kPairs = D / 64, kAtOnce = 16;
-  float top = kDpNegBig, sum = 0.f;
+  float top = kDpNothing, sum = 0.f;
   float2 out[kPairs] = {};
   __device__ __forceinline__ void add(const float* rec, long long stride, int c0, int c1) {
     const int lane = threadIdx.x & 31;
     for (int c = c0; c < c1; c += kAtOnce) {
-      const float2 ml = lane < kAtOnce && c + lane < c1 ? __ldcg((const float2*)(rec + (c + lane) * stride + D)) : make_float2(kDpNegBig, 0.f);
+      const float2 ml = lane < kAtOnce && c + lane < c1 ? __ldcg((const float2*)(rec + (c + lane) * stride + D)) : make_float2(kDpNothing, 0.f);
       float2 x[kAtOnce][kPairs];
 #pragma unroll
       for (int i = 0; i < kAtOnce; ++i)
@@ -253,7 +256,7 @@ struct Joined {
   template <typename QT>
   __device__ __forceinline__ void store(QT* to, float* lse) const {
     const int lane = threadIdx.x & 31;
-    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+    const float inv = join_inverse(top, sum);
 #pragma unroll
     for (int k = 0; k < kPairs; ++k) *(unsigned*)(to + 64 * k + 2 * lane) = pf_pack2<QT>(out[k].x * inv, out[k].y * inv);
     if (lse && lane == 0) *lse = join_lse(top, sum);
@@ -393,12 +396,14 @@ __global__ void __launch_bounds__(kDpThreads, kDpPerSm) paged_kernel(const Dense
   unsigned qf[TILES][D / 16][2];                // query heads as right operands
   float o[TILES][D / 16][4], m[TILES][2], l[TILES][2];      // heads 8 i + 2 (lane & 3) (+ 1)
   const int c0 = 2 * (lane & 3), g = lane >> 2;
+  unsigned some = 0;          // whether this warp has met a token of the pair
   bool first = true;
   for (int done = 1; done <= count; ++done) {
     const int h0 = at.pair / P.chunks * P.group + at.pair % P.chunks * 16, rows = min(P.group - at.pair % P.chunks * 16, 16);
     if (first) {
       // a new pair: its query rows (those beyond the group are zero), an empty state
       first = false;
+      some = 0;
 #pragma unroll
       for (int i = 0; i < TILES; ++i) {
         const int r = g + 8 * i;
@@ -409,13 +414,14 @@ __global__ void __launch_bounds__(kDpThreads, kDpPerSm) paged_kernel(const Dense
           qf[i][kk][1] = r < rows ? *(const unsigned*)(src + 16 * kk + 8) : 0u;
           o[i][kk][0] = o[i][kk][1] = o[i][kk][2] = o[i][kk][3] = 0.f;
         }
-        m[i][0] = m[i][1] = kDpNegBig;
+        m[i][0] = m[i][1] = kDpNothing;
         l[i][0] = l[i][1] = 0.f;
       }
     }
     ask();
     const unsigned valid = (unsigned)rows_ahead & 0xffffu;
     rows_ahead >>= 16;
+    some |= valid;
     dp_wait<kAhead>();
     __syncwarp();
     if (at.unit * kDpUnit + warp * kDpSlice < at.r.tokens) {
@@ -502,7 +508,7 @@ __global__ void __launch_bounds__(kDpThreads, kDpPerSm) paged_kernel(const Dense
           l[i][e] += __shfl_xor_sync(0xffffffffu, l[i][e], 4);
           l[i][e] += __shfl_xor_sync(0xffffffffu, l[i][e], 8);
           l[i][e] += __shfl_xor_sync(0xffffffffu, l[i][e], 16);
-          if (lane < 4) *(float2*)(ml + 2 * (warp * 16 + 8 * i + c0 + e)) = make_float2(m[i][e], l[i][e]);
+          if (lane < 4) *(float2*)(ml + 2 * (warp * 16 + 8 * i + c0 + e)) = make_float2(some ? fmaxf(m[i][e], kDpNegBig) : m[i][e], l[i][e]);
         }
       const bool alone = pair_ends && done > at.unit;      // every unit of the pair was in this range
       const long long pair = (long long)at.b * P.kv_heads * P.chunks + at.pair;
@@ -521,7 +527,7 @@ __global__ void __launch_bounds__(kDpThreads, kDpPerSm) paged_kernel(const Dense
         const int r = tid / (D / 4), c = 4 * (tid % (D / 4)), row = r + 4 * four;
         if (r < 4 && row < rows) {
           float2 each[kDpWarps];
-          float top = kDpNegBig;
+          float top = kDpNothing;
 #pragma unroll
           for (int w = 0; w < kDpWarps; ++w) {
             each[w] = *(const float2*)(ml + 2 * (w * 16 + row));
@@ -543,7 +549,7 @@ __global__ void __launch_bounds__(kDpThreads, kDpPerSm) paged_kernel(const Dense
           if (c == 0) *(float2*)(rec + D) = make_float2(top, weight);
           if (alone) {
             if (WEIGHTS && c == 0) P.lse[at.b * P.q_heads + h0 + row] = join_lse(top, weight);
-            const float inv = weight == 0.f ? 0.f : 1.f / weight;
+            const float inv = join_inverse(top, weight);
             *(uint2*)((QT*)P.out + at.b * P.o_sb + (long long)(h0 + row) * P.o_sh + c) =
                 make_uint2(pf_pack2<QT>(sum.x * inv, sum.y * inv), pf_pack2<QT>(sum.z * inv, sum.w * inv));
           } else {

@@ -70,7 +70,8 @@ def paged_attention(query: torch.Tensor, key_pages: torch.Tensor, value_pages: t
     step's, summed over the query heads of a KV head; the new token starts from zero.  ``out_weights`` alone gets this
     step's.  Entries behind a request's tokens are left as they were.
 
-    A negative length marks an unused row (zeros, nothing stored); a request without tokens gives zeros.  A page id
+    A negative length marks an unused row (zeros, nothing stored); a request without tokens gives zeros, one whose logits are
+    all -infinity NaN, as the formula does.  A page id
     outside the pool is never used as an address: its tokens are left out, a new one among them is not stored, and
     ``STATUS_BAD_INDEX`` is set in the device's status word, as it is for a length beyond the table.  Two requests may share pages as long as neither
     stores into them.  With weights the call takes scratch of 4 bytes per query head and token that the table can

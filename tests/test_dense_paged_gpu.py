@@ -415,3 +415,33 @@ def test_a_new_token_whose_page_is_not_there_is_left_out(heads, q_heads, dim, pa
             assert torch.equal(now[p, :, o][0], new[2])
             before[p, :, o] = new[2]
             assert torch.equal(now.view(torch.int16), before.view(torch.int16))
+
+
+@pytest.mark.parametrize("lengths", [[1], [37, 200], [9000, 5, 0], [300] * 40])
+@pytest.mark.parametrize("weights", [False, True])
+def test_logits_that_are_all_minus_infinity_are_not_a_number(lengths, weights):
+    """Zero divided by zero, as the formula has it and packed prompts give it; a row of the same request with one finite
+    logit has that token, and a request without tokens zeros."""
+    from inquant.dense_paged import paged_attention
+    pool = Pool(lengths, 2, 128, 16, torch.bfloat16, seed=33, spare=1)
+    q = query(len(lengths), 8, 128, torch.bfloat16)
+    q[:, :, 0] = 1.0
+    for b, n in enumerate(lengths):
+        if n:
+            p, o = pool.places(b, torch.arange(n, device=DEV))
+            pool.keys[p, :, o, 0] = -math.inf
+            p, o = pool.places(b, torch.tensor([n // 2], device=DEV))
+            pool.keys[p, 1, o, 0] = 0.25     # the one token that heads 4 to 7 have
+    into = torch.zeros((len(lengths), 2, pool.columns * 16), device=DEV) if weights else None
+    got = paged_attention(q, pool.keys, pool.values, pool.table, pool.n, out_weights=into)
+    out = got[0] if weights else got
+    for b, n in enumerate(lengths):
+        if n == 0:
+            assert (out[b] == 0).all()
+            continue
+        p, o = pool.places(b, torch.tensor([n // 2], device=DEV))
+        assert torch.isnan(out[b, :4]).all() and torch.equal(out[b, 4:], pool.values[p, 1, o].expand(4, 128))
+        if weights:
+            one = torch.zeros(n, device=DEV)
+            one[n // 2] = 4.0
+            assert torch.isnan(got[1][b, 0, :n]).all() and torch.equal(got[1][b, 1, :n], one)
