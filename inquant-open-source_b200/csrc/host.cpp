@@ -320,6 +320,26 @@ bool rows3(const at::Tensor& t) { return t.dim() == 3 && t.stride(2) == 1 && t.s
 bool rows4(const at::Tensor& t) {
   return t.dim() == 4 && t.stride(3) == 1 && t.stride(0) % 8 == 0 && t.stride(1) % 8 == 0 && t.stride(2) % 8 == 0 && aligned(t);
 }
+// Whether no two elements share memory, of a tensor of up to three axes that is written (strides are never negative).
+bool apart(const at::Tensor& t) {
+  int64_t strides[3], sizes[3], end = 1;
+  int n = 0;
+  for (int64_t i = 0; i < t.dim(); ++i) {
+    if (t.size(i) <= 1) continue;
+    int at = n++;
+    for (; at > 0 && strides[at - 1] > t.stride(i); --at) {
+      strides[at] = strides[at - 1];
+      sizes[at] = sizes[at - 1];
+    }
+    strides[at] = t.stride(i);
+    sizes[at] = t.size(i);
+  }
+  for (int i = 0; i < n; ++i) {
+    if (strides[i] < end) return false;
+    end += strides[i] * (sizes[i] - 1);
+  }
+  return true;
+}
 bool int32_vector(const at::Tensor& t, int64_t n, const at::Tensor& pages) {
   return t.dim() == 1 && t.size(0) == n && t.scalar_type() == at::kInt && t.device() == pages.device() && t.is_contiguous();
 }
@@ -390,8 +410,8 @@ PyObject* prompt_attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
     const at::Tensor *q, *k, *value = plain(args[2]), *out, *lse;
     if (!value || !packed(args, q, k, args[3], args[4], args[5], a) || !optional(args[6], out) || !optional(args[7], lse)) return none();
     if (!rows3(*value) || !like(*value, *q) || value->sizes() != k->sizes() || value->stride(0) <= 0 || value->stride(1) <= 0) return none();
-    if (out && (!rows3(*out) || !like(*out, *q) || out->sizes() != q->sizes() || out->stride(0) <= 0 || out->stride(1) <= 0)) return none();
-    if (lse && !float_rows(*lse, a.q_heads, a.q_rows, *q)) return none();
+    if (out && (!rows3(*out) || !like(*out, *q) || out->sizes() != q->sizes() || out->stride(0) <= 0 || out->stride(1) <= 0 || !apart(*out))) return none();
+    if (lse && (!float_rows(*lse, a.q_heads, a.q_rows, *q) || !apart(*lse))) return none();
     at::Tensor o = out ? *out : fresh(q->sizes(), *q, q->scalar_type()), l = lse ? *lse : fresh({a.q_heads, a.q_rows}, *q, at::kFloat);
     a.v = value->data_ptr();
     a.v_stride_t = value->stride(0);
@@ -421,7 +441,7 @@ PyObject* prompt_weights(PyObject*, PyObject* const* args, Py_ssize_t n) {
     inq_prompt_args_t a = {};
     const at::Tensor *q, *k, *lse = plain(args[2]), *out;
     if (!lse || !packed(args, q, k, args[3], args[4], args[5], a) || !optional(args[7], out)) return none();
-    if (!float_rows(*lse, a.q_heads, a.q_rows, *q) || (out && !float_rows(*out, a.kv_heads, a.k_rows, *q))) return none();
+    if (!float_rows(*lse, a.q_heads, a.q_rows, *q) || (out && (!float_rows(*out, a.kv_heads, a.k_rows, *q) || !apart(*out)))) return none();
     at::Tensor w = out ? *out : fresh({a.kv_heads, a.k_rows}, *q, at::kFloat);
     a.lse = static_cast<float*>(lse->data_ptr());
     a.lse_stride = lse->stride(0);
@@ -488,11 +508,12 @@ PyObject* paged_attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
     if (!scale_of(args[5], a.head_dim, a.scale) || !new_k != !new_v) return none();
     for (const at::Tensor* t : {new_k, new_v})
       if (t && (!rows3(*t) || !like(*t, *k) || t->size(0) != a.requests || t->size(1) != a.kv_heads || t->size(2) != a.head_dim)) return none();
-    if (out && (!rows3(*out) || !like(*out, *q) || out->sizes() != q->sizes())) return none();
+    if (out && (!rows3(*out) || !like(*out, *q) || out->sizes() != q->sizes() || !apart(*out))) return none();
     PyObject* const weights_given = args[9] != Py_None ? args[9] : args[8];
     if (!out_w) out_w = w;
     for (const at::Tensor* t : {w, out_w})
       if (t && !state(*t, at::kFloat, a.requests, a.kv_heads, (int64_t)a.table_columns * a.page_tokens, *k)) return none();
+    if (out_w && !apart(*out_w)) return none();
     at::Tensor o = out ? *out : fresh(q->sizes(), *q, q->scalar_type());
     a.q = q->data_ptr();
     a.q_stride_b = q->stride(0);
@@ -552,6 +573,7 @@ PyObject* evict_tokens(PyObject*, PyObject* const* args, Py_ssize_t n) {
     const int64_t requests = a.requests, heads = a.kv_heads;
     if (!int32_vector(*seen, requests, *k) || !state(*w, at::kFloat, requests, heads, 1, *k) || !state(*p, at::kInt, requests, heads, w->size(2), *k)) return none();
     if ((out_w && !state(*out_w, at::kFloat, requests, heads, v[0], *k)) || (out_p && !state(*out_p, at::kInt, requests, heads, v[0], *k))) return none();
+    if ((out_w && !apart(*out_w)) || (out_p && !apart(*out_p))) return none();
     if (out_n && !int32_vector(*out_n, requests, *k)) return none();
     at::Tensor nw = out_w ? *out_w : fresh({requests, heads, v[0]}, *k, at::kFloat), np = out_p ? *out_p : fresh({requests, heads, v[0]}, *k, at::kInt);
     at::Tensor nn = out_n ? *out_n : fresh({requests}, *k, at::kInt);

@@ -19,7 +19,7 @@ import ctypes
 import torch
 
 from . import _native as N
-from .prompt import _scale, prompt_attention, prompt_weights
+from .prompt import _rows_apart, _scale, prompt_attention, prompt_weights
 
 
 def _aligned(t: torch.Tensor) -> bool:
@@ -52,10 +52,12 @@ def _pairs(query: torch.Tensor, key_pages: torch.Tensor) -> int:
     return max(query.shape[0] * heads * ((query.shape[1] // heads + 15) // 16), 1)
 
 
-def _check_state(name: str, t: torch.Tensor, dtype: torch.dtype, requests: int, heads: int, columns: int, device) -> None:
+def _check_state(name: str, t: torch.Tensor, dtype: torch.dtype, requests: int, heads: int, columns: int, device, written: bool = False) -> None:
     if t.ndim != 3 or t.shape[0] != requests or t.shape[1] != heads or t.shape[2] < columns or t.dtype != dtype or t.device != device \
             or (t.shape[2] > 1 and t.stride(2) != 1):
         raise ValueError(f"{name} must be a {dtype} tensor [{requests}, {heads}, >= {columns}] with unit token stride on the pages' device")
+    if written and not _rows_apart(t):
+        raise ValueError(f"the rows of {name} must share no memory")
 
 
 def paged_attention(query: torch.Tensor, key_pages: torch.Tensor, value_pages: torch.Tensor, block_table: torch.Tensor,
@@ -112,13 +114,13 @@ def _paged_attention(query, key_pages, value_pages, block_table, lengths, scale,
     rows = [t if _aligned(t) else t.clone(memory_format=torch.contiguous_format) for t in rows]
     if out is None:
         out = torch.empty(query.shape, dtype=query.dtype, device=device)
-    elif out.shape != query.shape or out.dtype != query.dtype or out.device != device or not _aligned(out):
-        raise ValueError("out must be a [requests, Hq, D] tensor of the pages' dtype and device with aligned rows")
+    elif out.shape != query.shape or out.dtype != query.dtype or out.device != device or not _aligned(out) or not _rows_apart(out):
+        raise ValueError("out must be a [requests, Hq, D] tensor of the pages' dtype and device with aligned rows that share no memory")
     if weights is not None:
         _check_state("weights", weights, torch.float32, requests, heads, block_table.shape[1] * page_tokens, device)
         out_weights = weights if out_weights is None else out_weights
     if out_weights is not None:
-        _check_state("out_weights", out_weights, torch.float32, requests, heads, block_table.shape[1] * page_tokens, device)
+        _check_state("out_weights", out_weights, torch.float32, requests, heads, block_table.shape[1] * page_tokens, device, written=True)
     if requests == 0:
         return out if out_weights is None else (out, out_weights)
     lengths = lengths.contiguous()
@@ -199,8 +201,8 @@ def _evict_tokens(key_pages, value_pages, block_table, lengths, weights, positio
         out_positions = torch.empty((requests, heads, budget), dtype=torch.int32, device=device)
     if out_lengths is None:
         out_lengths = torch.empty_like(lengths, memory_format=torch.contiguous_format)
-    _check_state("out_weights", out_weights, torch.float32, requests, heads, budget, device)
-    _check_state("out_positions", out_positions, torch.int32, requests, heads, budget, device)
+    _check_state("out_weights", out_weights, torch.float32, requests, heads, budget, device, written=True)
+    _check_state("out_positions", out_positions, torch.int32, requests, heads, budget, device, written=True)
     if out_lengths.shape != lengths.shape or out_lengths.dtype != torch.int32 or out_lengths.device != device or not out_lengths.is_contiguous():
         raise ValueError("out_lengths must be a contiguous int32 tensor [requests] on the pages' device")
     if requests == 0:

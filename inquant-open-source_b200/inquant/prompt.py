@@ -27,6 +27,16 @@ def _rows(t: torch.Tensor) -> torch.Tensor:
     return t if ok else t.clone(memory_format=torch.contiguous_format)
 
 
+def _rows_apart(t: torch.Tensor) -> bool:
+    """Whether no two elements share memory, as it has to be where a kernel writes."""
+    end = 1
+    for stride, size in sorted((s, n) for s, n in zip(t.stride(), t.shape) if n > 1):
+        if stride < end:
+            return False
+        end += stride * (size - 1)
+    return True
+
+
 def _check_offsets(name: str, offsets: torch.Tensor, device: torch.device) -> torch.Tensor:
     if offsets.dtype != torch.int32 or offsets.ndim != 1 or offsets.numel() < 2:
         raise ValueError(f"{name} must be an int32 tensor [sequences + 1]")
@@ -113,12 +123,14 @@ def _prompt_attention(query, key, value, cu_seqlens, cu_seqlens_k, scale, out, l
     tokens, q_heads, dim = query.shape
     if out is None:
         out = torch.empty((tokens, q_heads, dim), dtype=query.dtype, device=query.device)
-    elif out.shape != query.shape or out.dtype != query.dtype or out.device != query.device or (tokens and _rows(out) is not out):
-        raise ValueError("out must be a [Tq, Hq, D] tensor of the query dtype and device with aligned rows")
+    elif out.shape != query.shape or out.dtype != query.dtype or out.device != query.device or (tokens and _rows(out) is not out) \
+            or not _rows_apart(out):
+        raise ValueError("out must be a [Tq, Hq, D] tensor of the query dtype and device with aligned rows that share no memory")
     if lse is None:
         lse = torch.empty((q_heads, tokens), dtype=torch.float32, device=query.device)
-    elif lse.shape != (q_heads, tokens) or lse.dtype != torch.float32 or lse.device != query.device or lse.stride(1) != 1:
-        raise ValueError("lse must be an fp32 tensor [Hq, Tq] on the query's device with unit token stride")
+    elif lse.shape != (q_heads, tokens) or lse.dtype != torch.float32 or lse.device != query.device or lse.stride(1) != 1 \
+            or not _rows_apart(lse):
+        raise ValueError("lse must be an fp32 tensor [Hq, Tq] on the query's device with unit token stride, its rows sharing no memory")
     if tokens == 0:
         return out, lse
     if key.shape[0] == 0:       # no key anywhere: one row that no sequence reaches stands for the tensors
@@ -170,8 +182,8 @@ def _prompt_weights(query, key, lse, cu_seqlens, cu_seqlens_k, scale, window, ou
     shape = (key.shape[1], key.shape[0])
     if out is None:
         out = torch.empty(shape, dtype=torch.float32, device=query.device)
-    elif out.shape != shape or out.dtype != torch.float32 or out.device != query.device or out.stride(1) != 1:
-        raise ValueError("out must be an fp32 tensor [H, Tk] on the query's device with unit token stride")
+    elif out.shape != shape or out.dtype != torch.float32 or out.device != query.device or out.stride(1) != 1 or not _rows_apart(out):
+        raise ValueError("out must be an fp32 tensor [H, Tk] on the query's device with unit token stride, its rows sharing no memory")
     if key.shape[0] == 0:
         return out
     if tokens == 0:             # no query anywhere: one row that no sequence reaches stands for the tensors

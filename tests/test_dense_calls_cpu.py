@@ -1,5 +1,6 @@
 """What the calls over packed prompts and uncompressed pages refuse, and the bookkeeping of ``DensePagedCache`` (no GPU: every
 refusal comes before the first launch)."""
+import contextlib
 import ctypes
 
 import pytest
@@ -426,3 +427,32 @@ def test_what_does_not_touch_a_step_does_not_end_it(monkeypatch):
     c.admit("d")
     with pytest.raises(RuntimeError, match="begin_decode"):
         c.advance()
+
+
+@pytest.mark.parametrize("call,name,shape,dtype", [
+    (prompt_attention, "out", (8, 4, 128), BF16), (prompt_attention, "lse", (4, 8), torch.float32), (prompt_weights, "out", (2, 8), torch.float32),
+    (paged_attention, "out", (3, 4, 128), BF16), (paged_attention, "weights", (3, 2, 32), torch.float32),
+    (paged_attention, "out_weights", (3, 2, 32), torch.float32), (evict_tokens, "out_weights", (3, 2, 32), torch.float32),
+    (evict_tokens, "out_positions", (3, 2, 32), torch.int32)])
+def test_results_whose_rows_share_memory_are_refused(no_device, monkeypatch, call, name, shape, dtype):
+    monkeypatch.setattr(torch.cuda, "device", lambda _device: contextlib.nullcontext())
+    case = dict(paged_case() if call is paged_attention else evict_case() if call is evict_tokens else prompt_case())
+    if call is prompt_weights:
+        case["lse"] = torch.zeros(4, 8)
+        del case["value"]
+    for axis in range(len(shape) - 1):
+        row = torch.zeros([1 if i == axis else n for i, n in enumerate(shape)], dtype=dtype)
+        views = [row.expand(shape)]                                            # the same row for all
+        if axis == 0:
+            step = [shape[-1] // 2] + [shape[-1]] * (len(shape) - 2) + [1]         # rows that begin inside the one before
+            views.append(torch.zeros(4096, dtype=dtype).as_strided(shape, step))
+        for view in views:
+            with pytest.raises(ValueError, match=name):
+                call(**{**case, name: view})
+    room = torch.zeros([2 * n for n in shape], dtype=dtype)[tuple(slice(n, None) for n in shape)]
+    for view in (room, torch.zeros(shape[::-1][1:] + shape[-1:], dtype=dtype).transpose(0, 1) if len(shape) == 3 else room):
+        with pytest.raises(pytest.fail.Exception, match="not refused"):        # gaps and other orders of rows are served
+            call(**{**case, name: view})
+    if name == "weights":                                                      # read alone, they may be the same row for all
+        with pytest.raises(pytest.fail.Exception, match="not refused"):
+            call(**{**case, name: torch.zeros(1, 1, 32).expand(shape), "out_weights": torch.zeros(shape)})

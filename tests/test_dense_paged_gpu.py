@@ -445,3 +445,29 @@ def test_logits_that_are_all_minus_infinity_are_not_a_number(lengths, weights):
             one = torch.zeros(n, device=DEV)
             one[n // 2] = 4.0
             assert torch.isnan(got[1][b, 0, :n]).all() and torch.equal(got[1][b, 1, :n], one)
+
+
+def test_results_whose_rows_share_memory_are_refused_before_any_launch():
+    """As without a GPU, where the native side of a call looks first."""
+    from inquant.dense_paged import evict_tokens, paged_attention
+    from inquant.prompt import prompt_attention, prompt_weights
+    lengths = [300, 40]
+    pool = Pool(lengths, 2, 128, 16, torch.bfloat16, seed=45)
+    kept, q, width = pool.keys.clone(), query(2, 4, 128, torch.bfloat16), pool.columns * 16
+    weights, positions, seen = eviction_state(lengths, 2, width, 46)
+    decode, cut = (pool.keys, pool.values, pool.table, pool.n), (pool.keys, pool.values, pool.table, pool.n, weights, positions, ints(seen), 64)
+    floats, whole = torch.zeros((1, 1, width), device=DEV), torch.zeros((1, 1, width), dtype=torch.int32, device=DEV)
+    rows, cu = query(8, 4, 128, torch.bfloat16), ints([0, 8])
+    for call in (lambda: paged_attention(q, *decode, out=q[:, :1].clone().expand(2, 4, 128)), lambda: paged_attention(q, *decode, out_weights=floats.expand(2, 2, width)),
+                 lambda: paged_attention(q, *decode, weights=floats.expand(2, 2, width)), lambda: evict_tokens(*cut, sink=1, recent=2, out_weights=floats.expand(2, 2, width)),
+                 lambda: evict_tokens(*cut, sink=1, recent=2, out_positions=whole.expand(2, 2, width)),
+                 lambda: prompt_attention(rows, rows, rows, cu, out=torch.zeros(4096, dtype=rows.dtype, device=DEV).as_strided((8, 4, 128), (64, 128, 1))),
+                 lambda: prompt_attention(rows, rows, rows, cu, lse=floats[0, :, :8].expand(4, 8)),
+                 lambda: prompt_weights(rows, rows, torch.zeros((4, 8), device=DEV), cu, out=floats[0, :, :8].expand(4, 8))):
+        with pytest.raises(ValueError):
+            call()
+    assert torch.equal(kept.view(torch.int16), pool.keys.view(torch.int16)) and (floats == 0).all() and (whole == 0).all()
+    # what is only read may be the same row for all
+    a = paged_attention(q, *decode, weights=floats.expand(2, 2, width), out_weights=torch.zeros((2, 2, width), device=DEV))
+    b = paged_attention(q, *decode, out_weights=torch.zeros((2, 2, width), device=DEV))
+    assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
