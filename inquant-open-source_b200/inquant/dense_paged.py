@@ -19,7 +19,7 @@ import ctypes
 import torch
 
 from . import _native as N
-from .prompt import _rows_apart, _scale, prompt_attention, prompt_weights
+from .prompt import _check_states, _check_window, _rows_apart, _scale, prompt_attention, prompt_weights
 
 
 def _aligned(t: torch.Tensor) -> bool:
@@ -283,6 +283,13 @@ class PromptStep:
             raise ValueError("Expected query [tokens of the step, Hq, D]")
         if key.shape != (total, cache.kv_heads, cache.head_dim) or value.shape != key.shape or key.dtype != cache.dtype or value.dtype != key.dtype:
             raise ValueError("Expected key/value [tokens of the step, H, D] of the cache's dtype")
+        if any(t.device != cache.device for t in (query, key, value)):
+            raise ValueError("query, key, value and the cache must share a device")
+        # all that the calls below refuse, before the rows are stored
+        _check_states("prompt_attention", query, key)
+        _scale(scale, cache.head_dim)
+        if cache.weights is not None:
+            _check_window(window)
         key_pages, value_pages = cache.key_pages[layer], cache.value_pages[layer]
         key_pages[self.new_pages, :, self.new_offsets] = key
         value_pages[self.new_pages, :, self.new_offsets] = value

@@ -66,6 +66,11 @@ def _scale(scale: float | None, dim: int) -> float:
     return scale
 
 
+def _check_window(window: int | None) -> None:
+    if window is not None and window < 1:
+        raise ValueError("window must be positive")
+
+
 def _arguments(query, key, cu_seqlens, cu_seqlens_k, scale, window, weights) -> N.PromptArgs:
     args = N.PromptArgs()
     args.q, args.k = query.data_ptr(), key.data_ptr()
@@ -168,8 +173,7 @@ def prompt_weights(query: torch.Tensor, key: torch.Tensor, lse: torch.Tensor, cu
 def _prompt_weights(query, key, lse, cu_seqlens, cu_seqlens_k, scale, window, out):
     _check_states("prompt_weights", query, key)
     scale = _scale(scale, query.shape[2])
-    if window is not None and window < 1:
-        raise ValueError("window must be positive")
+    _check_window(window)
     cu_seqlens = _check_offsets("cu_seqlens", cu_seqlens, query.device)
     cu_seqlens_k = cu_seqlens if cu_seqlens_k is None else _check_offsets("cu_seqlens_k", cu_seqlens_k, query.device)
     if cu_seqlens_k.numel() != cu_seqlens.numel():

@@ -456,3 +456,22 @@ def test_results_whose_rows_share_memory_are_refused(no_device, monkeypatch, cal
     if name == "weights":                                                      # read alone, they may be the same row for all
         with pytest.raises(pytest.fail.Exception, match="not refused"):
             call(**{**case, name: torch.zeros(1, 1, 32).expand(shape), "out_weights": torch.zeros(shape)})
+
+
+@pytest.mark.parametrize("changes", [dict(query=torch.zeros(3, 4, 64)), dict(query=torch.zeros(3, 4, 64, dtype=torch.float16)),
+                                     dict(query=torch.zeros(3, 4, 128, dtype=BF16)), dict(query=torch.zeros(3, 5, 64, dtype=BF16)),
+                                     dict(query=torch.zeros(3, 0, 64, dtype=BF16)), dict(scale=0.0), dict(scale=float("nan")), dict(window=0), dict(window=-1),
+                                     dict(query=torch.zeros(3, 4, 64, dtype=BF16, device="meta")), dict(key=torch.zeros(3, 2, 64, dtype=BF16, device="meta")),
+                                     dict(value=torch.zeros(3, 2, 64, dtype=BF16, device="meta"))])
+@pytest.mark.parametrize("weights", [True, False])
+def test_what_a_prompt_step_refuses_is_not_stored(no_device, weights, changes):
+    if "window" in changes and not weights:
+        changes = dict(scale=-1.0)                # there are no weights that a window would be of
+    c = cache(weights=weights)
+    c.admit("a")
+    step = c.begin_prompt(["a"], [3])
+    c.key_pages.fill_(7), c.value_pages.fill_(7)
+    rows = torch.zeros(3, 2, 64, dtype=BF16)
+    with pytest.raises((ValueError, NotImplementedError)):
+        step.attend(0, **{**dict(query=torch.zeros(3, 4, 64, dtype=BF16), key=rows, value=rows), **changes})
+    assert (c.key_pages == 7).all() and (c.value_pages == 7).all()
