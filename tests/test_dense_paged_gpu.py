@@ -471,3 +471,119 @@ def test_results_whose_rows_share_memory_are_refused_before_any_launch():
     a = paged_attention(q, *decode, weights=floats.expand(2, 2, width), out_weights=torch.zeros((2, 2, width), device=DEV))
     b = paged_attention(q, *decode, out_weights=torch.zeros((2, 2, width), device=DEV))
     assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+
+
+# slices of a row per CTA of 2561 to 4608 tokens, of up to 8192 and of more, in one CTA per row and in clusters
+@pytest.mark.parametrize("lengths,heads,budget", [
+    ([4000, 2561, 100] + [3900] * 37, 8, 3000), ([7000, 4609, 8192] + [6000] * 37, 8, 5000), ([9000, 16385, 8193] + [9000 + i for i in range(37)], 8, 8500),
+    ([70001], 2, 30000), ([131072, 50000], 1, 100000)])
+@pytest.mark.parametrize("in_place", [False, "state", True])
+def test_long_slices_of_rows(lengths, heads, budget, in_place):
+    """Ties everywhere, across the borders of slices and of what a CTA looks at in one go."""
+    pool = Pool(lengths, heads, 64, 64, torch.float16, seed=35)
+    weights, positions, seen = eviction_state(lengths, heads, pool.columns * 64, 36, ties=0.7)
+    check_evict(pool, heads, lengths, seen, weights, positions, budget, 4, 100, in_place)
+
+
+def test_offsets_that_pass_32_bits_for_keys_and_values():
+    """Pages that start between 2^31 and 5 2^30 elements: read, stored into and moved within."""
+    from inquant.dense_paged import evict_tokens, paged_attention
+    lengths, page_stride = [60], 2 ** 30
+    pool = Pool(lengths, 2, 128, 16, torch.bfloat16, seed=37)
+    q, new_k, new_v = (query(1, h, 128, torch.bfloat16, s) for h, s in ((14, 7), (2, 8), (2, 9)))
+    table = ints([[5, 2, 4, 3]])
+    assert pool.table.shape == table.shape and all(p * page_stride >= 2 ** 31 for p in table[0].tolist()) and 5 * page_stride > 2 ** 32
+    keys, values = (torch.empty(5 * page_stride + 4096, dtype=torch.bfloat16, device=DEV).as_strided((6, 2, 16, 128), (page_stride, 2048, 128, 1)) for _ in range(2))
+    keys[table[0].long()], values[table[0].long()] = pool.keys[pool.table[0].long()], pool.values[pool.table[0].long()]
+    near, far = (pool.keys, pool.values, pool.table), (keys, values, table)
+    old = torch.rand((1, 2, 64), device=DEV)
+    steps = [paged_attention(q, *at, pool.n, new_key=new_k, new_value=new_v, weights=old, out_weights=torch.zeros_like(old)) for at in (near, far)]
+    assert all(torch.equal(a, b) for a, b in zip(*steps))
+    check_token(pool, q, steps[1][0], steps[1][1], old, fresh=True)
+    positions = torch.arange(64, dtype=torch.int32, device=DEV).expand(1, 2, 64).contiguous()
+    cuts = [evict_tokens(*at, ints([61]), steps[0][1], positions, ints([61]), 33, sink=2, recent=9) for at in (near, far)]
+    assert all(torch.equal(a, b) for a, b in zip(*cuts))
+    for there, here in ((keys, pool.keys), (values, pool.values)):
+        a, b = there[table[0].long()], here[pool.table[0].long()]
+        assert torch.equal(a.view(torch.int16), b.view(torch.int16))
+
+
+def ragged(count, longest, seed):
+    g = torch.Generator().manual_seed(seed)
+    return [[0, -1, 1, longest][b] if b < 4 else int(torch.randint(1, longest + 1, (1,), generator=g)) for b in range(count)]
+
+
+def test_ranges_of_two_sizes():
+    """More than 48 units of 64 tokens for each CTA: three quarters of an even share first, then eighths."""
+    from inquant.dense_paged import paged_attention
+    lengths = ragged(64, 8192, 38)
+    pool = Pool(lengths, 8, 128, 16, torch.bfloat16, seed=39, spare=1)
+    ctas = 2 * torch.cuda.get_device_properties(0).multi_processor_count
+    assert sum(-(-max(n, 0) // 64) for n in lengths) * 8 > 48 * ctas
+    q = query(64, 32, 128, torch.bfloat16)
+    new_k, new_v = query(64, 8, 128, torch.bfloat16, 8), query(64, 8, 128, torch.bfloat16, 9)
+    old = torch.rand((64, 8, pool.columns * 16), device=DEV)
+    out, w = paged_attention(q, pool.keys, pool.values, pool.table, pool.n, new_key=new_k, new_value=new_v, weights=old, out_weights=torch.zeros_like(old))
+    check_token(pool, q, out, w, old, fresh=True)
+
+
+def test_a_captured_step_whose_ranges_change_their_kind():
+    """One launch serves lengths that are cut evenly and lengths that are cut into ranges of two sizes."""
+    from inquant.dense_paged import paged_attention
+    mixes = [ragged(64, 8192, 40), [40] * 64, ragged(64, 8192, 41)[::-1], [0] * 63 + [8000], ragged(64, 5200, 42)]
+    pool = Pool([8192] * 64, 8, 64, 64, torch.float16, seed=43)
+    q = query(64, 32, 64, torch.float16)
+    n, into = ints(mixes[0]), torch.zeros((64, 8, pool.columns * 64), device=DEV)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out, _ = paged_attention(q, pool.keys, pool.values, pool.table, n, out_weights=into)
+    for mix in mixes:
+        n.copy_(ints(mix))
+        graph.replay()
+        check_token(pool, q, out, into, tokens=[max(x, 0) for x in mix])
+
+
+@pytest.mark.parametrize("budget", [64, 300])
+def test_a_captured_eviction_follows_lengths_and_weights(budget):
+    from inquant.dense_paged import evict_tokens
+    mixes = [[700, 64, 300], [301, 65, 1], [0, -1, 640]]
+    pool = Pool([700] * 3, 2, 64, 16, torch.float16, seed=47)
+    rows = pool.keys.clone(), pool.values.clone()
+    states = [eviction_state(mix, 2, pool.columns * 16, 48 + i) for i, mix in enumerate(mixes)]
+    weights, positions, n, seen = states[0][0].clone(), states[0][1].clone(), ints(mixes[0]), ints(states[0][2])
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = evict_tokens(pool.keys, pool.values, pool.table, n, weights, positions, seen, budget, sink=2, recent=20)
+    for mix, (w, p, s) in zip(mixes[::-1], states[::-1]):
+        want_keys, want_values = rows[0].clone(), rows[1].clone()
+        want = evict_tokens(want_keys, want_values, pool.table, ints(mix), w, p, ints(s), budget, sink=2, recent=20)
+        pool.keys.copy_(rows[0]), pool.values.copy_(rows[1]), weights.copy_(w), positions.copy_(p), n.copy_(ints(mix)), seen.copy_(ints(s))
+        graph.replay()
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+        assert torch.equal(pool.keys.view(torch.int16), want_keys.view(torch.int16)) and torch.equal(pool.values.view(torch.int16), want_values.view(torch.int16))
+
+
+def test_two_streams_at_once():
+    """Decode and eviction of two caches, each on a stream of its own, over and over."""
+    from inquant.dense_paged import evict_tokens, paged_attention
+    pools = [Pool([4000, 900], 4, 128, 16, torch.bfloat16, seed=s) for s in (50, 51)]
+    q = query(2, 28, 128, torch.bfloat16)
+    width = pools[0].columns * 16
+    states = [eviction_state([4000, 900], 4, width, s) for s in (52, 53)]
+
+    def step(pool, state):
+        keys, values = pool.keys.clone(), pool.values.clone()
+        out, w = paged_attention(q, keys, values, pool.table, pool.n, weights=state[0], out_weights=torch.zeros_like(state[0]))
+        left = evict_tokens(keys, values, pool.table, pool.n, w, state[1], ints(state[2]), 700, sink=4, recent=64)
+        return out, w, *left, keys.view(torch.int16), values.view(torch.int16)
+
+    want = [step(*both) for both in zip(pools, states)]
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream() for _ in pools], [[], []]
+    for _ in range(8):
+        for i, both in enumerate(zip(pools, states)):
+            with torch.cuda.stream(streams[i]):
+                got[i].append(step(*both))
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert all(torch.equal(a, b) for each in got[i] for a, b in zip(each, want[i]))
