@@ -13,7 +13,7 @@
 // mma.sync suffices: per 512 bytes of a token it computes 8192 operations, a tenth of what the SM could do meanwhile.
 // The parts of a pair that ranges cut are joined, in their order, by the CTA that hands in the last one, or by a launch.
 // 131072 tokens of one request, 4 KV heads: 51 us, of them 45 of streaming (5.9 TB/s); 64 requests of up to 8192 tokens, 8 KV
-// heads, 159 us (6.0 TB/s); 700 tokens 10.5 us, launch and four dependent trips to memory.
+// heads, 156 to 162 us (5.9 TB/s); 700 tokens 8.9 us, launch and four dependent trips to memory (11 with the host's call).
 //
 // Where weights are asked for, a further launch turns the logits that the first one left into them:
 // out_w_j = w_j + sum_g 2^(s_gj - lse_g).

@@ -352,9 +352,10 @@ extern "C" int inq_evict_tokens(const inq_evict_args_t* a, inq_stream_t stream_)
   const long long slice = (P.capacity + ctas - 1) / ctas;
   // As many tokens move as places fall free, at most, and as there are behind the budget.  Where the rows fill the SMs and two
   // CTAs fit on one, few moves are done at once, beside the selection of other rows (256 rows of 2304 tokens, 256 of them
-  // evicted: 24.7 us against 26.8; 512 rows of 1024, a half evicted: 48.6 against 50.9).  Else they take a launch of their own,
-  // over all SMs (256 rows of 4096, one CTA per SM: 46 us against 49.5; 16 of 32768 to 8192: 42.6 against 54).  Other
-  // heads may still read a length when one writes it, so that it is not written in place.
+  // evicted: 24.7 us in a graph against 26.8; 512 rows of 1024, a half evicted: 48.6 against 50.9).  Else they take a launch
+  // of their own, over all SMs (256 rows of 4096, one CTA per SM: 46 us against 49.5; 16 of 32768 to 8192: 42.6 against 54).
+  // Rows are as long here as the table and `columns` allow, since the lengths are on the device: 256 rows of 2304 tokens
+  // take 48 us with a table of 32768.  Other heads may still read a length when one writes it, so that it is not written in place.
   const long long most = std::min<long long>(P.budget, std::max<long long>(P.capacity - P.budget, 1));
   P.moves_here = slice <= 5 * kEvThreads && rows * ctas > n_sm && most <= 4LL * ctas * (kEvThreads / 32) * kEvMoveEach && P.out_lengths != P.lengths;
   cudaStream_t stream = (cudaStream_t)stream_;
