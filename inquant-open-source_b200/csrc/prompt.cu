@@ -17,13 +17,13 @@
 //     only later queries see are set to zero and put back, by position, into the rows that do see them.
 // A step (two tiles, 128 keys) takes about 3700 cycles against 2048 of the tensor core and of the exponential unit alike:
 // the chain S -> P -> S of a tile bounds it, and beyond 1.06 PFLOP/s the power cap.  Back to back, at the clock that the cap
-// leaves, 8192 tokens of 28 heads take 450 to 463 us and 16 prompts of 16 to 2000 tokens of 32 heads 364 to 378 (in bursts too
+// leaves, 8192 tokens of 28 heads take 450 to 463 us and 16 prompts of 16 to 2000 tokens of 32 heads 364 to 380 (in bursts too
 // short for the cap 390 to 400 and 320 to 330); 301 tokens of 28 heads 12.5.
 //
 // prompt_weights_kernel.  w_j = sum over the group's heads and the last `window` queries of 2^(s_ij - lse_i).  The
 // contraction is transposed, S^T = K Q^T: two threads own a KEY row and add over columns, so that no atomics order a
 // sum.  4096 tokens of 28 heads 82 to 84 us, 54 of them exponentials; 8 requests of 900 to 16000 tokens of 32 heads, judged
-// by their last 64 queries, 55 to 64 us (the clock), 24 of them memory.
+// by their last 64 queries, 55 to 65 us (the clock), 24 of them memory.
 #include <algorithm>
 
 #include "attention.cuh"
